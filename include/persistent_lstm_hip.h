@@ -221,6 +221,84 @@ int plh_repeat_first_row(const void* in, void* out, int rows, int cols, void* st
  */
 int plh_probe_mfma_f16(double* tflops, double* clock_ghz);
 
+/*
+ * Operators of a residual block around a recurrence that is parallel over time, y = x + dropout(W_o scan(W_g norm(x))),
+ * for training and serving.  No counterpart in the reference, whose recurrence is the LSTM's alone.
+ *   - dtype names the element type of the activations (PLH_F16, PLH_BF16, PLH_F32); sums, statistics and states are
+ *     fp32, rounded once where an activation is written.
+ *   - Pointers need the alignment of their elements only; strides are in elements.  Kernels move 16, 8, 4 or 2 bytes
+ *     per lane, the widest that the pointers, the strides and the row length allow.
+ *   - Asynchronous on `stream`; no atomics, so that results are the same from call to call.  All can be captured in a
+ *     HIP graph.
+ */
+#define PLH_F16 0
+#define PLH_BF16 1
+#define PLH_F32 2
+
+/*
+ * Gated linear recurrence over gates [batch][seq_len][parts * hidden], parts = 3 with an output gate (f, g, o), 2
+ * without (f, g):
+ *     a_t = sigmoid(f_t)   c_t = a_t c_{t-1} + (1 - a_t) g_t   out_t = sigmoid(o_t) c_t, or c_t
+ *   gates     element (b, t, k) at b * stride_b + t * stride_t + k
+ *   lengths   device int32 [batch] or NULL (every row runs seq_len steps): row b runs min(max(lengths[b], 0), seq_len)
+ *             steps, its c stays as it is after them and its out is zero there.  What gates hold there is not read.
+ *   c0        device fp32 [batch][hidden] or NULL for zeros
+ *   out       [batch][seq_len][hidden], contiguous
+ *   c_n       device fp32 [batch][hidden] or NULL: c after the last step
+ *   states    device fp32 [plh_gated_scan_states(seq_len)][batch][hidden] or NULL: what the backward pass needs
+ *   workspace device memory of plh_gated_scan_workspace_bytes(...) bytes (0 for many channels), 16-byte aligned,
+ *             used until the call's work on `stream` is done; nothing is kept in it
+ * seq_len = 1 is the step of a serving loop; c_n may then be c0 (in place).
+ * Limits: hidden <= 2^24, batch * hidden <= 2^29, seq_len <= 2^30.
+ */
+int64_t plh_gated_scan_states(int64_t seq_len);
+int64_t plh_gated_scan_workspace_bytes(int64_t batch, int64_t seq_len, int hidden);
+int plh_gated_scan_forward(int dtype, int output_gate, const void* gates, int64_t stride_b, int64_t stride_t,
+                           int64_t batch, int64_t seq_len, int hidden, const int32_t* lengths, const float* c0,
+                           void* out, float* c_n, float* states, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+/*
+ * Its gradient: d_gates [batch][seq_len][parts * hidden] (contiguous; zero past a row's length) and d_c0 [batch][hidden]
+ * (fp32, or NULL) from d_out [batch][seq_len][hidden] (contiguous; not read past a row's length) and d_cn (fp32
+ * [batch][hidden], or NULL for zeros).  gates, lengths and states as in the forward call that wrote states.
+ */
+int plh_gated_scan_backward(int dtype, int output_gate, const void* gates, int64_t stride_b, int64_t stride_t,
+                            int64_t batch, int64_t seq_len, int hidden, const int32_t* lengths, const float* states,
+                            const void* d_out, const float* d_cn, void* d_gates, float* d_c0, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/*
+ * Layer norm over the last dimension of x [rows][cols] (row r at r * stride):
+ *     y = (x - mean) * rstd * weight + bias,   rstd = 1 / sqrt(variance + eps), the variance over cols elements
+ *   weight, bias  [cols] of wdtype (PLH_F32 or dtype), either may be NULL (1 and 0)
+ *   y             [rows][cols], contiguous
+ *   mean, rstd    device fp32 [rows] or NULL: what the backward pass needs
+ * Limits: cols <= 2^24.
+ */
+int plh_layer_norm_forward(int dtype, int wdtype, const void* x, int64_t stride, int64_t rows, int64_t cols,
+                           const void* weight, const void* bias, float eps, void* y, float* mean, float* rstd,
+                           void* stream);
+/*
+ * Its gradient: d_x [rows][cols] (contiguous), d_weight and d_bias [cols] of wdtype, each of the three or NULL.
+ * d_y [rows][cols] contiguous.  workspace as above, of plh_layer_norm_workspace_bytes(...) bytes.
+ */
+int64_t plh_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+int plh_layer_norm_backward(int dtype, int wdtype, const void* x, int64_t stride, int64_t rows, int64_t cols,
+                            const void* weight, const float* mean, const float* rstd, const void* d_y, void* d_x,
+                            void* d_weight, void* d_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * out[e] = residual[e] + (keep(e) ? x[e] * 65536 / (65536 - threshold) : 0) for e < n (residual NULL: 0).  keep(e) is
+ * r(e) >= threshold, 0 <= threshold <= 65536: an element is dropped with probability threshold / 65536, and then it
+ * is not read into the result, infinity and NaN included.  r(e) are 16 bits of Philox4x32-10 with the key `seed` and
+ * the counter (e / 8, offset), 64 bits each: the low (e even) or high half of output word (e % 8) / 2.  So a mask is
+ * a function of (seed, offset, e) alone, needs no storage, and the gradient is the same call with d_out for x and no
+ * residual.  offset_dev: NULL, or a device int64 that is added to `offset` when the kernel runs (a captured graph's
+ * replays then get masks of their own).
+ */
+int plh_dropout_add(int dtype, const void* x, const void* residual, void* out, int64_t n, int threshold, uint64_t seed,
+                    uint64_t offset, const int64_t* offset_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

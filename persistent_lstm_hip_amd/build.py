@@ -11,6 +11,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -19,8 +21,8 @@ LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpersistent_lstm_hip.so")
 BENCH_PATH = os.path.join(LIB_DIR, "plh_bench")
 SOURCES = ["plh_wavefront.hip", "plh_sliced.hip", "plh_rec.hip", "plh_gemm.hip", "plh_pack.hip", "plh_launch.hip",
-           "plh_probe.hip", "plh_capi.hip"]
-HEADERS = ["plh_internal.h", os.path.join("..", "..", "include", "persistent_lstm_hip.h")]
+           "plh_probe.hip", "plh_capi.hip", "plh_scan.hip", "plh_norm.hip", "plh_dropout.hip"]
+HEADERS = ["plh_internal.h", "plh_device.h", "plh_ops.h", os.path.join("..", "..", "include", "persistent_lstm_hip.h")]
 
 ARCH = "gfx950"
 HIPCC_FLAGS = [
@@ -28,7 +30,6 @@ HIPCC_FLAGS = [
     "-std=c++17",
     f"--offload-arch={ARCH}",
     "-fPIC",
-    "-shared",
     # Keep packed-FP32 VALU ops out of the generated code (v_pk_{add,mul,fma}_f32).
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",
@@ -49,15 +50,25 @@ def build(verbose: bool = False) -> str:
     """Compile every source for gfx950 and link the shared library.  Always recompiles."""
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
-    cmd = [hipcc()] + HIPCC_FLAGS + [os.path.join(CSRC, s) for s in SOURCES] + LINK_FLAGS + ["-o", tmp]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    out = "\n".join(l for l in proc.stdout.splitlines() if "packed-fp32-ops" not in l)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{out}")
-    if verbose and out.strip():
-        print(out)
+
+    def run(cmd: list) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        out = "\n".join(l for l in proc.stdout.splitlines() if "packed-fp32-ops" not in l)
+        if proc.returncode != 0:
+            raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{out}")
+        if verbose and out.strip():
+            print(out, flush=True)
+
+    def compile_one(source: str, objects: str) -> str:
+        obj = os.path.join(objects, source + ".o")
+        run([hipcc()] + HIPCC_FLAGS + ["-c", os.path.join(CSRC, source), "-o", obj])
+        return obj
+
+    with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(4) as pool:
+        objs = list(pool.map(lambda s: compile_one(s, objects), SOURCES))
+        run([hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}"] + objs + LINK_FLAGS + ["-o", tmp])
     os.replace(tmp, LIB_PATH)
     # Native driver of the C ABI (profiling target and integration example), linked to the library.
     # (plh_issue_probe.hip: a developer probe kernel of plh_bench --issue, not part of the library.)

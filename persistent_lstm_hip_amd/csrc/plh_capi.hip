@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "plh_internal.h"
+#include "plh_ops.h"
 #include "../../include/persistent_lstm_hip.h"
 
 namespace {
@@ -30,6 +31,25 @@ int fail(int code, const std::string& msg) {
 int fail_hip(hipError_t e, const char* what) {
   return fail(PLH_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
+
+}  // namespace
+
+namespace plh {
+
+int op_error(int code, const char* what, const char* msg) noexcept {
+  try {
+    g_last_error.assign(what).append(": ").append(msg);
+  } catch (...) {  // no memory for the message: the code still says what happened
+    g_last_error.clear();
+  }
+  return code;
+}
+
+int op_error(hipError_t e, const char* what) noexcept { return op_error(PLH_ERR_HIP, what, hipGetErrorString(e)); }
+
+}  // namespace plh
+
+namespace {
 
 // Co-resident workgroup capacity per device and set of kernel variants (plh::capacity_key), queried once.
 std::mutex g_cap_mu;

@@ -83,6 +83,24 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.plh_probe_mfma_f16.argtypes = [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]
     lib.plh_input_projection.restype = _i32
     lib.plh_input_projection.argtypes = [_vp, _i64, _vp, _i32, _vp, _i64, _i64, _i32, _i32, _vp]
+    lib.plh_gated_scan_states.restype = _i64
+    lib.plh_gated_scan_states.argtypes = [_i64]
+    lib.plh_gated_scan_workspace_bytes.restype = _i64
+    lib.plh_gated_scan_workspace_bytes.argtypes = [_i64, _i64, _i32]
+    scan = [_i32, _i32, _vp, _i64, _i64, _i64, _i64, _i32, _vp]
+    lib.plh_gated_scan_forward.restype = _i32
+    lib.plh_gated_scan_forward.argtypes = scan + [_vp, _vp, _vp, _vp, _vp, _i64, _vp]
+    lib.plh_gated_scan_backward.restype = _i32
+    lib.plh_gated_scan_backward.argtypes = scan + [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
+    norm = [_i32, _i32, _vp, _i64, _i64, _i64, _vp]
+    lib.plh_layer_norm_forward.restype = _i32
+    lib.plh_layer_norm_forward.argtypes = norm + [_vp, ctypes.c_float, _vp, _vp, _vp, _vp]
+    lib.plh_layer_norm_workspace_bytes.restype = _i64
+    lib.plh_layer_norm_workspace_bytes.argtypes = [_i64, _i64]
+    lib.plh_layer_norm_backward.restype = _i32
+    lib.plh_layer_norm_backward.argtypes = norm + [_vp] * 7 + [_i64, _vp]
+    lib.plh_dropout_add.restype = _i32
+    lib.plh_dropout_add.argtypes = [_i32, _vp, _vp, _vp, _i64, _i32, ctypes.c_uint64, ctypes.c_uint64, _vp, _vp]
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
