@@ -38,10 +38,21 @@ constexpr float kOpLog2e = 1.4426950408889634f;
 // The logistic function and its complement, s = 1 / (1 + e) and 1 - s = e s with e = 2^min(-z log2 e, 126): the
 // complement keeps its relative precision where s is close to 1, and the cap keeps e s from being inf * 0 (it moves s
 // by less than 2^-126).  The minimum returns NaN for a NaN argument.
-__device__ __forceinline__ void logistic(float z, float& s, float& not_s) {
+__device__ __forceinline__ void logistic_fast(float z, float& s, float& not_s) {
   const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(z * -kOpLog2e, 126.0f));
   s = __builtin_amdgcn_rcpf(1.0f + e);
   not_s = e * s;
+}
+// The same for values that are multiplied with each other many times over: v_rcp_f32 alone is off by up to one unit
+// in the last place, one step of Newton's iteration rounds it.
+__device__ __forceinline__ void logistic(float z, float& s, float& not_s) {
+  const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(z * -kOpLog2e, 126.0f));
+  const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d);
+  s = fmaf(fmaf(-d, r, 1.0f), r, r);
+  not_s = e * s;
+}
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -kOpLog2e));
 }
 
 template <typename T>

@@ -28,7 +28,7 @@ constexpr int kSlab = 64;
 constexpr int kTile = 64;
 
 // Workgroups that a launch should have at least: with fewer slabs than that the time axis is split into segments.
-constexpr int kScanGroups = 2048;
+constexpr int kScanGroups = 512;
 
 struct Split {
   int tiles;      // tiles of a row
@@ -83,7 +83,8 @@ struct Place {
   template <typename T>
   __device__ __forceinline__ Place(const ScanArgs<T>& p, unsigned slab) {
     const int tid = threadIdx.x;
-    lane = tid % kWave, wave = tid / kWave, ct = tid % CT, tg = tid / CT;
+    lane = tid % kWave, ct = tid % CT, tg = tid / CT;
+    wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     n = (int64_t)slab * kSlab + ct * VEC;
     on = n < p.channels;
     b = 0, h = 0, len = 0;
@@ -101,60 +102,104 @@ struct Place {
   }
 };
 
-// The maps of the time groups, composed: on entry A, B are a thread's own map (FORWARD: of its steps in order,
-// else in reverse order); on return the map of everything in this wave that comes before this thread's steps, with the
-// whole wave's map in LDS at [wave][channel] for the caller to fold after a barrier.
-template <int VEC, bool FORWARD>
-__device__ __forceinline__ void wave_maps(const Place<VEC>& at, float (&A)[VEC], float (&B)[VEC],
-                                          float (*lds_a)[kSlab], float (*lds_b)[kSlab]) {
-  constexpr int CT = Place<VEC>::CT;
+// v of the even and of the odd time group of a pair of groups, in both (one exchange per level and value).
+template <int VEC, int LEVEL>
+__device__ __forceinline__ void pair_of(float v, float& even, float& odd) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  uint32_t lo, hi;
+  if constexpr (VEC == 4 && LEVEL == 0) {  // groups of 16 lanes: neighbouring rows
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    lo = r[0], hi = r[1];
+  } else {  // halves of the wave
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    lo = r[0], hi = r[1];
+  }
+  even = __builtin_bit_cast(float, lo), odd = __builtin_bit_cast(float, hi);
+}
+
+// The maps of the time groups of a wave, composed.  In: a thread's own factor A and its own sums B[k] (k = 0: of its
+// steps in order; k = 1: in reverse order, SUMS = 2 only).  Out: pa[k], pb[k], the map of everything in this wave
+// that comes before the thread's steps in direction k (REVERSE0: direction 0 is reverse order too); A and B become the
+// wave's own.
+template <int VEC, int SUMS, bool REVERSE0>
+__device__ __forceinline__ void wave_maps(int lane, float (&A)[VEC], float (&B)[SUMS][VEC], float (&pa)[SUMS][VEC],
+                                          float (&pb)[SUMS][VEC]) {
+  constexpr int kLevels = VEC == 4 ? 2 : VEC == 2 ? 1 : 0;
 #pragma unroll
-  for (int d = CT; d < kWave; d *= 2) {
-    const bool has = FORWARD ? at.lane >= d : at.lane < kWave - d;
+  for (int k = 0; k < SUMS; ++k)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) pa[k][j] = 1.0f, pb[k][j] = 0.0f;
+  const auto level = [&](auto lv) {
+    constexpr int L = decltype(lv)::value;
+    const bool odd = (lane & (VEC == 4 && L == 0 ? 16 : 32)) != 0;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const float pa = FORWARD ? __shfl_up(A[j], d) : __shfl_down(A[j], d);
-      const float pb = FORWARD ? __shfl_up(B[j], d) : __shfl_down(B[j], d);
-      if (has) {
-        B[j] = fmaf(A[j], pb, B[j]);
-        A[j] *= pa;
+      float a0, a1;
+      pair_of<VEC, L>(A[j], a0, a1);
+#pragma unroll
+      for (int k = 0; k < SUMS; ++k) {
+        const bool rev = REVERSE0 || k == 1;
+        float b0, b1;
+        pair_of<VEC, L>(B[k][j], b0, b1);
+        // the other group of the pair comes first for the odd one in order, for the even one in reverse
+        const float fa = rev ? a1 : a0, fb = rev ? b1 : b0, sa = rev ? a0 : a1, sb = rev ? b0 : b1;
+        if (odd != rev) {
+          pb[k][j] = fmaf(pa[k][j], fb, pb[k][j]);
+          pa[k][j] *= fa;
+        }
+        B[k][j] = fmaf(sa, fb, sb);
       }
+      A[j] = a0 * a1;
     }
-  }
-  const bool whole = FORWARD ? at.lane >= kWave - CT : at.lane < CT;
-  if (whole) {
+  };
+  if constexpr (kLevels >= 1) level(std::integral_constant<int, 0>());
+  if constexpr (kLevels >= 2) level(std::integral_constant<int, 1>());
+}
+
+// The four waves' maps in LDS: [parity of the tile][wave][A, sums...][channel].  Two halves in turn need one barrier
+// per tile: the half written next was last read before the barrier in between.
+template <int SUMS>
+using WaveMaps = float[2][kScanThreads / kWave][1 + SUMS][kSlab];
+
+template <int VEC, int SUMS>
+__device__ __forceinline__ void put_maps(const Place<VEC>& at, float (&lds)[kScanThreads / kWave][1 + SUMS][kSlab],
+                                         const float (&A)[VEC], const float (&B)[SUMS][VEC]) {
+  if (at.lane < Place<VEC>::CT) {
+    Vec<float, VEC> v;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      lds_a[at.wave][at.ct * VEC + j] = A[j];
-      lds_b[at.wave][at.ct * VEC + j] = B[j];
+    for (int j = 0; j < VEC; ++j) v.v[j] = A[j];
+    store_vec(&lds[at.wave][0][at.ct * VEC], v);
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v.v[j] = B[k][j];
+      store_vec(&lds[at.wave][1 + k][at.ct * VEC], v);
     }
-  }
-  const bool first = FORWARD ? at.lane < CT : at.lane >= kWave - CT;
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    const float pa = FORWARD ? __shfl_up(A[j], CT) : __shfl_down(A[j], CT);
-    const float pb = FORWARD ? __shfl_up(B[j], CT) : __shfl_down(B[j], CT);
-    A[j] = first ? 1.0f : pa;
-    B[j] = first ? 0.0f : pb;
   }
 }
 
-// The carry through the four waves' maps: `carry` becomes the value after the whole tile, and the return in `mine` is
-// the value that this thread's steps start from.  (A, B) is the thread's map from wave_maps.
-template <int VEC, bool FORWARD>
-__device__ __forceinline__ void fold_waves(const Place<VEC>& at, const float (&A)[VEC], const float (&B)[VEC],
-                                           const float (*lds_a)[kSlab], const float (*lds_b)[kSlab],
-                                           float (&carry)[VEC], float (&mine)[VEC]) {
+// The carry through the four waves' maps: `carry` becomes the value after the whole tile, `mine` the value that this
+// thread's steps start from; (pa, pb) is the thread's map from wave_maps.
+template <int VEC, int SUMS, int K, bool REVERSE>
+__device__ __forceinline__ void fold_waves(const Place<VEC>& at, const float (&lds)[kScanThreads / kWave][1 + SUMS][kSlab],
+                                           const float (&pa)[VEC], const float (&pb)[VEC], float (&carry)[VEC],
+                                           float (&mine)[VEC]) {
   constexpr int W = kScanThreads / kWave;
+  float before[VEC];
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    const int w = FORWARD ? i : W - 1 - i;
+    const int w = REVERSE ? W - 1 - i : i;
+    if (w == at.wave) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (w == at.wave) mine[j] = fmaf(A[j], carry[j], B[j]);
-      carry[j] = fmaf(lds_a[w][at.ct * VEC + j], carry[j], lds_b[w][at.ct * VEC + j]);
+      for (int j = 0; j < VEC; ++j) before[j] = carry[j];
     }
+    const Vec<float, VEC> a = load_vec<float, VEC>(&lds[w][0][at.ct * VEC]);
+    const Vec<float, VEC> b = load_vec<float, VEC>(&lds[w][1 + K][at.ct * VEC]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) carry[j] = fmaf(a.v[j], carry[j], b.v[j]);
   }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) mine[j] = fmaf(pa[j], before[j], pb[j]);
 }
 
 // The carry at a segment's start: the maps of the segments before it, in order, applied to `carry`.
@@ -170,107 +215,151 @@ __device__ __forceinline__ void fold_segments(const ScanArgs<T>& p, const Place<
   }
 }
 
+// A thread's rows of a tile.  Steps past the row's length hold f = +inf, so that a = 1 and 1 - a = 0 without a test,
+// and zeros.
+template <typename T, int VEC, bool G, bool O, bool D>
+struct Rows {
+  static constexpr int R = Place<VEC>::R;
+  Vec<T, VEC> f[R], g[R], o[R], d[R];
+
+  __device__ __forceinline__ void load(const ScanArgs<T>& p, const Place<VEC>& at, int tile) {
+    const int t0 = tile * kTile + at.tg * R;
+    const T* src = p.gates + at.b * p.stride_b + (int64_t)t0 * p.stride_t + at.h;
+    const T* grad = D ? p.d_out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h : nullptr;
+    const auto row = [&](int r) {
+      f[r] = load_vec<T, VEC>(src);
+      if (G) g[r] = load_vec<T, VEC>(src + p.H);
+      if (O) o[r] = load_vec<T, VEC>(src + 2 * p.H);
+      if (D) d[r] = load_vec<T, VEC>(grad);
+    };
+    if (__all(t0 + R <= at.len)) {  // (the usual case: no branch per row)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        row(r);
+        src += p.stride_t;
+        if (D) grad += p.H;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          f[r].v[j] = (T)__builtin_inff();
+          if (G) g[r].v[j] = (T)0.0f;
+          if (O) o[r].v[j] = (T)0.0f;
+          if (D) d[r].v[j] = (T)0.0f;
+        }
+        if (t0 + r < at.len) row(r);
+        src += p.stride_t;
+        if (D) grad += p.H;
+      }
+    }
+  }
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ Vec<T, VEC> zero_unless(bool live, const Vec<T, VEC>& v) {
+  Vec<T, VEC> z;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) z.v[j] = live ? v.v[j] : (T)0.0f;
+  return z;
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_carry(const float* src, const Place<VEC>& at, float (&c)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) c[j] = 0.0f;
+  if (!src || !at.on) return;
+  const Vec<float, VEC> v = load_vec<float, VEC>(src + at.n);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) c[j] = v.v[j];
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_carry(float* dst, const Place<VEC>& at, const float (&c)[VEC]) {
+  Vec<float, VEC> v;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) v.v[j] = c[j];
+  store_vec(dst + at.n, v);
+}
+
 // Forward.  MAPS: only the segments' maps (of all but the last), for the launch that follows.
 template <typename T, int VEC, bool GATED, bool MAPS>
 __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs<T> p) {
   using P = Place<VEC>;
   constexpr int R = P::R;
-  __shared__ float lds_a[2][4][kSlab], lds_b[2][4][kSlab];
+  __shared__ WaveMaps<1> lds;
   const unsigned slab = blockIdx.x % p.slabs;
   const int seg = blockIdx.x / p.slabs;
   const P at(p, slab);
   float carry[VEC], prod[VEC];
+  load_carry<VEC>(MAPS ? nullptr : p.c0, at, carry);
+  if (!MAPS) fold_segments<T, VEC>(p, at, 0, seg, 1, carry);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) carry[j] = 0.0f, prod[j] = 1.0f;
-  if (!MAPS && at.on) {
-    if (p.c0) {
-      const Vec<float, VEC> c = load_vec<float, VEC>(p.c0 + at.n);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) carry[j] = c.v[j];
-    }
-    fold_segments<T, VEC>(p, at, 0, seg, 1, carry);
-  }
+  for (int j = 0; j < VEC; ++j) prod[j] = 1.0f;
   const int tile_end = min(p.tiles, (seg + 1) * p.seg_tiles);
-  const T* const row = p.gates + at.b * p.stride_b + at.h;
-  for (int tile = seg * p.seg_tiles; tile < tile_end; ++tile) {
+  Rows<T, VEC, true, GATED && !MAPS, false> x, next;
+  int tile = seg * p.seg_tiles;
+  if (tile < tile_end) next.load(p, at, tile);
+  for (; tile < tile_end; ++tile) {
+    x = next;
+    if (tile + 1 < tile_end) next.load(p, at, tile + 1);
     const int t0 = tile * kTile + at.tg * R;
-    Vec<T, VEC> f[R] = {}, g[R] = {}, o[R] = {};
+    float a[R][VEC], b[R][VEC], A[VEC], B[1][VEC], pa[1][VEC], pb[1][VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (t0 + r < at.len) {
-        const T* src = row + (int64_t)(t0 + r) * p.stride_t;
-        f[r] = load_vec<T, VEC>(src);
-        g[r] = load_vec<T, VEC>(src + p.H);
-        if (GATED && !MAPS) o[r] = load_vec<T, VEC>(src + 2 * p.H);
-      }
-    }
-    float a[R][VEC], b[R][VEC], A[VEC], B[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[j] = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const bool live = t0 + r < at.len;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        float s = 1.0f, ns = 0.0f, in = 0.0f;
-        if (live) {
-          logistic((float)f[r].v[j], s, ns);
-          in = ns * (float)g[r].v[j];
-        }
-        a[r][j] = s, b[r][j] = in;
-        B[j] = fmaf(s, B[j], in);
-        A[j] *= s;
+        float ns;
+        logistic((float)x.f[r].v[j], a[r][j], ns);
+        b[r][j] = ns * (float)x.g[r].v[j];
+        B[0][j] = fmaf(a[r][j], B[0][j], b[r][j]);
+        A[j] *= a[r][j];
       }
     }
-    float(*la)[kSlab] = lds_a[tile & 1];
-    float(*lb)[kSlab] = lds_b[tile & 1];
-    wave_maps<VEC, true>(at, A, B, la, lb);
-    __syncthreads();  // (the other half of the buffers is written next, so one barrier per tile is enough)
-    if (!MAPS && p.states && at.on && at.tg == 0) {
-      Vec<float, VEC> c;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) c.v[j] = carry[j];
-      store_vec(p.states + (int64_t)tile * p.channels + at.n, c);
-    }
-    float c[VEC];
+    wave_maps<VEC, 1, false>(at.lane, A, B, pa, pb);
+    auto& maps = lds[tile & 1];
+    put_maps<VEC, 1>(at, maps, A, B);
+    __syncthreads();
     if (MAPS) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
+      for (int w = 0; w < kScanThreads / kWave; ++w)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) prod[j] *= la[w][at.ct * VEC + j];
+        for (int j = 0; j < VEC; ++j) prod[j] *= maps[w][0][at.ct * VEC + j];
+    } else if (p.states && at.on && at.tg == 0) {
+      store_carry<VEC>(p.states + (int64_t)tile * p.channels, at, carry);
     }
-    fold_waves<VEC, true>(at, A, B, la, lb, carry, c);
+    float c[VEC];
+    fold_waves<VEC, 1, 0, false>(at, maps, pa[0], pb[0], carry, c);
     if (!MAPS && at.on) {
       T* dst = p.out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h;
+      Vec<T, VEC> y[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        if (t0 + r < p.T_) {
-          Vec<T, VEC> y;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            c[j] = fmaf(a[r][j], c[j], b[r][j]);
-            float h = c[j];
-            if (GATED) {
-              float s, ns;
-              logistic((float)o[r].v[j], s, ns);
-              h *= s;
-            }
-            y.v[j] = (T)(t0 + r < at.len ? h : 0.0f);
-          }
-          store_vec(dst + (int64_t)r * p.H, y);
+        for (int j = 0; j < VEC; ++j) {
+          c[j] = fmaf(a[r][j], c[j], b[r][j]);
+          y[r].v[j] = (T)(GATED ? c[j] * sigmoid((float)x.o[r].v[j]) : c[j]);
         }
+      }
+      if (__all(t0 + R <= at.len)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) store_vec(dst + (int64_t)r * p.H, y[r]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (t0 + r < p.T_) store_vec(dst + (int64_t)r * p.H, zero_unless(t0 + r < at.len, y[r]));
       }
     }
   }
   if (at.on && at.tg == 0) {
-    Vec<float, VEC> va, vb;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) va.v[j] = prod[j], vb.v[j] = carry[j];
     if (MAPS) {
-      store_vec(p.seg_a + (int64_t)seg * p.channels + at.n, va);
-      store_vec(p.seg_b + (int64_t)seg * p.channels + at.n, vb);
+      store_carry<VEC>(p.seg_a + (int64_t)seg * p.channels, at, prod);
+      store_carry<VEC>(p.seg_b + (int64_t)seg * p.channels, at, carry);
     } else if (seg == p.segs - 1 && p.c_n) {
-      store_vec(p.c_n + at.n, vb);
+      store_carry<VEC>(p.c_n, at, carry);
     }
   }
 }
@@ -281,140 +370,121 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs<T>
   using P = Place<VEC>;
   constexpr int R = P::R;
   constexpr int kParts = GATED ? 3 : 2;
-  __shared__ float lds_a[2][4][kSlab], lds_b[2][4][kSlab], lds_fa[2][4][kSlab], lds_fb[2][4][kSlab];
+  constexpr int kSums = MAPS ? 1 : 2;  // the sums in reverse order; else first those in order, for c
+  constexpr int kRev = kSums - 1;
+  __shared__ WaveMaps<kSums> lds;
   const unsigned slab = blockIdx.x % p.slabs;
   const int seg = blockIdx.x / p.slabs + (MAPS ? 1 : 0);
   const P at(p, slab);
   float carry[VEC], prod[VEC];
+  load_carry<VEC>(MAPS ? nullptr : p.d_cn, at, carry);
+  if (!MAPS) fold_segments<T, VEC>(p, at, p.segs - 1, seg, -1, carry);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) carry[j] = 0.0f, prod[j] = 1.0f;
-  if (!MAPS && at.on) {
-    if (p.d_cn) {
-      const Vec<float, VEC> c = load_vec<float, VEC>(p.d_cn + at.n);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) carry[j] = c.v[j];
-    }
-    fold_segments<T, VEC>(p, at, p.segs - 1, seg, -1, carry);
-  }
+  for (int j = 0; j < VEC; ++j) prod[j] = 1.0f;
   const int tile_first = seg * p.seg_tiles;
-  const T* const row = p.gates + at.b * p.stride_b + at.h;
-  for (int tile = min(p.tiles, (seg + 1) * p.seg_tiles) - 1; tile >= tile_first; --tile) {
-    const int t0 = tile * kTile + at.tg * R;
-    Vec<T, VEC> f[R] = {}, g[R] = {}, o[R] = {}, dh[R] = {};
-    const T* const d_row = p.d_out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h;
+  Rows<T, VEC, !MAPS, GATED, true> x, next;
+  float start[VEC], next_start[VEC];
+  int tile = min(p.tiles, (seg + 1) * p.seg_tiles) - 1;
+  if (tile >= tile_first) {
+    next.load(p, at, tile);
+    load_carry<VEC>(MAPS ? nullptr : p.states + (int64_t)tile * p.channels, at, next_start);
+  }
+  for (; tile >= tile_first; --tile) {
+    x = next;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (t0 + r < at.len) {
-        const T* src = row + (int64_t)(t0 + r) * p.stride_t;
-        f[r] = load_vec<T, VEC>(src);
-        if (!MAPS) g[r] = load_vec<T, VEC>(src + p.H);
-        if (GATED) o[r] = load_vec<T, VEC>(src + 2 * p.H);
-        dh[r] = load_vec<T, VEC>(d_row + (int64_t)r * p.H);
-      }
+    for (int j = 0; j < VEC; ++j) start[j] = next_start[j];
+    if (tile > tile_first) {
+      next.load(p, at, tile - 1);
+      load_carry<VEC>(MAPS ? nullptr : p.states + (int64_t)(tile - 1) * p.channels, at, next_start);
     }
-    float a[R][VEC], na[R][VEC], u[R][VEC], A[VEC], E[VEC], FA[VEC], FB[VEC];
+    const int t0 = tile * kTile + at.tg * R;
+    float a[R][VEC], na[R][VEC], u[R][VEC], w[R][VEC];  // a, 1 - a, u = s dh, w = (1 - s) u
+    float A[VEC], B[kSums][VEC], pa[kSums][VEC], pb[kSums][VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, E[j] = 0.0f, FB[j] = 0.0f;
+    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = B[kRev][j] = 0.0f;
 #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
-      const bool live = t0 + r < at.len;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        float s = 1.0f, ns = 0.0f, d = 0.0f;
-        if (live) {
-          logistic((float)f[r].v[j], s, ns);
-          d = (float)dh[r].v[j];
-          if (GATED) {
-            float so, nso;
-            logistic((float)o[r].v[j], so, nso);
-            d *= so;
-          }
+        logistic((float)x.f[r].v[j], a[r][j], na[r][j]);
+        u[r][j] = (float)x.d[r].v[j];
+        if (GATED) {
+          float s, ns;
+          logistic_fast((float)x.o[r].v[j], s, ns);
+          u[r][j] *= s;
+          w[r][j] = ns * u[r][j];
         }
-        a[r][j] = s, na[r][j] = ns, u[r][j] = d;
-        E[j] = s * (E[j] + d);
-        A[j] *= s;
+        B[kRev][j] = a[r][j] * (B[kRev][j] + u[r][j]);
+        A[j] *= a[r][j];
       }
     }
-    const int half = tile & 1;
     if (!MAPS) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float in = t0 + r < at.len ? na[r][j] * (float)g[r].v[j] : 0.0f;
-          FB[j] = fmaf(a[r][j], FB[j], in);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) FA[j] = A[j];
-      wave_maps<VEC, true>(at, FA, FB, lds_fa[half], lds_fb[half]);
+        for (int j = 0; j < VEC; ++j) B[0][j] = fmaf(a[r][j], B[0][j], na[r][j] * (float)x.g[r].v[j]);
     }
-    wave_maps<VEC, false>(at, A, E, lds_a[half], lds_b[half]);
-    __syncthreads();  // (as in the forward kernel)
+    wave_maps<VEC, kSums, MAPS>(at.lane, A, B, pa, pb);
+    auto& maps = lds[tile & 1];
+    put_maps<VEC, kSums>(at, maps, A, B);
+    __syncthreads();
     if (MAPS) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
+      for (int i = 0; i < kScanThreads / kWave; ++i)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) prod[j] *= lds_a[half][w][at.ct * VEC + j];
+        for (int j = 0; j < VEC; ++j) prod[j] *= maps[i][0][at.ct * VEC + j];
     }
     float e[VEC];
-    fold_waves<VEC, false>(at, A, E, lds_a[half], lds_b[half], carry, e);
+    fold_waves<VEC, kSums, kRev, true>(at, maps, pa[kRev], pb[kRev], carry, e);
     if (!MAPS && at.on) {
       // c before each of this thread's steps, from the state that the forward pass left at the tile's start
-      const Vec<float, VEC> st = load_vec<float, VEC>(p.states + (int64_t)tile * p.channels + at.n);
-      float start[VEC], c[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) start[j] = st.v[j];
-      fold_waves<VEC, true>(at, FA, FB, lds_fa[half], lds_fb[half], start, c);
-      float before[R][VEC];
+      float c[VEC], before[R][VEC];
+      fold_waves<VEC, kSums, 0, false>(at, maps, pa[0], pb[0], start, c);
+      Vec<T, VEC> df[R], dg[R], d_o[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           before[r][j] = c[j];
-          const float in = t0 + r < at.len ? na[r][j] * (float)g[r].v[j] : 0.0f;
-          c[j] = fmaf(a[r][j], c[j], in);
+          c[j] = fmaf(a[r][j], c[j], na[r][j] * (float)x.g[r].v[j]);
+          if (GATED) d_o[r].v[j] = (T)(w[r][j] * c[j]);
         }
       }
-      T* const dst = p.d_gates + (at.b * p.T_ + t0) * (int64_t)(kParts * p.H) + at.h;
 #pragma unroll
       for (int r = R - 1; r >= 0; --r) {
-        const bool live = t0 + r < at.len;
-        Vec<T, VEC> df, dg, d_o;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float D = u[r][j] + e[j];
+          const float n = na[r][j] * D;
           e[j] = a[r][j] * D;
-          df.v[j] = dg.v[j] = d_o.v[j] = (T)0.0f;
-          if (live) {
-            const float gv = (float)g[r].v[j];
-            dg.v[j] = (T)(na[r][j] * D);
-            df.v[j] = (T)(e[j] * na[r][j] * (before[r][j] - gv));
-            if (GATED) {
-              float so, nso;
-              logistic((float)o[r].v[j], so, nso);
-              d_o.v[j] = (T)(nso * u[r][j] * fmaf(a[r][j], before[r][j], na[r][j] * gv));
-            }
-          }
+          dg[r].v[j] = (T)n;
+          df[r].v[j] = (T)(a[r][j] * n * (before[r][j] - (float)x.g[r].v[j]));
         }
-        if (t0 + r < p.T_) {
-          T* q = dst + (int64_t)r * (kParts * p.H);
-          store_vec(q, df);
-          store_vec(q + p.H, dg);
-          if (GATED) store_vec(q + 2 * p.H, d_o);
+      }
+      T* const dst = p.d_gates + (at.b * p.T_ + t0) * (int64_t)(kParts * p.H) + at.h;
+      const bool all = __all(t0 + R <= at.len);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        T* const q = dst + (int64_t)r * (kParts * p.H);
+        if (all) {
+          store_vec(q, df[r]);
+          store_vec(q + p.H, dg[r]);
+          if (GATED) store_vec(q + 2 * p.H, d_o[r]);
+        } else if (t0 + r < p.T_) {
+          const bool live = t0 + r < at.len;
+          store_vec(q, zero_unless(live, df[r]));
+          store_vec(q + p.H, zero_unless(live, dg[r]));
+          if (GATED) store_vec(q + 2 * p.H, zero_unless(live, d_o[r]));
         }
       }
     }
   }
   if (at.on && at.tg == 0) {
-    Vec<float, VEC> va, vb;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) va.v[j] = prod[j], vb.v[j] = carry[j];
     if (MAPS) {
-      store_vec(p.seg_a + (int64_t)seg * p.channels + at.n, va);
-      store_vec(p.seg_b + (int64_t)seg * p.channels + at.n, vb);
+      store_carry<VEC>(p.seg_a + (int64_t)seg * p.channels, at, prod);
+      store_carry<VEC>(p.seg_b + (int64_t)seg * p.channels, at, carry);
     } else if (seg == 0 && p.d_c0) {
-      store_vec(p.d_c0 + at.n, vb);
+      store_carry<VEC>(p.d_c0, at, carry);
     }
   }
 }
