@@ -2,8 +2,9 @@
 
     python -m persistent_lstm_hip_amd.build        # -> persistent_lstm_hip_amd/lib/libpersistent_lstm_hip.so
 
-The library exposes the C ABI declared in include/persistent_lstm_hip.h.  It is built in-tree so
-that the .so travels with the source tree; nothing is installed.
+The library exposes the C ABI declared in include/persistent_lstm_hip.h.  Beside it the module plh_torch.so, the
+torch front end of the block operators, is compiled as plain C++ against the installed torch.  Both are built in-tree so
+that they travel with the source tree; nothing is installed.
 """
 from __future__ import annotations
 
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
@@ -19,6 +21,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpersistent_lstm_hip.so")
+TORCH_PATH = os.path.join(LIB_DIR, "plh_torch.so")
 BENCH_PATH = os.path.join(LIB_DIR, "plh_bench")
 SOURCES = ["plh_wavefront.hip", "plh_sliced.hip", "plh_rec.hip", "plh_gemm.hip", "plh_pack.hip", "plh_launch.hip",
            "plh_probe.hip", "plh_capi.hip", "plh_scan.hip", "plh_norm.hip", "plh_dropout.hip"]
@@ -46,6 +49,13 @@ def hipcc() -> str:
     return path
 
 
+def host_compiler() -> str:
+    path = shutil.which("g++") or shutil.which("c++")
+    if path is None:
+        raise RuntimeError("g++ not found: the torch front end needs a C++ compiler")
+    return path
+
+
 def build(verbose: bool = False) -> str:
     """Compile every source for gfx950 and link the shared library.  Always recompiles."""
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -66,10 +76,27 @@ def build(verbose: bool = False) -> str:
         run([hipcc()] + HIPCC_FLAGS + ["-c", os.path.join(CSRC, source), "-o", obj])
         return obj
 
+    import torch
+
+    torch_dir = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
     with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(4) as pool:
+        front_obj = os.path.join(objects, "plh_torch.o")
+        front = pool.submit(run, [host_compiler(), "-std=c++17", "-O2", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
+                                  "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=plh_torch"] +
+                            [a for d in (os.path.join(torch_dir, "include"),
+                                         os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                                         os.path.join(rocm, "include"), sysconfig.get_paths()["include"])
+                             for a in ("-isystem", d)] +
+                            ["-c", os.path.join(CSRC, "plh_torch.cpp"), "-o", front_obj])
         objs = list(pool.map(lambda s: compile_one(s, objects), SOURCES))
         run([hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}"] + objs + LINK_FLAGS + ["-o", tmp])
-    os.replace(tmp, LIB_PATH)
+        os.replace(tmp, LIB_PATH)
+        front.result()
+        run([host_compiler(), "-shared", front_obj, "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_hip",
+             "-ltorch_cpu", "-ltorch", "-ltorch_python", "-L" + LIB_DIR, "-lpersistent_lstm_hip", "-Wl,-rpath,$ORIGIN",
+             "-o", TORCH_PATH + ".tmp"])
+    os.replace(TORCH_PATH + ".tmp", TORCH_PATH)
     # Native driver of the C ABI (profiling target and integration example), linked to the library.
     # (plh_issue_probe.hip: a developer probe kernel of plh_bench --issue, not part of the library.)
     cmd = [hipcc(), "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs p) {
       const uint32_t r = (rnd.w[i / 2] >> (16 * (i % 2))) & 0xFFFFu;
       float v = r >= p.threshold ? (float)vx[i] * p.scale : 0.0f;
       if (RESIDUAL) v += (float)vr[i];
-      y[i] = (T)v;
+      y[i] = round_to<T>(v);
     }
     if (live == 8) {
 #pragma unroll

@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_forward_kernel(Nor
       if (c < p.cols) {
         Vec<T, VEC> t;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) t.v[j] = (T)fmaf(x[i][j] * rstd, w[i][j], b[i][j]);
+        for (int j = 0; j < VEC; ++j) t.v[j] = round_to<T>(fmaf(x[i][j] * rstd, w[i][j], b[i][j]));
         store_vec(dst + c, t);
       }
     }
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_backward_kernel(No
       if (c < p.cols) {
         Vec<T, VEC> t;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) t.v[j] = (T)(rstd * (v[i][j] - m1 - xh[i][j] * m2));
+        for (int j = 0; j < VEC; ++j) t.v[j] = round_to<T>(rstd * (v[i][j] - m1 - xh[i][j] * m2));
         store_vec(dst + c, t);
       }
     }
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(NormArg
       float w[1], b[1];
       load_param<T, 1>(p.weight, p.w32, c, 1.0f, w);
       load_param<T, 1>(p.bias, p.w32, c, 0.0f, b);
-      static_cast<T*>(p.y)[r * p.cols + c] = (T)fmaf(((float)src[c] - mean) * rstd, w[0], b[0]);
+      static_cast<T*>(p.y)[r * p.cols + c] = round_to<T>(fmaf(((float)src[c] - mean) * rstd, w[0], b[0]));
     }
     if (threadIdx.x == 0) {
       if (p.mean) p.mean[r] = mean;
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(NormAr
       float w[1];
       load_param<T, 1>(p.weight, p.w32, c, 1.0f, w);
       const float xh = ((float)src[c] - mean) * rstd;
-      static_cast<T*>(p.d_x)[r * p.cols + c] = (T)(rstd * ((float)grad[c] * w[0] - m1 - xh * m2));
+      static_cast<T*>(p.d_x)[r * p.cols + c] = round_to<T>(rstd * ((float)grad[c] * w[0] - m1 - xh * m2));
     }
   }
 }
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(NormArgs p) {
   if (p.w32)
     static_cast<float*>(dst)[k] = s;
   else
-    static_cast<T*>(dst)[k] = (T)s;
+    static_cast<T*>(dst)[k] = round_to<T>(s);
 }
 
 // Threads per row and pieces per thread for `pieces` pieces of VEC columns; {0, 0}: too many for registers.

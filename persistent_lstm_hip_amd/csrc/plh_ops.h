@@ -33,6 +33,14 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
   *reinterpret_cast<Vec<T, N>*>(p) = v;
 }
 
+// v rounded to T as an fp32 value.  (Left alone, the compiler may fold the operation that made v into the conversion,
+// in some variants of a kernel and not in others, which then differ in a last place now and then.)
+template <typename T>
+__device__ __forceinline__ T round_to(float v) {
+  if constexpr (sizeof(T) < sizeof(float)) asm("" : "+v"(v));
+  return (T)v;
+}
+
 constexpr float kOpLog2e = 1.4426950408889634f;
 
 // The logistic function and its complement, s = 1 / (1 + e) and 1 - s = e s with e = 2^min(-z log2 e, 126): the

@@ -89,13 +89,8 @@ struct Place {
     on = n < p.channels;
     b = 0, h = 0, len = 0;
     if (on) {
-      if (p.channels <= 0xFFFFFFFFll) {
-        b = (uint32_t)n / (uint32_t)p.H;
-        h = (int)((uint32_t)n % (uint32_t)p.H);
-      } else {
-        b = n / p.H;
-        h = (int)(n % p.H);
-      }
+      b = (uint32_t)n / (uint32_t)p.H;  // (channels <= 2^29)
+      h = (int)((uint32_t)n % (uint32_t)p.H);
       len = p.T_;
       if (p.lengths) len = min(max(p.lengths[b], 0), p.T_);
     }
@@ -341,7 +336,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs<T> 
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           c[j] = fmaf(a[r][j], c[j], b[r][j]);
-          y[r].v[j] = (T)(GATED ? c[j] * sigmoid((float)x.o[r].v[j]) : c[j]);
+          y[r].v[j] = round_to<T>(GATED ? c[j] * sigmoid((float)x.o[r].v[j]) : c[j]);
         }
       }
       if (__all(t0 + R <= at.len)) {
@@ -447,7 +442,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs<T>
         for (int j = 0; j < VEC; ++j) {
           before[r][j] = c[j];
           c[j] = fmaf(a[r][j], c[j], na[r][j] * (float)x.g[r].v[j]);
-          if (GATED) d_o[r].v[j] = (T)(w[r][j] * c[j]);
+          if (GATED) d_o[r].v[j] = round_to<T>(w[r][j] * c[j]);
         }
       }
 #pragma unroll
@@ -457,8 +452,8 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs<T>
           const float D = u[r][j] + e[j];
           const float n = na[r][j] * D;
           e[j] = a[r][j] * D;
-          dg[r].v[j] = (T)n;
-          df[r].v[j] = (T)(a[r][j] * n * (before[r][j] - (float)x.g[r].v[j]));
+          dg[r].v[j] = round_to<T>(n);
+          df[r].v[j] = round_to<T>(a[r][j] * n * (before[r][j] - (float)x.g[r].v[j]));
         }
       }
       T* const dst = p.d_gates + (at.b * p.T_ + t0) * (int64_t)(kParts * p.H) + at.h;
@@ -489,8 +484,42 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs<T>
   }
 }
 
+// One step of every row, for serving: a thread per VEC channels, nothing to scan.  (The tiled kernel would leave 63 of
+// 64 steps idle: 20.4 us for 512 rows of 512 channels in bfloat16.)
+template <typename T, int VEC, bool GATED>
+__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanArgs<T> p) {
+  const int64_t n = ((int64_t)blockIdx.x * kScanThreads + threadIdx.x) * VEC;
+  if (n >= p.channels) return;
+  const uint32_t b = (uint32_t)n / (uint32_t)p.H, h = (uint32_t)n % (uint32_t)p.H;  // (channels <= 2^29)
+  Vec<float, VEC> c = {};
+  if (p.c0) c = load_vec<float, VEC>(p.c0 + n);
+  if (p.states) store_vec(p.states + n, c);
+  Vec<T, VEC> y = {};
+  if (!p.lengths || p.lengths[b] > 0) {
+    const T* const src = p.gates + b * p.stride_b + h;
+    const Vec<T, VEC> f = load_vec<T, VEC>(src), g = load_vec<T, VEC>(src + p.H);
+    Vec<T, VEC> o = {};
+    if (GATED) o = load_vec<T, VEC>(src + 2 * p.H);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float a, na;
+      logistic((float)f.v[j], a, na);
+      c.v[j] = fmaf(a, c.v[j], na * (float)g.v[j]);
+      y.v[j] = round_to<T>(GATED ? c.v[j] * sigmoid((float)o.v[j]) : c.v[j]);
+    }
+  }
+  if (p.c_n) store_vec(p.c_n + n, c);
+  store_vec(p.out + n, y);
+}
+
 template <typename T, int VEC, bool GATED>
 hipError_t launch_forward(const ScanArgs<T>& p, hipStream_t s) {
+  if (p.T_ == 1) {
+    const int64_t threads = (p.channels + VEC - 1) / VEC;
+    hipLaunchKernelGGL((scan_step_kernel<T, VEC, GATED>), dim3((unsigned)((threads + kScanThreads - 1) / kScanThreads)),
+                       dim3(kScanThreads), 0, s, p);
+    return hipGetLastError();
+  }
   if (p.segs > 1) {
     hipLaunchKernelGGL((scan_forward_kernel<T, VEC, GATED, true>), dim3(p.slabs * (unsigned)(p.segs - 1)),
                        dim3(kScanThreads), 0, s, p);

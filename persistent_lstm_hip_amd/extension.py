@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
 from functools import lru_cache
 from typing import Dict, List, Optional, Sequence
@@ -23,6 +24,7 @@ import torch
 
 # Built by persistent_lstm_hip_amd/build.py.
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libpersistent_lstm_hip.so")
+TORCH_PATH = os.path.join(os.path.dirname(LIB_PATH), "plh_torch.so")  # the block operators' torch front end
 
 PLH_OK = 0
 PLH_ERR_INVALID = 1
@@ -661,3 +663,18 @@ def require_extension() -> NativeLibrary:
     if ext is None:
         raise RuntimeError(f"persistent_lstm_hip_amd native library unavailable: {_load_error}")
     return ext
+
+
+@lru_cache(maxsize=1)
+def require_torch_ops():
+    """The module plh_torch (csrc/plh_torch.cpp), the torch front end of the block operators; RuntimeError (never a
+    fallback) if it or the library under it is unavailable."""
+    require_extension()
+    try:
+        spec = importlib.util.spec_from_file_location("plh_torch", TORCH_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except (ImportError, OSError) as exc:
+        raise RuntimeError(f"persistent_lstm_hip_amd: cannot load {TORCH_PATH} ({exc}): run "
+                           "`python -m persistent_lstm_hip_amd.build`") from exc
+    return module

@@ -14,7 +14,6 @@ import torch
 import ops_plain as plain
 import persistent_lstm_hip_amd as P
 from ops_plain import U, assert_within
-from persistent_lstm_hip_amd import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -381,6 +380,21 @@ def test_norm_of_more_dimensions(gpu):
     assert torch.equal(P.layer_norm(one, w), P.layer_norm(one.unsqueeze(0), w)[0])
 
 
+def test_norm_reads_rows_where_they_are(gpu):
+    """Of what it may read in place the operator makes no copy: one allocation, the output's."""
+    _say("norm copies")
+    big = torch.randn(600, 1100, device="cuda")
+    cube = torch.randn(30, 20, 1000, device="cuda")
+    for x, copies in ((big[:, 50:1050], 0), (big[::2, :1000], 0), (cube, 0), (cube[:, :10], 1), (big.t(), 1)):
+        y = P.layer_norm(x)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = P.layer_norm(x, eps=1e-5)
+        peak = torch.cuda.max_memory_allocated() - before
+        assert y.nelement() * 4 * (1 + copies) <= peak < y.nelement() * 4 * (2 + copies), (x.shape, x.stride())
+
+
 @pytest.mark.parametrize("dtype,mean", [(F32, 1000.0), (F16, 1000.0), (BF16, 100.0)])
 def test_norm_of_a_large_mean(gpu, dtype, mean):
     _say(f"norm mean {mean} {dtype}")
@@ -568,7 +582,10 @@ def test_operators_refuse_on_the_device(gpu):
     z, c = torch.zeros(2, 3, 12, device="cuda"), torch.zeros(2, 4, device="cuda")
     for bad in (lambda: P.gated_scan(z.double()), lambda: P.gated_scan(z[0]), lambda: P.gated_scan(z[..., :11]),
                 lambda: P.gated_scan(z, c[:1]), lambda: P.gated_scan(z, c.cpu()), lambda: P.gated_scan(z, lengths=[1]),
-                lambda: P.gated_scan(z, lengths=[1, 4]), lambda: P.gated_scan_step(z[:, 0], c.half()),
+                lambda: P.gated_scan(z, lengths=[1, 4]), lambda: P.gated_scan(z, lengths=[-1, 2]),
+                lambda: P.gated_scan(z, lengths=[1.5, 2.0]), lambda: P.gated_scan(z, lengths=[True, False]),
+                lambda: P.gated_scan(z, lengths=torch.ones(2, 1, dtype=torch.int32)), lambda: P.gated_scan(z[..., :0]),
+                lambda: P.gated_scan(z[..., :9], output_gate=False), lambda: P.gated_scan_step(z[:, 0], c.half()),
                 lambda: P.gated_scan_step(z, c), lambda: P.gated_scan_step(z[:, 0], c.t().contiguous().t(), inplace=True),
                 lambda: P.gated_scan_step(z[:, 0].requires_grad_(True), c),
                 lambda: P.layer_norm(c, torch.ones(5, device="cuda")), lambda: P.layer_norm(c, torch.ones(4)),

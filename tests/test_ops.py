@@ -72,37 +72,13 @@ def test_public_names():
     lambda t: P.gated_scan_step(t(2, 12), t(2, 4)),
     lambda t: P.layer_norm(t(2, 8)),
     lambda t: P.dropout_add(t(2, 8), p=0.1, seed=1),
+    lambda t: P.dropout_add(t(2, 8), p=0.1, seed=-1, offset=torch.zeros(1, dtype=torch.int64)),
 ])
 def test_host_tensors_are_refused(call):
     with pytest.raises(ValueError, match="HIP device"):
         call(torch.zeros)
     with pytest.raises(ValueError, match="must be a tensor"):
         call(lambda *shape: [0.0])
-
-
-@pytest.mark.parametrize("lengths", [[1.5, 2.0], [1], [1, 2, 3], torch.ones(2, 1, dtype=torch.int32), [True, False],
-                                     [-1, 2], [1, 6]])
-def test_lengths_that_are_not_lengths_are_refused(lengths):
-    with pytest.raises(ValueError, match="lengths"):
-        ops._lengths(lengths, 2, 5, torch.device("cuda", 0))
-
-
-def test_gate_widths():
-    assert ops._scan_shape(torch.empty(0, 0, 12), True) == 4 and ops._scan_shape(torch.empty(0, 12), False) == 6
-    for width, gated in ((13, True), (13, False), (0, True)):
-        with pytest.raises(ValueError, match="columns"):
-            ops._scan_shape(torch.empty(1, width), gated)
-
-
-def test_rows_of_a_matrix_are_views_where_one_stride_serves():
-    x = torch.zeros(4, 5, 6)
-    assert ops._matrix(x).data_ptr() == x.data_ptr() and ops._matrix(x).shape == (20, 6)
-    wide = torch.zeros(7, 10)[:, 2:8]
-    assert ops._matrix(wide).data_ptr() == wide.data_ptr() and ops._matrix(wide).stride(0) == 10
-    assert ops._matrix(x.transpose(0, 1)).is_contiguous()  # its leading dimensions do not merge
-    assert ops._matrix(torch.zeros(6, 4).t()).stride(1) == 1
-    assert ops._matrix(torch.zeros(12)[::2]).stride(1) == 1
-    assert ops._matrix(torch.zeros(3, 0, 6)).shape == (0, 6)
 
 
 # ---- the C ABI refuses before it touches a device ------------------------------------------------
