@@ -106,7 +106,7 @@ template <typename T>
 hipError_t launch_dropout(const DropoutArgs& p, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const unsigned grid = (unsigned)std::min<int64_t>((p.n + 2047) / 2048, 256 * 8);
-  const bool wide = aligned<T>(p.x, V) && aligned<T>(p.residual, V) && aligned<T>(p.out, V);
+  const bool wide = aligned(p.x, 16) && aligned(p.residual, 16) && aligned(p.out, 16);
   if (wide && p.residual)
     hipLaunchKernelGGL((dropout_kernel<T, V, true>), dim3(grid), dim3(256), 0, s, p);
   else if (wide)

@@ -377,8 +377,8 @@ hipError_t launch_vec(const NormArgs& p, const Shape& sh, hipStream_t s) {
 template <typename T>
 int norm_vec(const NormArgs& p) {
   for (int v : {16 / (int)sizeof(T), 4})
-    if (p.cols % v == 0 && p.stride % v == 0 && aligned<T>(p.x, v) && aligned<T>(p.y, v) && aligned<T>(p.d_y, v) &&
-        aligned<T>(p.d_x, v))
+    if (p.cols % v == 0 && p.stride % v == 0 && aligned(p.x, v * (int)sizeof(T)) && aligned(p.y, v * (int)sizeof(T)) && aligned(p.d_y, v * (int)sizeof(T)) &&
+        aligned(p.d_x, v * (int)sizeof(T)))
       return v;
   return 1;
 }
@@ -479,7 +479,7 @@ int plh_layer_norm_backward(int dtype, int wdtype, const void* x, int64_t stride
     return plh::op_error(PLH_ERR_INVALID, what, "mean, rstd and d_y are required");
   if ((d_weight || d_bias) && (!workspace || workspace_bytes < plh_layer_norm_workspace_bytes(rows, cols)))
     return plh::op_error(PLH_ERR_INVALID, what, "workspace missing or smaller than plh_layer_norm_workspace_bytes()");
-  if (!plh::aligned<float>(workspace, 4))
+  if (!plh::aligned(workspace, 16))
     return plh::op_error(PLH_ERR_INVALID, what, "workspace must be 16-byte aligned");
   plh::NormArgs p = {};
   p.x = x, p.stride = stride, p.rows = rows, p.cols = (int)cols;

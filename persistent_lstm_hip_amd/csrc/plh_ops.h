@@ -18,27 +18,58 @@ namespace {
 
 constexpr int kWave = 64;
 
-// N consecutive elements, moved with one load or store of N * sizeof(T) bytes.
+// N consecutive elements, moved with one load or store of N * sizeof(T) bytes.  The address needs an element's
+// alignment only: gfx950 takes wide global accesses at any (element) address, so odd row lengths and strides cost the
+// lines that they straddle and no narrower instruction.
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Vec {
+struct Vec {
   T v[N];
 };
 
 template <typename T, int N>
 __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
-  return *reinterpret_cast<const Vec<T, N>*>(p);
+  Vec<T, N> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
-  *reinterpret_cast<Vec<T, N>*>(p) = v;
+  __builtin_memcpy(p, &v, sizeof(v));
 }
 
-// v rounded to T as an fp32 value.  (Left alone, the compiler may fold the operation that made v into the conversion,
-// in some variants of a kernel and not in others, which then differ in a last place now and then.)
+// Barrier that orders LDS traffic only: global loads and stores stay in flight across it (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Values rounded to T as fp32 values.  (Left alone, the compiler may fold the operation that made a value into its
+// conversion, in some variants of a kernel and not in others, which then differ in a last place now and then.)
 template <typename T>
 __device__ __forceinline__ T round_to(float v) {
   if constexpr (sizeof(T) < sizeof(float)) asm("" : "+v"(v));
   return (T)v;
+}
+// The same for a vector, with one conversion instruction for two values of 16 bits.
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> round_to(const float (&v)[N]) {
+  Vec<T, N> r;
+  if constexpr (sizeof(T) < sizeof(float) && N % 2 == 0) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      f32x2 p = {v[j], v[j + 1]};
+      asm("" : "+v"(p));
+      const t2 q = __builtin_convertvector(p, t2);
+      r.v[j] = q[0], r.v[j + 1] = q[1];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.v[j] = round_to<T>(v[j]);
+  }
+  return r;
 }
 
 constexpr float kOpLog2e = 1.4426950408889634f;
@@ -63,10 +94,7 @@ __device__ __forceinline__ float sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -kOpLog2e));
 }
 
-template <typename T>
-inline bool aligned(const void* p, int n) {
-  return (reinterpret_cast<uintptr_t>(p) % (sizeof(T) * n)) == 0;
-}
+inline bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
 
 // Calls f with a value of the element type that `dtype` names; false if it names none.
 template <typename F>

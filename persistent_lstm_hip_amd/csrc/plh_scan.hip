@@ -19,15 +19,25 @@
 namespace plh {
 namespace {
 
-// A workgroup of 256 threads carries a slab of 64 channels through time, 64 steps (a tile) at a time.  Channels are
-// numbered row after row, n = b H + h, so that slabs are full whatever H is.  A thread has VEC neighbouring channels
-// for 16 / VEC consecutive steps: 64 / VEC threads side by side read 64 channels of one step, the groups of so many
-// threads are consecutive in time.
-constexpr int kScanThreads = 256;
-constexpr int kSlab = 64;
-constexpr int kTile = 64;
+// A workgroup carries a slab of channels through time, 64 steps (a tile) at a time.  A thread has VEC neighbouring
+// channels for R consecutive steps; CT threads side by side read one step of the slab, the groups of so many threads
+// are consecutive in time.  A row's channels are cut into pieces of VEC, the last of which is moved back to end with
+// the row: its channels are then carried by two threads, which compute and store the same.  Pieces are numbered row
+// after row, so that slabs are full whatever H is.
+//   VEC 4, CT 16: 256 threads, 64 channels, 4 steps each (the usual slab)
+//   VEC 4, CT 32: 512 threads, 128 channels, 4 steps each (backward, see wide_slabs)
+//   VEC 1, CT 64: 256 threads, 64 channels, 16 steps each (H < 4)
+constexpr int kTile = 64;  // steps
+template <int CT>
+constexpr int kSlabThreads = CT == 32 ? 512 : 256;
 
-// Workgroups that a launch should have at least: with fewer slabs than that the time axis is split into segments.
+// Channels per thread.
+inline int scan_vec(int64_t hidden) { return hidden >= 4 ? 4 : 1; }
+
+// Workgroups that a launch should have: two per CU.  With fewer slabs the time axis is split into segments, whose maps
+// a launch of its own computes first.  Forward / backward with about 512, 1024 and 2048 workgroups: 2 x 16384 x 640 bf16
+// (20 slabs) 60 / 94, 59 / 100, 56 / 95 us; 32 x 2048 x 512 (256 slabs) 83 / 125, 83 / 144, 85 / 147; 16 x 2048 x 2048
+// fp32 (512 slabs) 220 / 375 unsplit, 274 / 473 in two segments.
 constexpr int kScanGroups = 512;
 
 struct Split {
@@ -36,13 +46,18 @@ struct Split {
   int segs;
 };
 
-int64_t slabs_of(int64_t batch, int64_t hidden) { return (batch * hidden + kSlab - 1) / kSlab; }
+int64_t pieces_of(int64_t batch, int64_t hidden) { return batch * ((hidden + scan_vec(hidden) - 1) / scan_vec(hidden)); }
+// Slabs of the usual kind.
+int64_t slabs_of(int64_t batch, int64_t hidden) {
+  const int ct = hidden >= 4 ? 16 : 64;
+  return (pieces_of(batch, hidden) + ct - 1) / ct;
+}
 
 Split split_for(int64_t batch, int64_t seq_len, int64_t hidden) {
   Split s;
   s.tiles = (int)((seq_len + kTile - 1) / kTile);
   const int64_t slabs = std::max<int64_t>(slabs_of(batch, hidden), 1);
-  const int want = (int)std::max<int64_t>(1, kScanGroups / slabs);
+  const int want = (int)std::max<int64_t>(1, (kScanGroups + slabs / 2) / slabs);
   s.seg_tiles = std::max(1, (s.tiles + want - 1) / want);
   s.segs = std::max(1, (s.tiles + s.seg_tiles - 1) / s.seg_tiles);
   return s;
@@ -54,7 +69,7 @@ struct ScanArgs {
   int64_t stride_b, stride_t;  // elements
   int64_t channels;            // B H
   int T_, H, tiles, seg_tiles, segs;
-  unsigned slabs;
+  unsigned slabs, pieces;
   const int32_t* lengths;
   const float* c0;
   T* out;         // [B][T][H]
@@ -67,42 +82,57 @@ struct ScanArgs {
   float* d_c0;
 };
 
+// The slab of a launch's workgroup i of n.  Workgroups go round the eight XCDs in turn; here each XCD gets neighbouring
+// slabs, so that a cache line that two slabs share is read into one L2 (33 x 1001 x 333 fp16, no slab aligned: forward
+// 47.7 -> 40.2 us, backward 79.4 -> 68.2).
+__device__ __forceinline__ unsigned slab_of(unsigned i, unsigned n) {
+  const unsigned per = n / 8;
+  return i < per * 8 ? (i % 8) * per + i / 8 : i;
+}
+
 // Where a thread stands: its channels, its place among the time groups, its row's length.
-template <int VEC>
+template <int VEC_, int CT_>
 struct Place {
-  static constexpr int CT = kSlab / VEC;          // threads side by side
-  static constexpr int TG = kScanThreads / CT;    // time groups
-  static constexpr int R = kTile / TG;            // steps of a thread
-  static constexpr int WG = kWave / CT;           // time groups of a wave
+  static constexpr int VEC = VEC_, CT = CT_;
+  static constexpr int TG = VEC == 4 ? 16 : 4;          // time groups
+  static constexpr int R = kTile / TG;                  // steps of a thread
+  static constexpr int THREADS = kSlabThreads<CT>, WAVES = THREADS / kWave, SLAB = CT * VEC;
+  static_assert(THREADS == CT * TG && ((VEC == 4 && (CT == 16 || CT == 32)) || (VEC == 1 && CT == 64)),
+                "four, two or one time groups in a wave");
   int lane, wave, ct, tg;
-  int64_t n;  // first channel
   bool on;
-  int64_t b;
+  int64_t b, n;  // row; first channel, counted over all rows
   int h, len;
+  int live_tiles;  // tiles that a row of the slab reaches (the same in every wave: each has all of the slab's channels)
 
   template <typename T>
   __device__ __forceinline__ Place(const ScanArgs<T>& p, unsigned slab) {
     const int tid = threadIdx.x;
     lane = tid % kWave, ct = tid % CT, tg = tid / CT;
     wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    n = (int64_t)slab * kSlab + ct * VEC;
-    on = n < p.channels;
-    b = 0, h = 0, len = 0;
+    const uint32_t per = (p.H + VEC - 1) / VEC, piece = slab * CT + ct;  // (batch * hidden <= 2^29)
+    on = piece < p.pieces;
+    b = 0, n = 0, h = 0, len = 0;
     if (on) {
-      b = (uint32_t)n / (uint32_t)p.H;  // (channels <= 2^29)
-      h = (int)((uint32_t)n % (uint32_t)p.H);
+      b = piece / per;
+      h = min((int)(piece % per) * VEC, p.H - VEC);
+      n = b * p.H + h;
       len = p.T_;
       if (p.lengths) len = min(max(p.lengths[b], 0), p.T_);
     }
+    int most = len;
+#pragma unroll
+    for (int d = 1; d < CT; d *= 2) most = max(most, __shfl_xor(most, d));
+    live_tiles = __builtin_amdgcn_readfirstlane((most + kTile - 1) / kTile);
   }
 };
 
 // v of the even and of the odd time group of a pair of groups, in both (one exchange per level and value).
-template <int VEC, int LEVEL>
+template <int LEVEL>
 __device__ __forceinline__ void pair_of(float v, float& even, float& odd) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);
   uint32_t lo, hi;
-  if constexpr (VEC == 4 && LEVEL == 0) {  // groups of 16 lanes: neighbouring rows
+  if constexpr (LEVEL == 0) {  // groups of 16 lanes: neighbouring rows
     const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     lo = r[0], hi = r[1];
   } else {  // halves of the wave
@@ -116,26 +146,25 @@ __device__ __forceinline__ void pair_of(float v, float& even, float& odd) {
 // steps in order; k = 1: in reverse order, SUMS = 2 only).  Out: pa[k], pb[k], the map of everything in this wave
 // that comes before the thread's steps in direction k (REVERSE0: direction 0 is reverse order too); A and B become the
 // wave's own.
-template <int VEC, int SUMS, bool REVERSE0>
+template <typename P, int SUMS, bool REVERSE0, int VEC = P::VEC>
 __device__ __forceinline__ void wave_maps(int lane, float (&A)[VEC], float (&B)[SUMS][VEC], float (&pa)[SUMS][VEC],
                                           float (&pb)[SUMS][VEC]) {
-  constexpr int kLevels = VEC == 4 ? 2 : VEC == 2 ? 1 : 0;
 #pragma unroll
   for (int k = 0; k < SUMS; ++k)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) pa[k][j] = 1.0f, pb[k][j] = 0.0f;
   const auto level = [&](auto lv) {
     constexpr int L = decltype(lv)::value;
-    const bool odd = (lane & (VEC == 4 && L == 0 ? 16 : 32)) != 0;
+    const bool odd = (lane & (L == 0 ? 16 : 32)) != 0;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       float a0, a1;
-      pair_of<VEC, L>(A[j], a0, a1);
+      pair_of<L>(A[j], a0, a1);
 #pragma unroll
       for (int k = 0; k < SUMS; ++k) {
         const bool rev = REVERSE0 || k == 1;
         float b0, b1;
-        pair_of<VEC, L>(B[k][j], b0, b1);
+        pair_of<L>(B[k][j], b0, b1);
         // the other group of the pair comes first for the odd one in order, for the even one in reverse
         const float fa = rev ? a1 : a0, fb = rev ? b1 : b0, sa = rev ? a0 : a1, sb = rev ? b0 : b1;
         if (odd != rev) {
@@ -147,49 +176,63 @@ __device__ __forceinline__ void wave_maps(int lane, float (&A)[VEC], float (&B)[
       A[j] = a0 * a1;
     }
   };
-  if constexpr (kLevels >= 1) level(std::integral_constant<int, 0>());
-  if constexpr (kLevels >= 2) level(std::integral_constant<int, 1>());
+  if constexpr (P::CT == 16) level(std::integral_constant<int, 0>());
+  if constexpr (P::CT <= 32) level(std::integral_constant<int, 1>());
 }
 
-// The four waves' maps in LDS: [parity of the tile][wave][A, sums...][channel].  Two halves in turn need one barrier
+// The waves' maps in LDS: [parity of the tile][wave][A, sums...][channel].  Two halves in turn need one barrier
 // per tile: the half written next was last read before the barrier in between.
-template <int SUMS>
-using WaveMaps = float[2][kScanThreads / kWave][1 + SUMS][kSlab];
+struct alignas(16) Lds4 {
+  float v[4];
+};
+template <int VEC>
+__device__ __forceinline__ void put_lds(float* dst, const float (&v)[VEC]) {
+  if constexpr (VEC == 4)
+    *reinterpret_cast<Lds4*>(dst) = Lds4{{v[0], v[1], v[2], v[3]}};
+  else
+    dst[0] = v[0];
+}
+template <int VEC>
+__device__ __forceinline__ Vec<float, VEC> get_lds(const float* src) {
+  if constexpr (VEC == 4) {
+    const Lds4 r = *reinterpret_cast<const Lds4*>(src);
+    return {{r.v[0], r.v[1], r.v[2], r.v[3]}};
+  } else {
+    return {{src[0]}};
+  }
+}
+template <typename P, int SUMS>
+using TileMaps = float[P::WAVES][1 + SUMS][P::SLAB];
+template <typename P, int SUMS>
+using WaveMaps = TileMaps<P, SUMS>[2];
 
-template <int VEC, int SUMS>
-__device__ __forceinline__ void put_maps(const Place<VEC>& at, float (&lds)[kScanThreads / kWave][1 + SUMS][kSlab],
-                                         const float (&A)[VEC], const float (&B)[SUMS][VEC]) {
-  if (at.lane < Place<VEC>::CT) {
-    Vec<float, VEC> v;
+template <typename P, int SUMS, int VEC = P::VEC>
+__device__ __forceinline__ void put_maps(const P& at, TileMaps<P, SUMS>& lds, const float (&A)[VEC],
+                                         const float (&B)[SUMS][VEC]) {
+  if (at.lane < P::CT) {
+    put_lds<VEC>(&lds[at.wave][0][at.ct * VEC], A);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v.v[j] = A[j];
-    store_vec(&lds[at.wave][0][at.ct * VEC], v);
-#pragma unroll
-    for (int k = 0; k < SUMS; ++k) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v.v[j] = B[k][j];
-      store_vec(&lds[at.wave][1 + k][at.ct * VEC], v);
-    }
+    for (int k = 0; k < SUMS; ++k) put_lds<VEC>(&lds[at.wave][1 + k][at.ct * VEC], B[k]);
   }
 }
 
-// The carry through the four waves' maps: `carry` becomes the value after the whole tile, `mine` the value that this
+// The carry through the waves' maps: `carry` becomes the value after the whole tile, `mine` the value that this
 // thread's steps start from; (pa, pb) is the thread's map from wave_maps.
-template <int VEC, int SUMS, int K, bool REVERSE>
-__device__ __forceinline__ void fold_waves(const Place<VEC>& at, const float (&lds)[kScanThreads / kWave][1 + SUMS][kSlab],
-                                           const float (&pa)[VEC], const float (&pb)[VEC], float (&carry)[VEC],
-                                           float (&mine)[VEC]) {
-  constexpr int W = kScanThreads / kWave;
+template <typename P, int SUMS, int K, bool REVERSE, int VEC = P::VEC>
+__device__ __forceinline__ void fold_waves(const P& at, const TileMaps<P, SUMS>& lds, const float (&pa)[VEC],
+                                           const float (&pb)[VEC], float (&carry)[VEC], float (&mine)[VEC]) {
+  constexpr int W = P::WAVES;
   float before[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) before[j] = carry[j];
 #pragma unroll
   for (int i = 0; i < W; ++i) {
     const int w = REVERSE ? W - 1 - i : i;
-    if (w == at.wave) {
+    if (i > 0 && w == at.wave) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) before[j] = carry[j];
     }
-    const Vec<float, VEC> a = load_vec<float, VEC>(&lds[w][0][at.ct * VEC]);
-    const Vec<float, VEC> b = load_vec<float, VEC>(&lds[w][1 + K][at.ct * VEC]);
+    const Vec<float, VEC> a = get_lds<VEC>(&lds[w][0][at.ct * VEC]), b = get_lds<VEC>(&lds[w][1 + K][at.ct * VEC]);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) carry[j] = fmaf(a.v[j], carry[j], b.v[j]);
   }
@@ -197,27 +240,46 @@ __device__ __forceinline__ void fold_waves(const Place<VEC>& at, const float (&l
   for (int j = 0; j < VEC; ++j) mine[j] = fmaf(pa[j], before[j], pb[j]);
 }
 
-// The carry at a segment's start: the maps of the segments before it, in order, applied to `carry`.
-template <typename T, int VEC>
-__device__ __forceinline__ void fold_segments(const ScanArgs<T>& p, const Place<VEC>& at, int from, int to, int step,
-                                              float (&carry)[VEC]) {
-  if (!at.on) return;
-  for (int s = from; s != to; s += step) {
-    const int64_t o = (int64_t)s * p.channels + at.n;
-    const Vec<float, VEC> a = load_vec<float, VEC>(p.seg_a + o), b = load_vec<float, VEC>(p.seg_b + o);
+// The carry at a segment's start: the maps of the n segments before it, segment `first` + i `step` for i = 0 .. n - 1 in
+// this order, applied to `carry`.  Each time group composes a run of them, and the runs are composed as a tile's are.
+// (One thread after the other through the same maps, an L2 latency each, took 60 us for 255 segments.)
+template <typename T, typename P, int SUMS, int VEC = P::VEC>
+__device__ __forceinline__ void fold_segments(const ScanArgs<T>& p, const P& at, int first, int step, int n,
+                                              TileMaps<P, SUMS>& lds, float (&carry)[VEC]) {
+  if (n == 0) return;
+  float A[VEC], B[1][VEC], pa[1][VEC], pb[1][VEC], none[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) carry[j] = fmaf(a.v[j], carry[j], b.v[j]);
+  for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = 0.0f;
+  if (at.on) {
+    const int run = (n + P::TG - 1) / P::TG, end = min(n, (at.tg + 1) * run);
+#pragma unroll 4
+    for (int i = at.tg * run; i < end; ++i) {
+      const int64_t o = (int64_t)(first + i * step) * p.channels + at.n;
+      const Vec<float, VEC> a = load_vec<float, VEC>(p.seg_a + o), b = load_vec<float, VEC>(p.seg_b + o);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        B[0][j] = fmaf(a.v[j], B[0][j], b.v[j]);
+        A[j] *= a.v[j];
+      }
+    }
   }
+  wave_maps<P, 1, false>(at.lane, A, B, pa, pb);
+  if (at.lane < P::CT) {
+    put_lds<VEC>(&lds[at.wave][0][at.ct * VEC], A);
+    put_lds<VEC>(&lds[at.wave][1][at.ct * VEC], B[0]);
+  }
+  lds_barrier();
+  fold_waves<P, SUMS, 0, false>(at, lds, pa[0], pb[0], carry, none);
 }
 
 // A thread's rows of a tile.  Steps past the row's length hold f = +inf, so that a = 1 and 1 - a = 0 without a test,
 // and zeros.
-template <typename T, int VEC, bool G, bool O, bool D>
+template <typename T, typename P, bool G, bool O, bool D>
 struct Rows {
-  static constexpr int R = Place<VEC>::R;
+  static constexpr int VEC = P::VEC, R = P::R;
   Vec<T, VEC> f[R], g[R], o[R], d[R];
 
-  __device__ __forceinline__ void load(const ScanArgs<T>& p, const Place<VEC>& at, int tile) {
+  __device__ __forceinline__ void load(const ScanArgs<T>& p, const P& at, int tile) {
     const int t0 = tile * kTile + at.tg * R;
     const T* src = p.gates + at.b * p.stride_b + (int64_t)t0 * p.stride_t + at.h;
     const T* grad = D ? p.d_out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h : nullptr;
@@ -260,8 +322,21 @@ __device__ __forceinline__ Vec<T, VEC> zero_unless(bool live, const Vec<T, VEC>&
   return z;
 }
 
-template <int VEC>
-__device__ __forceinline__ void load_carry(const float* src, const Place<VEC>& at, float (&c)[VEC]) {
+// Zeros for the tiles first .. end - 1, which no row of the slab reaches, of dst [B][T][PARTS H].
+template <int PARTS, typename P, typename T>
+__device__ __forceinline__ void zero_tiles(T* dst, const ScanArgs<T>& p, const P& at, int first, int end) {
+  if (!at.on) return;
+  const Vec<T, P::VEC> zero = {};
+  const int t_end = min(end * kTile, p.T_);
+  for (int t = first * kTile + at.tg; t < t_end; t += P::TG) {
+    T* const q = dst + (at.b * p.T_ + t) * (int64_t)(PARTS * p.H) + at.h;
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) store_vec(q + k * p.H, zero);
+  }
+}
+
+template <typename P, int VEC = P::VEC>
+__device__ __forceinline__ void load_carry(const float* src, const P& at, float (&c)[VEC]) {
 #pragma unroll
   for (int j = 0; j < VEC; ++j) c[j] = 0.0f;
   if (!src || !at.on) return;
@@ -270,35 +345,100 @@ __device__ __forceinline__ void load_carry(const float* src, const Place<VEC>& a
   for (int j = 0; j < VEC; ++j) c[j] = v.v[j];
 }
 
-template <int VEC>
-__device__ __forceinline__ void store_carry(float* dst, const Place<VEC>& at, const float (&c)[VEC]) {
+template <typename P, int VEC = P::VEC>
+__device__ __forceinline__ void store_carry(float* dst, const P& at, const float (&c)[VEC]) {
   Vec<float, VEC> v;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) v.v[j] = c[j];
   store_vec(dst + at.n, v);
 }
 
-// Forward.  MAPS: only the segments' maps (of all but the last), for the launch that follows.
-template <typename T, int VEC, bool GATED, bool MAPS>
-__global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs<T> p) {
-  using P = Place<VEC>;
+// The maps of the segments, for the launch that follows: of all but the last in order (of c), or of all but the first
+// in reverse order (of E).  Each time group composes a run of the segment, and the runs are composed once at the end.
+template <typename T, int VEC, int CT, bool REVERSE, bool GATED>
+__global__ void __launch_bounds__(kSlabThreads<CT>) scan_maps_kernel(ScanArgs<T> p) {
+  using P = Place<VEC, CT>;
   constexpr int R = P::R;
-  __shared__ WaveMaps<1> lds;
-  const unsigned slab = blockIdx.x % p.slabs;
-  const int seg = blockIdx.x / p.slabs;
-  const P at(p, slab);
-  float carry[VEC], prod[VEC];
-  load_carry<VEC>(MAPS ? nullptr : p.c0, at, carry);
-  if (!MAPS) fold_segments<T, VEC>(p, at, 0, seg, 1, carry);
+  __shared__ alignas(16) TileMaps<P, 1> lds;
+  const int seg = blockIdx.x / p.slabs + (REVERSE ? 1 : 0);
+  const P at(p, slab_of(blockIdx.x % p.slabs, p.slabs));
+  float A[VEC], B[1][VEC], pa[1][VEC], pb[1][VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) prod[j] = 1.0f;
-  const int tile_end = min(p.tiles, (seg + 1) * p.seg_tiles);
-  Rows<T, VEC, true, GATED && !MAPS, false> x, next;
-  int tile = seg * p.seg_tiles;
-  if (tile < tile_end) next.load(p, at, tile);
-  for (; tile < tile_end; ++tile) {
-    x = next;
-    if (tile + 1 < tile_end) next.load(p, at, tile + 1);
+  for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = 0.0f;
+  const int run = p.seg_tiles * R, first = seg * p.seg_tiles * kTile + at.tg * run;
+  const int steps = min(run, at.len - first);
+  const T* const src = p.gates + at.b * p.stride_b + (int64_t)first * p.stride_t + at.h;
+  const T* const grad = REVERSE ? p.d_out + (at.b * p.T_ + first) * (int64_t)p.H + at.h : nullptr;
+  const auto rows = [&](int t0, auto count) __attribute__((always_inline)) {
+    constexpr int N = decltype(count)::value;
+    Vec<T, VEC> f[N], x[N], o[N];  // x: g, or the gradient of the output
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      const T* const q = src + (int64_t)(t0 + r) * p.stride_t;
+      f[r] = load_vec<T, VEC>(q);
+      x[r] = load_vec<T, VEC>(REVERSE ? grad + (int64_t)(t0 + r) * p.H : q + p.H);
+      if (REVERSE && GATED) o[r] = load_vec<T, VEC>(q + 2 * p.H);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = REVERSE ? N - 1 - i : i;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float s, ns;
+        logistic((float)f[r].v[j], s, ns);
+        float v = (float)x[r].v[j];
+        if (REVERSE) {
+          if (GATED) v *= sigmoid((float)o[r].v[j]);
+          B[0][j] = s * (B[0][j] + v);
+        } else {
+          B[0][j] = fmaf(s, B[0][j], ns * v);
+        }
+        A[j] *= s;
+      }
+    }
+  };
+  using Many = std::integral_constant<int, 4>;
+  using One = std::integral_constant<int, 1>;
+  if (REVERSE) {
+    int t = steps;
+    for (; t % 4 != 0 && t > 0; --t) rows(t - 1, One());
+    for (; t > 0; t -= 4) rows(t - 4, Many());
+  } else {
+    int t = 0;
+    for (; t + 4 <= steps; t += 4) rows(t, Many());
+    for (; t < steps; ++t) rows(t, One());
+  }
+  wave_maps<P, 1, REVERSE>(at.lane, A, B, pa, pb);
+  put_maps<P, 1>(at, lds, A, B);
+  lds_barrier();
+  if (!at.on || at.tg != 0) return;
+  float prod[VEC], sum[VEC], none[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) prod[j] = 1.0f, sum[j] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < P::WAVES; ++w) {
+    const Vec<float, VEC> a = get_lds<VEC>(&lds[w][0][at.ct * VEC]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) prod[j] *= a.v[j];
+  }
+  fold_waves<P, 1, 0, REVERSE>(at, lds, pa[0], pb[0], sum, none);
+  store_carry(p.seg_a + (int64_t)seg * p.channels, at, prod);
+  store_carry(p.seg_b + (int64_t)seg * p.channels, at, sum);
+}
+
+template <typename T, int VEC, int CT, bool GATED>
+__global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan_forward_kernel(ScanArgs<T> p) {
+  using P = Place<VEC, CT>;
+  constexpr int R = P::R;
+  __shared__ alignas(16) WaveMaps<P, 1> lds;
+  const int seg = blockIdx.x / p.slabs;
+  const P at(p, slab_of(blockIdx.x % p.slabs, p.slabs));
+  float carry[VEC];
+  load_carry(p.c0, at, carry);
+  const int tile_first = seg * p.seg_tiles, tile_end = min(p.tiles, (seg + 1) * p.seg_tiles);
+  fold_segments<T, P, 1>(p, at, 0, 1, seg, lds[(tile_first + 1) & 1], carry);
+  using Tile = Rows<T, P, true, GATED, false>;
+  const auto process = [&](const Tile& x, int tile) __attribute__((always_inline)) {
     const int t0 = tile * kTile + at.tg * R;
     float a[R][VEC], b[R][VEC], A[VEC], B[1][VEC], pa[1][VEC], pb[1][VEC];
 #pragma unroll
@@ -314,89 +454,73 @@ __global__ void __launch_bounds__(kScanThreads) scan_forward_kernel(ScanArgs<T> 
         A[j] *= a[r][j];
       }
     }
-    wave_maps<VEC, 1, false>(at.lane, A, B, pa, pb);
+    wave_maps<P, 1, false>(at.lane, A, B, pa, pb);
     auto& maps = lds[tile & 1];
-    put_maps<VEC, 1>(at, maps, A, B);
-    __syncthreads();
-    if (MAPS) {
-#pragma unroll
-      for (int w = 0; w < kScanThreads / kWave; ++w)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) prod[j] *= maps[w][0][at.ct * VEC + j];
-    } else if (p.states && at.on && at.tg == 0) {
-      store_carry<VEC>(p.states + (int64_t)tile * p.channels, at, carry);
-    }
+    put_maps<P, 1>(at, maps, A, B);
+    lds_barrier();
+    if (p.states && at.on && at.tg == 0) store_carry(p.states + (int64_t)tile * p.channels, at, carry);
     float c[VEC];
-    fold_waves<VEC, 1, 0, false>(at, maps, pa[0], pb[0], carry, c);
-    if (!MAPS && at.on) {
-      T* dst = p.out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h;
-      Vec<T, VEC> y[R];
+    fold_waves<P, 1, 0, false>(at, maps, pa[0], pb[0], carry, c);
+    if (!at.on) return;
+    T* dst = p.out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h;
+    Vec<T, VEC> y[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+    for (int r = 0; r < R; ++r) {
+      float h[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          c[j] = fmaf(a[r][j], c[j], b[r][j]);
-          y[r].v[j] = round_to<T>(GATED ? c[j] * sigmoid((float)x.o[r].v[j]) : c[j]);
-        }
+      for (int j = 0; j < VEC; ++j) {
+        c[j] = fmaf(a[r][j], c[j], b[r][j]);
+        h[j] = GATED ? c[j] * sigmoid((float)x.o[r].v[j]) : c[j];
       }
-      if (__all(t0 + R <= at.len)) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) store_vec(dst + (int64_t)r * p.H, y[r]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (t0 + r < p.T_) store_vec(dst + (int64_t)r * p.H, zero_unless(t0 + r < at.len, y[r]));
-      }
+      y[r] = round_to<T, VEC>(h);
     }
-  }
-  if (at.on && at.tg == 0) {
-    if (MAPS) {
-      store_carry<VEC>(p.seg_a + (int64_t)seg * p.channels, at, prod);
-      store_carry<VEC>(p.seg_b + (int64_t)seg * p.channels, at, carry);
-    } else if (seg == p.segs - 1 && p.c_n) {
-      store_carry<VEC>(p.c_n, at, carry);
+    if (__all(t0 + R <= at.len)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) store_vec(dst + (int64_t)r * p.H, y[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (t0 + r < p.T_) store_vec(dst + (int64_t)r * p.H, zero_unless(t0 + r < at.len, y[r]));
     }
+  };
+  const int live_end = min(tile_end, at.live_tiles);
+  Tile x, next;  // a tile's loads are in flight while the one before is computed
+  if (tile_first < live_end) next.load(p, at, tile_first);
+  for (int tile = tile_first; tile < live_end; ++tile) {
+    x = next;
+    if (tile + 1 < live_end) next.load(p, at, tile + 1);
+    process(x, tile);
   }
+  zero_tiles<1>(p.out, p, at, max(tile_first, live_end), tile_end);
+  if (at.on && at.tg == 0 && seg == p.segs - 1 && p.c_n) store_carry(p.c_n, at, carry);
 }
 
-// Backward: tiles from the last to the first.  MAPS: only the segments' maps of E (of all but the first).
-template <typename T, int VEC, bool GATED, bool MAPS>
-__global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs<T> p) {
-  using P = Place<VEC>;
+// Backward: tiles from the last to the first.
+template <typename T, int VEC, int CT, bool GATED>
+__global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArgs<T> p) {
+  using P = Place<VEC, CT>;
   constexpr int R = P::R;
   constexpr int kParts = GATED ? 3 : 2;
-  constexpr int kSums = MAPS ? 1 : 2;  // the sums in reverse order; else first those in order, for c
-  constexpr int kRev = kSums - 1;
-  __shared__ WaveMaps<kSums> lds;
-  const unsigned slab = blockIdx.x % p.slabs;
-  const int seg = blockIdx.x / p.slabs + (MAPS ? 1 : 0);
-  const P at(p, slab);
-  float carry[VEC], prod[VEC];
-  load_carry<VEC>(MAPS ? nullptr : p.d_cn, at, carry);
-  if (!MAPS) fold_segments<T, VEC>(p, at, p.segs - 1, seg, -1, carry);
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) prod[j] = 1.0f;
-  const int tile_first = seg * p.seg_tiles;
-  Rows<T, VEC, !MAPS, GATED, true> x, next;
-  float start[VEC], next_start[VEC];
-  int tile = min(p.tiles, (seg + 1) * p.seg_tiles) - 1;
-  if (tile >= tile_first) {
-    next.load(p, at, tile);
-    load_carry<VEC>(MAPS ? nullptr : p.states + (int64_t)tile * p.channels, at, next_start);
-  }
-  for (; tile >= tile_first; --tile) {
-    x = next;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) start[j] = next_start[j];
-    if (tile > tile_first) {
-      next.load(p, at, tile - 1);
-      load_carry<VEC>(MAPS ? nullptr : p.states + (int64_t)(tile - 1) * p.channels, at, next_start);
+  __shared__ alignas(16) WaveMaps<P, 2> lds;
+  const int seg = blockIdx.x / p.slabs;
+  const P at(p, slab_of(blockIdx.x % p.slabs, p.slabs));
+  float carry[VEC];
+  load_carry(p.d_cn, at, carry);
+  const int tile_first = seg * p.seg_tiles, tile_last = min(p.tiles, (seg + 1) * p.seg_tiles) - 1;
+  fold_segments<T, P, 2>(p, at, p.segs - 1, -1, p.segs - 1 - seg, lds[(tile_last + 1) & 1], carry);
+  struct Tile : Rows<T, P, true, GATED, true> {
+    float start[VEC];  // c before the tile, from the forward pass
+    __device__ __forceinline__ void load(const ScanArgs<T>& p, const P& at, int tile) {
+      Rows<T, P, true, GATED, true>::load(p, at, tile);
+      load_carry(p.states + (int64_t)tile * p.channels, at, start);
     }
+  };
+  const auto process = [&](const Tile& x, int tile) __attribute__((always_inline)) {
     const int t0 = tile * kTile + at.tg * R;
     float a[R][VEC], na[R][VEC], u[R][VEC], w[R][VEC];  // a, 1 - a, u = s dh, w = (1 - s) u
-    float A[VEC], B[kSums][VEC], pa[kSums][VEC], pb[kSums][VEC];
+    float A[VEC], B[2][VEC], pa[2][VEC], pb[2][VEC];    // sums in order (for c) and in reverse order (for E)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = B[kRev][j] = 0.0f;
+    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = B[1][j] = 0.0f;
 #pragma unroll
     for (int r = R - 1; r >= 0; --r) {
 #pragma unroll
@@ -409,151 +533,168 @@ __global__ void __launch_bounds__(kScanThreads) scan_backward_kernel(ScanArgs<T>
           u[r][j] *= s;
           w[r][j] = ns * u[r][j];
         }
-        B[kRev][j] = a[r][j] * (B[kRev][j] + u[r][j]);
+        B[1][j] = a[r][j] * (B[1][j] + u[r][j]);
         A[j] *= a[r][j];
       }
     }
-    if (!MAPS) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) B[0][j] = fmaf(a[r][j], B[0][j], na[r][j] * (float)x.g[r].v[j]);
-    }
-    wave_maps<VEC, kSums, MAPS>(at.lane, A, B, pa, pb);
+      for (int j = 0; j < VEC; ++j) B[0][j] = fmaf(a[r][j], B[0][j], na[r][j] * (float)x.g[r].v[j]);
+    wave_maps<P, 2, false>(at.lane, A, B, pa, pb);
     auto& maps = lds[tile & 1];
-    put_maps<VEC, kSums>(at, maps, A, B);
-    __syncthreads();
-    if (MAPS) {
+    put_maps<P, 2>(at, maps, A, B);
+    lds_barrier();
+    float e[VEC], start[VEC], c[VEC], before[R][VEC];
+    fold_waves<P, 2, 1, true>(at, maps, pa[1], pb[1], carry, e);
+    if (!at.on) return;
 #pragma unroll
-      for (int i = 0; i < kScanThreads / kWave; ++i)
+    for (int j = 0; j < VEC; ++j) start[j] = x.start[j];
+    fold_waves<P, 2, 0, false>(at, maps, pa[0], pb[0], start, c);
+    Vec<T, VEC> df[R], dg[R], d_o[R];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) prod[j] *= maps[i][0][at.ct * VEC + j];
+    for (int r = 0; r < R; ++r) {
+      float d[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        before[r][j] = c[j];
+        c[j] = fmaf(a[r][j], c[j], na[r][j] * (float)x.g[r].v[j]);
+        d[j] = GATED ? w[r][j] * c[j] : 0.0f;
+      }
+      if (GATED) d_o[r] = round_to<T, VEC>(d);
     }
-    float e[VEC];
-    fold_waves<VEC, kSums, kRev, true>(at, maps, pa[kRev], pb[kRev], carry, e);
-    if (!MAPS && at.on) {
-      // c before each of this thread's steps, from the state that the forward pass left at the tile's start
-      float c[VEC], before[R][VEC];
-      fold_waves<VEC, kSums, 0, false>(at, maps, pa[0], pb[0], start, c);
-      Vec<T, VEC> df[R], dg[R], d_o[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+    for (int r = R - 1; r >= 0; --r) {
+      float n[VEC], m[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          before[r][j] = c[j];
-          c[j] = fmaf(a[r][j], c[j], na[r][j] * (float)x.g[r].v[j]);
-          if (GATED) d_o[r].v[j] = round_to<T>(w[r][j] * c[j]);
-        }
+      for (int j = 0; j < VEC; ++j) {
+        const float D = u[r][j] + e[j];
+        n[j] = na[r][j] * D;
+        e[j] = a[r][j] * D;
+        m[j] = a[r][j] * n[j] * (before[r][j] - (float)x.g[r].v[j]);
       }
+      dg[r] = round_to<T, VEC>(n);
+      df[r] = round_to<T, VEC>(m);
+    }
+    T* const dst = p.d_gates + (at.b * p.T_ + t0) * (int64_t)(kParts * p.H) + at.h;
+    const bool all = __all(t0 + R <= at.len);
 #pragma unroll
-      for (int r = R - 1; r >= 0; --r) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float D = u[r][j] + e[j];
-          const float n = na[r][j] * D;
-          e[j] = a[r][j] * D;
-          dg[r].v[j] = round_to<T>(n);
-          df[r].v[j] = round_to<T>(a[r][j] * n * (before[r][j] - (float)x.g[r].v[j]));
-        }
-      }
-      T* const dst = p.d_gates + (at.b * p.T_ + t0) * (int64_t)(kParts * p.H) + at.h;
-      const bool all = __all(t0 + R <= at.len);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        T* const q = dst + (int64_t)r * (kParts * p.H);
-        if (all) {
-          store_vec(q, df[r]);
-          store_vec(q + p.H, dg[r]);
-          if (GATED) store_vec(q + 2 * p.H, d_o[r]);
-        } else if (t0 + r < p.T_) {
-          const bool live = t0 + r < at.len;
-          store_vec(q, zero_unless(live, df[r]));
-          store_vec(q + p.H, zero_unless(live, dg[r]));
-          if (GATED) store_vec(q + 2 * p.H, zero_unless(live, d_o[r]));
-        }
+    for (int r = 0; r < R; ++r) {
+      T* const q = dst + (int64_t)r * (kParts * p.H);
+      if (all) {
+        store_vec(q, df[r]);
+        store_vec(q + p.H, dg[r]);
+        if (GATED) store_vec(q + 2 * p.H, d_o[r]);
+      } else if (t0 + r < p.T_) {
+        const bool live = t0 + r < at.len;
+        store_vec(q, zero_unless(live, df[r]));
+        store_vec(q + p.H, zero_unless(live, dg[r]));
+        if (GATED) store_vec(q + 2 * p.H, zero_unless(live, d_o[r]));
       }
     }
+  };
+  zero_tiles<kParts>(p.d_gates, p, at, max(tile_first, at.live_tiles), tile_last + 1);
+  const int live_last = min(tile_last, at.live_tiles - 1);
+  Tile x, next;  // (as in the forward kernel)
+  if (live_last >= tile_first) next.load(p, at, live_last);
+  for (int tile = live_last; tile >= tile_first; --tile) {
+    x = next;
+    if (tile > tile_first) next.load(p, at, tile - 1);
+    process(x, tile);
   }
-  if (at.on && at.tg == 0) {
-    if (MAPS) {
-      store_carry<VEC>(p.seg_a + (int64_t)seg * p.channels, at, prod);
-      store_carry<VEC>(p.seg_b + (int64_t)seg * p.channels, at, carry);
-    } else if (seg == 0 && p.d_c0) {
-      store_carry<VEC>(p.d_c0, at, carry);
-    }
-  }
+  if (at.on && at.tg == 0 && seg == 0 && p.d_c0) store_carry(p.d_c0, at, carry);
 }
+
+constexpr int kStepThreads = 256;
 
 // One step of every row, for serving: a thread per VEC channels, nothing to scan.  (The tiled kernel would leave 63 of
 // 64 steps idle: 20.4 us for 512 rows of 512 channels in bfloat16.)
 template <typename T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanArgs<T> p) {
-  const int64_t n = ((int64_t)blockIdx.x * kScanThreads + threadIdx.x) * VEC;
-  if (n >= p.channels) return;
-  const uint32_t b = (uint32_t)n / (uint32_t)p.H, h = (uint32_t)n % (uint32_t)p.H;  // (channels <= 2^29)
-  Vec<float, VEC> c = {};
-  if (p.c0) c = load_vec<float, VEC>(p.c0 + n);
-  if (p.states) store_vec(p.states + n, c);
-  Vec<T, VEC> y = {};
-  if (!p.lengths || p.lengths[b] > 0) {
-    const T* const src = p.gates + b * p.stride_b + h;
-    const Vec<T, VEC> f = load_vec<T, VEC>(src), g = load_vec<T, VEC>(src + p.H);
-    Vec<T, VEC> o = {};
-    if (GATED) o = load_vec<T, VEC>(src + 2 * p.H);
+__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanArgs<T> p) {
+  const uint32_t piece = blockIdx.x * kStepThreads + threadIdx.x, per = (p.H + VEC - 1) / VEC;
+  if (piece >= p.pieces) return;
+  const int64_t b = piece / per;
+  const int h = (int)(piece % per) * VEC;
+  const bool on = !p.lengths || p.lengths[b] > 0;
+  const auto step = [&](auto width, int h) __attribute__((always_inline)) {
+    constexpr int N = decltype(width)::value;
+    const int64_t n = b * p.H + h;
+    Vec<float, N> c = {};
+    if (p.c0) c = load_vec<float, N>(p.c0 + n);
+    if (p.states) store_vec(p.states + n, c);
+    Vec<T, N> y = {};
+    if (on) {
+      const T* const src = p.gates + b * p.stride_b + h;
+      const Vec<T, N> f = load_vec<T, N>(src), g = load_vec<T, N>(src + p.H);
+      Vec<T, N> o = {};
+      if (GATED) o = load_vec<T, N>(src + 2 * p.H);
+      float out[N];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      float a, na;
-      logistic((float)f.v[j], a, na);
-      c.v[j] = fmaf(a, c.v[j], na * (float)g.v[j]);
-      y.v[j] = round_to<T>(GATED ? c.v[j] * sigmoid((float)o.v[j]) : c.v[j]);
+      for (int j = 0; j < N; ++j) {
+        float a, na;
+        logistic((float)f.v[j], a, na);
+        c.v[j] = fmaf(a, c.v[j], na * (float)g.v[j]);
+        out[j] = GATED ? c.v[j] * sigmoid((float)o.v[j]) : c.v[j];
+      }
+      y = round_to<T, N>(out);
     }
+    if (p.c_n) store_vec(p.c_n + n, c);
+    store_vec(p.out + n, y);
+  };
+  if (h + VEC <= p.H) {
+    step(std::integral_constant<int, VEC>(), h);
+  } else {  // (c_n may be c0, so no channel may be another thread's too)
+    for (int k = h; k < p.H; ++k) step(std::integral_constant<int, 1>(), k);
   }
-  if (p.c_n) store_vec(p.c_n + n, c);
-  store_vec(p.out + n, y);
 }
 
 template <typename T, int VEC, bool GATED>
 hipError_t launch_forward(const ScanArgs<T>& p, hipStream_t s) {
+  constexpr int CT = VEC == 4 ? 16 : 64, kThreads = Place<VEC, CT>::THREADS;
   if (p.T_ == 1) {
-    const int64_t threads = (p.channels + VEC - 1) / VEC;
-    hipLaunchKernelGGL((scan_step_kernel<T, VEC, GATED>), dim3((unsigned)((threads + kScanThreads - 1) / kScanThreads)),
-                       dim3(kScanThreads), 0, s, p);
+    hipLaunchKernelGGL((scan_step_kernel<T, VEC, GATED>), dim3((p.pieces + kStepThreads - 1) / kStepThreads),
+                       dim3(kStepThreads), 0, s, p);
     return hipGetLastError();
   }
   if (p.segs > 1) {
-    hipLaunchKernelGGL((scan_forward_kernel<T, VEC, GATED, true>), dim3(p.slabs * (unsigned)(p.segs - 1)),
-                       dim3(kScanThreads), 0, s, p);
+    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, false, false>), dim3(p.slabs * (unsigned)(p.segs - 1)),
+                       dim3(kThreads), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((scan_forward_kernel<T, VEC, GATED, false>), dim3(p.slabs * (unsigned)p.segs), dim3(kScanThreads),
-                     0, s, p);
+  hipLaunchKernelGGL((scan_forward_kernel<T, VEC, CT, GATED>), dim3(p.slabs * (unsigned)p.segs), dim3(kThreads), 0, s,
+                     p);
   return hipGetLastError();
+}
+
+// Whether the backward pass takes slabs of 128 channels in 512 threads: rows of 16-bit elements are then read 256 bytes
+// at a time instead of 128, with one workgroup per CU and no split.  16 x 4096 x 2048 bf16: 411 -> 353 us.  Rows that
+// are hardly longer gain nothing (512 x 1000 x 128: 189 and 190 us), a time axis that has to be split loses (33 x
+// 1001 x 333: 70 and 77 us), and the forward pass loses too (243 and 269 us).
+template <typename T>
+bool wide_slabs(const ScanArgs<T>& p) {
+  return sizeof(T) == 2 && p.H >= 256 && p.slabs >= 512 && p.segs == 1;
 }
 
 template <typename T, int VEC, bool GATED>
-hipError_t launch_backward(const ScanArgs<T>& p, hipStream_t s) {
+hipError_t launch_backward(ScanArgs<T> p, hipStream_t s) {
+  constexpr int CT = VEC == 4 ? 16 : 64, kThreads = Place<VEC, CT>::THREADS;
+  if constexpr (sizeof(T) == 2 && VEC == 4) {
+    if (wide_slabs(p)) {
+      p.slabs = (p.pieces + 31) / 32;
+      hipLaunchKernelGGL((scan_backward_kernel<T, 4, 32, GATED>), dim3(p.slabs), dim3(Place<4, 32>::THREADS), 0, s, p);
+      return hipGetLastError();
+    }
+  }
   if (p.segs > 1) {
-    hipLaunchKernelGGL((scan_backward_kernel<T, VEC, GATED, true>), dim3(p.slabs * (unsigned)(p.segs - 1)),
-                       dim3(kScanThreads), 0, s, p);
+    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, true, GATED>), dim3(p.slabs * (unsigned)(p.segs - 1)),
+                       dim3(kThreads), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((scan_backward_kernel<T, VEC, GATED, false>), dim3(p.slabs * (unsigned)p.segs), dim3(kScanThreads),
-                     0, s, p);
+  hipLaunchKernelGGL((scan_backward_kernel<T, VEC, CT, GATED>), dim3(p.slabs * (unsigned)p.segs), dim3(kThreads), 0, s,
+                     p);
   return hipGetLastError();
-}
-
-// Channels per thread: the widest of 4, 2 and 1 at which every access of a row is aligned.
-template <typename T>
-int scan_vec(const ScanArgs<T>& p) {
-  for (int v : {4, 2})
-    if (p.H % v == 0 && p.stride_b % v == 0 && p.stride_t % v == 0 && aligned<T>(p.gates, v) && aligned<T>(p.out, v) &&
-        aligned<T>(p.d_out, v) && aligned<T>(p.d_gates, v) && aligned<float>(p.c0, v) && aligned<float>(p.c_n, v) &&
-        aligned<float>(p.states, v) && aligned<float>(p.seg_a, v) && aligned<float>(p.seg_b, v) &&
-        aligned<float>(p.d_cn, v) && aligned<float>(p.d_c0, v))
-      return v;
-  return 1;
 }
 
 template <typename T, bool BACKWARD>
@@ -565,11 +706,7 @@ hipError_t launch_scan(const ScanArgs<T>& p, bool gated, hipStream_t s) {
     else
       return gated ? launch_forward<T, V, true>(p, s) : launch_forward<T, V, false>(p, s);
   };
-  switch (scan_vec(p)) {
-    case 4: return go(std::integral_constant<int, 4>());
-    case 2: return go(std::integral_constant<int, 2>());
-    default: return go(std::integral_constant<int, 1>());
-  }
+  return scan_vec(p.H) == 4 ? go(std::integral_constant<int, 4>()) : go(std::integral_constant<int, 1>());
 }
 
 // The checks that both directions share; PLH_OK or the error code.
@@ -586,7 +723,7 @@ int check_scan(const char* what, int dtype, const void* gates, int64_t stride_b,
   const int64_t need = plh_gated_scan_workspace_bytes(batch, seq_len, hidden);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return op_error(PLH_ERR_INVALID, what, "workspace missing or smaller than plh_gated_scan_workspace_bytes()");
-  if (!aligned<float>(workspace, 4)) return op_error(PLH_ERR_INVALID, what, "workspace must be 16-byte aligned");
+  if (!aligned(workspace, 16)) return op_error(PLH_ERR_INVALID, what, "workspace must be 16-byte aligned");
   return PLH_OK;
 }
 
@@ -601,6 +738,7 @@ ScanArgs<T> scan_args(const void* gates, int64_t stride_b, int64_t stride_t, int
   p.T_ = (int)seq_len, p.H = hidden;
   p.tiles = sp.tiles, p.seg_tiles = sp.seg_tiles, p.segs = sp.segs;
   p.slabs = (unsigned)slabs_of(batch, hidden);
+  p.pieces = (unsigned)pieces_of(batch, hidden);
   p.lengths = lengths;
   p.seg_a = (float*)workspace;
   p.seg_b = p.seg_a ? p.seg_a + (p.channels * sp.segs + 3) / 4 * 4 : nullptr;
