@@ -40,7 +40,7 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
   if constexpr (LPR > kWave) {
     constexpr int N = LPR / kWave;
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
+    lds_barrier();
     v = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) v += lds[i];
@@ -61,109 +61,168 @@ __device__ __forceinline__ void load_param(const void* p, bool p32, int c, float
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[j] = fill;
   } else if (p32) {
+    const Vec<float, VEC> t = load_vec<float, VEC>(static_cast<const float*>(p) + c);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = static_cast<const float*>(p)[c + j];
+    for (int j = 0; j < VEC; ++j) v[j] = t.v[j];
   } else {
+    const Vec<T, VEC> t = load_vec<T, VEC>(static_cast<const T*>(p) + c);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = (float)static_cast<const T*>(p)[c + j];
+    for (int j = 0; j < VEC; ++j) v[j] = (float)t.v[j];
   }
 }
 
-// LPR threads per row, each with NV pieces of VEC neighbouring columns: piece i of thread l starts at column
-// (i LPR + l) VEC.  A workgroup takes rows until none is left and keeps weight and bias in registers.
-template <typename T, int VEC, int LPR, int NV>
-__global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_forward_kernel(NormArgs p) {
-  constexpr int kThreads = LPR > 256 ? LPR : 256, kRows = kThreads / LPR;
+// LPR threads per row, each with NV pieces of VEC neighbouring columns: piece i of thread l is number i LPR + l.  The
+// last piece of a row is moved back to end with it; its first `skip` elements then belong to the piece before: they
+// are computed and stored by both, and counted once.
+template <int VEC, int LPR, int NV>
+struct Pieces {
+  int col[NV];  // first column; -1: none
+  int skip;     // of the thread's last piece
+
+  __device__ __forceinline__ explicit Pieces(int cols) {
+    skip = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LPR + (int)threadIdx.x % LPR) * VEC;
+      col[i] = c < cols ? min(c, cols - VEC) : -1;
+      if (c < cols) skip = c - col[i];
+    }
+  }
+  // Whether element j of piece i counts.  (Only a thread's last piece can be the row's.)
+  __device__ __forceinline__ bool counts(int i, int j) const {
+    return j >= skip || (i + 1 < NV && col[i + 1] >= 0);
+  }
+};
+
+template <int LPR>
+constexpr int kNormThreads = LPR > 256 ? LPR : 256;
+
+// A workgroup takes rows until none is left, keeps weight and bias in registers, and loads its next row while it
+// reduces the one before.  TAIL: VEC does not divide the row length.
+template <typename T, int VEC, int LPR, int NV, bool TAIL>
+__global__ void __launch_bounds__(kNormThreads<LPR>) norm_forward_kernel(NormArgs p) {
+  constexpr int kThreads = kNormThreads<LPR>, kRows = kThreads / LPR;
   __shared__ float lds[2][kThreads / kWave];
-  const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+  const Pieces<VEC, LPR, NV> at(p.cols);
   float w[NV][VEC], b[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * LPR + l) * VEC;
-    if (c < p.cols) {
-      load_param<T, VEC>(p.weight, p.w32, c, 1.0f, w[i]);
-      load_param<T, VEC>(p.bias, p.w32, c, 0.0f, b[i]);
+    if (at.col[i] >= 0) {
+      load_param<T, VEC>(p.weight, p.w32, at.col[i], 1.0f, w[i]);
+      load_param<T, VEC>(p.bias, p.w32, at.col[i], 0.0f, b[i]);
     }
   }
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t r = base + sub;
-    const bool on = r < p.rows;
+  Vec<T, VEC> next[NV] = {};
+  const auto load = [&](int64_t r) __attribute__((always_inline)) {
+    if (r >= p.rows) return;
     const T* const src = static_cast<const T*>(p.x) + r * p.stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (at.col[i] >= 0) next[i] = load_vec<T, VEC>(src + at.col[i]);
+  };
+  int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / LPR;
+  const int64_t step = (int64_t)gridDim.x * kRows, rounds = (p.rows + step - 1) / step;
+  load(r);
+  for (int64_t k = 0; k < rounds; ++k, r += step) {
     float x[NV][VEC], sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + l) * VEC;
-      Vec<T, VEC> t = {};
-      if (on && c < p.cols) t = load_vec<T, VEC>(src + c);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum += x[i][j] = (float)t.v[j];
+      for (int j = 0; j < VEC; ++j) {
+        x[i][j] = at.col[i] >= 0 ? (float)next[i].v[j] : 0.0f;
+        sum += !TAIL || at.counts(i, j) ? x[i][j] : 0.0f;
+      }
     }
+    if (k + 1 < rounds) load(r + step);
     const float mean = mean_of(row_sum<LPR>(sum, lds[0]), p);
     float sq = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if ((i * LPR + l) * VEC < p.cols) {
+      if (at.col[i] >= 0) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           x[i][j] -= mean;
-          sq = fmaf(x[i][j], x[i][j], sq);
+          if (!TAIL || at.counts(i, j)) sq = fmaf(x[i][j], x[i][j], sq);
         }
       }
     }
     const float rstd = 1.0f / __builtin_sqrtf(fmaf(row_sum<LPR>(sq, lds[1]), p.inv_cols, p.eps));
-    if (!on) continue;
+    if (r >= p.rows) continue;  // (kRows > 1 only: no barrier is skipped)
     T* const dst = static_cast<T*>(p.y) + r * p.cols;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + l) * VEC;
-      if (c < p.cols) {
-        Vec<T, VEC> t;
+      if (at.col[i] >= 0) {
+        float y[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) t.v[j] = round_to<T>(fmaf(x[i][j] * rstd, w[i][j], b[i][j]));
-        store_vec(dst + c, t);
+        for (int j = 0; j < VEC; ++j) y[j] = fmaf(x[i][j] * rstd, w[i][j], b[i][j]);
+        store_vec(dst + at.col[i], round_to<T, VEC>(y));
       }
     }
-    if (l == 0) {
+    if (threadIdx.x % LPR == 0) {
       if (p.mean) p.mean[r] = mean;
       if (p.rstd) p.rstd[r] = rstd;
     }
   }
 }
 
-template <typename T, int VEC, int LPR, int NV>
-__global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_backward_kernel(NormArgs p) {
-  constexpr int kThreads = LPR > 256 ? LPR : 256, kRows = kThreads / LPR;
+// Backward.  A row is held as it was loaded and converted again for its second use: that keeps the 16-bit kernels, with
+// the next row in flight, at 128 registers and so four waves per SIMD.  32-bit elements take more, and where a
+// workgroup's registers run out (1024 threads; 512 with 16 32-bit elements each) the next row is not loaded ahead.
+template <typename T, int VEC, int LPR, int NV, bool TAIL>
+__global__ void __launch_bounds__(kNormThreads<LPR>, sizeof(T) == 2 || LPR == 1024 ? 4 : 3)
+    norm_backward_kernel(NormArgs p) {
+  constexpr int kThreads = kNormThreads<LPR>, kRows = kThreads / LPR;
+  constexpr bool kAhead = LPR < (VEC * NV * sizeof(T) > 32 ? 512 : 1024);
   __shared__ float lds[2][kThreads / kWave];
-  const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+  const Pieces<VEC, LPR, NV> at(p.cols);
   float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * LPR + l) * VEC;
-    if (c < p.cols) load_param<T, VEC>(p.weight, p.w32, c, 1.0f, w[i]);
+    if (at.col[i] >= 0) load_param<T, VEC>(p.weight, p.w32, at.col[i], 1.0f, w[i]);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.0f;
   }
-  for (int64_t base = (int64_t)blockIdx.x * kRows; base < p.rows; base += (int64_t)gridDim.x * kRows) {
-    const int64_t r = base + sub;
-    const bool on = r < p.rows;
+  struct Row {
+    Vec<T, VEC> x[NV], g[NV];
+    float mean, rstd;
+  } row = {}, next = {};
+  const auto load = [&](Row& to, int64_t r) __attribute__((always_inline)) {
+    if (r >= p.rows) return;
     const T* const src = static_cast<const T*>(p.x) + r * p.stride;
     const T* const grad = static_cast<const T*>(p.d_y) + r * p.cols;
-    const float mean = on ? p.mean[r] : 0.0f, rstd = on ? p.rstd[r] : 0.0f;
-    float xh[NV][VEC], v[NV][VEC], s1 = 0.0f, s2 = 0.0f;
+    to.mean = p.mean[r], to.rstd = p.rstd[r];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + l) * VEC;
-      if (on && c < p.cols) {
-        const Vec<T, VEC> tx = load_vec<T, VEC>(src + c), tg = load_vec<T, VEC>(grad + c);
+      if (at.col[i] >= 0) {
+        to.x[i] = load_vec<T, VEC>(src + at.col[i]);
+        to.g[i] = load_vec<T, VEC>(grad + at.col[i]);
+      }
+    }
+  };
+  int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / LPR;
+  const int64_t step = (int64_t)gridDim.x * kRows, rounds = (p.rows + step - 1) / step;
+  if (kAhead) load(next, r);
+  for (int64_t k = 0; k < rounds; ++k, r += step) {
+    const bool on = r < p.rows;
+    if (kAhead) {
+      row = next;
+      if (k + 1 < rounds) load(next, r + step);
+    } else {
+      load(row, r);
+    }
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (on && at.col[i] >= 0) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float g = (float)tg.v[j];
-          xh[i][j] = ((float)tx.v[j] - mean) * rstd;
-          v[i][j] = g * w[i][j];
-          dw[i][j] = fmaf(g, xh[i][j], dw[i][j]);
+          const float g = (float)row.g[i].v[j], xh = ((float)row.x[i].v[j] - row.mean) * row.rstd, v = g * w[i][j];
+          dw[i][j] = fmaf(g, xh, dw[i][j]);
           db[i][j] += g;
-          s1 += v[i][j];
-          s2 = fmaf(v[i][j], xh[i][j], s2);
+          if (!TAIL || at.counts(i, j)) {
+            s1 += v;
+            s2 = fmaf(v, xh, s2);
+          }
         }
       }
     }
@@ -172,34 +231,36 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_backward_kernel(No
     T* const dst = static_cast<T*>(p.d_x) + r * p.cols;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + l) * VEC;
-      if (c < p.cols) {
-        Vec<T, VEC> t;
+      if (at.col[i] >= 0) {
+        float d[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) t.v[j] = round_to<T>(rstd * (v[i][j] - m1 - xh[i][j] * m2));
-        store_vec(dst + c, t);
+        for (int j = 0; j < VEC; ++j) {
+          const float xh = ((float)row.x[i].v[j] - row.mean) * row.rstd;
+          d[j] = row.rstd * ((float)row.g[i].v[j] * w[i][j] - m1 - xh * m2);
+        }
+        store_vec(dst + at.col[i], round_to<T, VEC>(d));
       }
     }
   }
   if (!p.part) return;
   // The rows of a workgroup that ran side by side are summed in their order, then written as one row of partial sums.
   __shared__ float sums[kRows > 1 ? kThreads * VEC * NV : 1];
+  const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
   float* const out = p.part + (int64_t)blockIdx.x * 2 * p.cols;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if constexpr (kRows > 1) {
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sums[(sub * NV * VEC + i * VEC + j) * LPR + l] = k ? db[i][j] : dw[i][j];
-      __syncthreads();
+      lds_barrier();
     }
     if (sub == 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + l) * VEC;
-        if (c < p.cols) {
+        if (at.col[i] >= 0) {
           Vec<float, VEC> t;
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
@@ -208,37 +269,56 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_backward_kernel(No
               for (int q = 1; q < kRows; ++q) s += sums[(q * NV * VEC + i * VEC + j) * LPR + l];
             t.v[j] = s;
           }
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) out[(int64_t)k * p.cols + c + j] = t.v[j];
+          store_vec(out + (int64_t)k * p.cols + at.col[i], t);
         }
       }
     }
   }
 }
 
-// Rows too long for registers: a workgroup per row, which reads it once per sum.
+// Rows too long for registers: a workgroup per row, which reads it once per sum (again from its XCD's L2: 2000 rows of
+// 40000 bf16).
 constexpr int kWideThreads = 1024;
 
-template <typename T>
+// f(vector of N elements' first column) over the thread's columns of a row, whole vectors first.
+template <int VEC, typename F>
+__device__ __forceinline__ void over_row(int cols, F&& f) {
+  const int whole = cols / VEC * VEC;
+  for (int c = threadIdx.x * VEC; c < whole; c += kWideThreads * VEC) f(c, std::integral_constant<int, VEC>());
+  if (whole + (int)threadIdx.x < cols) f(whole + (int)threadIdx.x, std::integral_constant<int, 1>());
+}
+
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(NormArgs p) {
   __shared__ float lds[2][kWideThreads / kWave];
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const T* const src = static_cast<const T*>(p.x) + r * p.stride;
     float s = 0.0f;
-    for (int c = threadIdx.x; c < p.cols; c += kWideThreads) s += (float)src[c];
+    over_row<VEC>(p.cols, [&](int c, auto n) {
+      constexpr int N = decltype(n)::value;
+      const Vec<T, N> x = load_vec<T, N>(src + c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += (float)x.v[j];
+    });
     const float mean = mean_of(row_sum<kWideThreads>(s, lds[0]), p);
     s = 0.0f;
-    for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
-      const float d = (float)src[c] - mean;
-      s = fmaf(d, d, s);
-    }
+    over_row<VEC>(p.cols, [&](int c, auto n) {
+      constexpr int N = decltype(n)::value;
+      const Vec<T, N> x = load_vec<T, N>(src + c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s = fmaf((float)x.v[j] - mean, (float)x.v[j] - mean, s);
+    });
     const float rstd = 1.0f / __builtin_sqrtf(fmaf(row_sum<kWideThreads>(s, lds[1]), p.inv_cols, p.eps));
-    for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
-      float w[1], b[1];
-      load_param<T, 1>(p.weight, p.w32, c, 1.0f, w);
-      load_param<T, 1>(p.bias, p.w32, c, 0.0f, b);
-      static_cast<T*>(p.y)[r * p.cols + c] = round_to<T>(fmaf(((float)src[c] - mean) * rstd, w[0], b[0]));
-    }
+    over_row<VEC>(p.cols, [&](int c, auto n) {
+      constexpr int N = decltype(n)::value;
+      const Vec<T, N> x = load_vec<T, N>(src + c);
+      float w[N], b[N], y[N];
+      load_param<T, N>(p.weight, p.w32, c, 1.0f, w);
+      load_param<T, N>(p.bias, p.w32, c, 0.0f, b);
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[j] = fmaf(((float)x.v[j] - mean) * rstd, w[j], b[j]);
+      store_vec(static_cast<T*>(p.y) + r * p.cols + c, round_to<T, N>(y));
+    });
     if (threadIdx.x == 0) {
       if (p.mean) p.mean[r] = mean;
       if (p.rstd) p.rstd[r] = rstd;
@@ -246,7 +326,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(NormArg
   }
 }
 
-template <typename T>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(NormArgs p) {
   __shared__ float lds[2][kWideThreads / kWave];
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -254,40 +334,59 @@ __global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(NormAr
     const T* const grad = static_cast<const T*>(p.d_y) + r * p.cols;
     const float mean = p.mean[r], rstd = p.rstd[r];
     float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
-      float w[1];
-      load_param<T, 1>(p.weight, p.w32, c, 1.0f, w);
-      const float v = (float)grad[c] * w[0];
-      s1 += v;
-      s2 = fmaf(v, ((float)src[c] - mean) * rstd, s2);
-    }
+    over_row<VEC>(p.cols, [&](int c, auto n) {
+      constexpr int N = decltype(n)::value;
+      const Vec<T, N> x = load_vec<T, N>(src + c), g = load_vec<T, N>(grad + c);
+      float w[N];
+      load_param<T, N>(p.weight, p.w32, c, 1.0f, w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float v = (float)g.v[j] * w[j];
+        s1 += v;
+        s2 = fmaf(v, ((float)x.v[j] - mean) * rstd, s2);
+      }
+    });
     const float m1 = row_sum<kWideThreads>(s1, lds[0]) * p.inv_cols;
     const float m2 = row_sum<kWideThreads>(s2, lds[1]) * p.inv_cols;
-    for (int c = threadIdx.x; c < p.cols; c += kWideThreads) {
-      float w[1];
-      load_param<T, 1>(p.weight, p.w32, c, 1.0f, w);
-      const float xh = ((float)src[c] - mean) * rstd;
-      static_cast<T*>(p.d_x)[r * p.cols + c] = round_to<T>(rstd * ((float)grad[c] * w[0] - m1 - xh * m2));
-    }
+    over_row<VEC>(p.cols, [&](int c, auto n) {
+      constexpr int N = decltype(n)::value;
+      const Vec<T, N> x = load_vec<T, N>(src + c), g = load_vec<T, N>(grad + c);
+      float w[N], d[N];
+      load_param<T, N>(p.weight, p.w32, c, 1.0f, w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float xh = ((float)x.v[j] - mean) * rstd;
+        d[j] = rstd * ((float)g.v[j] * w[j] - m1 - xh * m2);
+      }
+      store_vec(static_cast<T*>(p.d_x) + r * p.cols + c, round_to<T, N>(d));
+    });
   }
 }
 
-// The workgroups' sums for such rows: a thread per column, the rows in as many runs as there are groups.
-template <typename T>
+// The workgroups' sums for such rows: VEC columns per thread (the last thread's moved back to end with the row, as
+// above), the rows in as many runs as there are groups.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) norm_columns_kernel(NormArgs p) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  int c = (blockIdx.x * 256 + threadIdx.x) * VEC;
   if (c >= p.cols) return;
+  c = min(c, p.cols - VEC);
   const int64_t per = (p.rows + p.groups - 1) / p.groups;
   const int64_t end = min(p.rows, (blockIdx.y + 1) * per);
-  float dw = 0.0f, db = 0.0f;
+  Vec<float, VEC> dw = {}, db = {};
+#pragma unroll 2
   for (int64_t r = blockIdx.y * per; r < end; ++r) {
-    const float g = (float)static_cast<const T*>(p.d_y)[r * p.cols + c];
-    dw = fmaf(g, ((float)static_cast<const T*>(p.x)[r * p.stride + c] - p.mean[r]) * p.rstd[r], dw);
-    db += g;
+    const Vec<T, VEC> x = load_vec<T, VEC>(static_cast<const T*>(p.x) + r * p.stride + c);
+    const Vec<T, VEC> g = load_vec<T, VEC>(static_cast<const T*>(p.d_y) + r * p.cols + c);
+    const float mean = p.mean[r], rstd = p.rstd[r];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      dw.v[j] = fmaf((float)g.v[j], ((float)x.v[j] - mean) * rstd, dw.v[j]);
+      db.v[j] += (float)g.v[j];
+    }
   }
   float* const out = p.part + (int64_t)blockIdx.y * 2 * p.cols;
-  out[c] = dw;
-  out[(int64_t)p.cols + c] = db;
+  store_vec(out + c, dw);
+  store_vec(out + p.cols + c, db);
 }
 
 // Sums over the workgroups, in a fixed order: 32 threads per column.
@@ -302,7 +401,7 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(NormArgs p) {
     for (int g = q; g < p.groups; g += 32) s += p.part[g * n + c];
   }
   lds[q][threadIdx.x % 32] = s;
-  __syncthreads();
+  lds_barrier();
   if (q != 0 || c >= n) return;
   s = 0.0f;
 #pragma unroll
@@ -316,7 +415,12 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(NormArgs p) {
     static_cast<T*>(dst)[k] = round_to<T>(s);
 }
 
-// Threads per row and pieces per thread for `pieces` pieces of VEC columns; {0, 0}: too many for registers.
+// Elements of a piece: 16 bytes, or one element of rows that are shorter than that.
+template <typename T>
+constexpr int kNormVec = 16 / (int)sizeof(T);
+
+// Threads per row and pieces per thread for `pieces` pieces of VEC columns, up to 16 elements (VEC 8: 2, VEC 4: 4 pieces)
+// per thread; {0, 0}: too many for the registers of a workgroup.
 struct Shape {
   int lpr, nv;
 };
@@ -324,46 +428,47 @@ Shape shape_for(int64_t pieces, int vec) {
   for (int lpr : {8, 16, 32, 64})
     if (pieces <= lpr) return {lpr, 1};
   if (pieces <= 128) return {64, 2};
-  if (vec < 8) {
+  if (vec == 8) {
+    for (int lpr : {256, 512, 1024})
+      if (pieces <= 2 * lpr) return {lpr, pieces <= lpr ? 1 : 2};
+  } else {
     if (pieces <= 256) return {64, 4};
     for (int lpr : {256, 512, 1024})
       if (pieces <= 4 * lpr) return {lpr, pieces <= 2 * lpr ? 2 : 4};
-  } else {
-    for (int lpr : {256, 512, 1024})
-      if (pieces <= 2 * lpr) return {lpr, pieces <= lpr ? 1 : 2};
   }
   return {0, 0};
 }
 
-template <typename T, bool BACKWARD, int VEC, int LPR, int NV>
-hipError_t launch_shape(const NormArgs& p, hipStream_t s) {
-  constexpr int kThreads = LPR > 256 ? LPR : 256, kRows = kThreads / LPR;
+template <typename T, bool BACKWARD, int VEC, int LPR, int NV, bool TAIL>
+hipError_t launch_tail(NormArgs p, hipStream_t s) {
+  constexpr int kThreads = kNormThreads<LPR>, kRows = kThreads / LPR;
   const int64_t need = (p.rows + kRows - 1) / kRows;
-  if (BACKWARD) {
-    hipLaunchKernelGGL((norm_backward_kernel<T, VEC, LPR, NV>), dim3((unsigned)std::min<int64_t>(need, p.groups)),
-                       dim3(kThreads), 0, s, p);
-  } else {
-    hipLaunchKernelGGL((norm_forward_kernel<T, VEC, LPR, NV>),
-                       dim3((unsigned)std::min<int64_t>(need, 256 * 2048 / kThreads)), dim3(kThreads), 0, s, p);
-  }
+  const unsigned grid = (unsigned)std::min<int64_t>(need, BACKWARD ? p.groups : 256 * (2048 / kThreads));
+  if constexpr (BACKWARD)
+    hipLaunchKernelGGL((norm_backward_kernel<T, VEC, LPR, NV, TAIL>), dim3(grid), dim3(kThreads), 0, s, p);
+  else
+    hipLaunchKernelGGL((norm_forward_kernel<T, VEC, LPR, NV, TAIL>), dim3(grid), dim3(kThreads), 0, s, p);
   return hipGetLastError();
 }
 
 template <typename T, bool BACKWARD, int VEC>
 hipError_t launch_vec(const NormArgs& p, const Shape& sh, hipStream_t s) {
-#define PLH_NORM_SHAPE(L, N) \
-  if (sh.lpr == L && sh.nv == N) return launch_shape<T, BACKWARD, VEC, L, N>(p, s)
+#define PLH_NORM_SHAPE(L, N)                                                 \
+  if (sh.lpr == L && sh.nv == N)                                             \
+  return p.cols % VEC ? launch_tail<T, BACKWARD, VEC, L, N, true>(p, s) : launch_tail<T, BACKWARD, VEC, L, N, false>(p, s)
   PLH_NORM_SHAPE(8, 1);
-  PLH_NORM_SHAPE(16, 1);
-  PLH_NORM_SHAPE(32, 1);
-  PLH_NORM_SHAPE(64, 1);
-  PLH_NORM_SHAPE(64, 2);
-  PLH_NORM_SHAPE(256, 2);
-  PLH_NORM_SHAPE(512, 2);
-  PLH_NORM_SHAPE(1024, 2);
+  if constexpr (VEC > 1) {
+    PLH_NORM_SHAPE(16, 1);
+    PLH_NORM_SHAPE(32, 1);
+    PLH_NORM_SHAPE(64, 1);
+    PLH_NORM_SHAPE(64, 2);
+    PLH_NORM_SHAPE(256, 2);
+    PLH_NORM_SHAPE(512, 2);
+    PLH_NORM_SHAPE(1024, 2);
+  }
   if constexpr (VEC == 8) {
     PLH_NORM_SHAPE(256, 1);
-  } else {
+  } else if constexpr (VEC == 4) {
     PLH_NORM_SHAPE(64, 4);
     PLH_NORM_SHAPE(256, 4);
     PLH_NORM_SHAPE(512, 4);
@@ -373,57 +478,46 @@ hipError_t launch_vec(const NormArgs& p, const Shape& sh, hipStream_t s) {
   return hipErrorInvalidValue;
 }
 
-// The widest piece at which every access of a row is aligned.
-template <typename T>
-int norm_vec(const NormArgs& p) {
-  for (int v : {16 / (int)sizeof(T), 4})
-    if (p.cols % v == 0 && p.stride % v == 0 && aligned(p.x, v * (int)sizeof(T)) && aligned(p.y, v * (int)sizeof(T)) && aligned(p.d_y, v * (int)sizeof(T)) &&
-        aligned(p.d_x, v * (int)sizeof(T)))
-      return v;
-  return 1;
+// Workgroups of the backward pass, of `threads` threads with `side` rows side by side, each with a row of partial sums:
+// 1024 threads per CU with one piece per thread, 512 with more (longer rows, whose partial sums weigh more), one
+// workgroup at least.  With 512 and 1024 threads per CU: 512000 x 128 fp16 83 and 79 us, 300000 x 129 84 and 68,
+// 65536 x 1024 bf16 77 and 82, 7301 x 1001 fp16 16.9 and 18.3, 30000 x 2048 fp32 137 and 145.
+int64_t groups_for(int64_t rows, int threads, int side, int nv) {
+  const int64_t most = std::max(256, 256 * (nv == 1 ? 1024 : 512) / threads);
+  return std::max<int64_t>(1, std::min<int64_t>((rows + side - 1) / side, most));
 }
-
-// Workgroups of the backward pass, each with a row of partial sums.
-int64_t groups_for(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(rows, 1024)); }
+constexpr int kWideGroups = 64;  // runs of rows of norm_columns_kernel
 
 template <typename T, bool BACKWARD>
 hipError_t launch_norm(NormArgs p, hipStream_t s) {
-  const int vec = norm_vec<T>(p);
+  constexpr int V = kNormVec<T>;
+  const int vec = p.cols >= V ? V : 1;
   const Shape sh = shape_for((p.cols + vec - 1) / vec, vec);
+  if (BACKWARD && !p.d_weight && !p.d_bias) p.part = nullptr;
   hipError_t e = hipSuccess;
-  const unsigned wide = (unsigned)std::min<int64_t>(p.rows, 1024);
-  if (BACKWARD) {
-    const bool sums = p.d_weight || p.d_bias;
-    if (!sums) p.part = nullptr;
-    if (sh.lpr) {
-      const int threads = std::max(sh.lpr, 256);
-      p.groups = (int)std::min<int64_t>((p.rows + threads / sh.lpr - 1) / (threads / sh.lpr), 1024);
-    } else if (p.d_x) {
-      hipLaunchKernelGGL(norm_backward_wide_kernel<T>, dim3(wide), dim3(kWideThreads), 0, s, p);
-      e = hipGetLastError();
-    }
-    if (e != hipSuccess) return e;
-    if (!sh.lpr && sums) {
-      p.groups = (int)std::min<int64_t>(p.rows, 64);
-      hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((p.cols + 255) / 256, p.groups), dim3(256), 0, s, p);
-      e = hipGetLastError();
-    }
-    if (e != hipSuccess) return e;
-  } else if (!sh.lpr) {
-    hipLaunchKernelGGL(norm_forward_wide_kernel<T>, dim3(wide), dim3(kWideThreads), 0, s, p);
-    return hipGetLastError();
-  }
   if (sh.lpr) {
-    if (vec == 8) {
-      if constexpr (sizeof(T) == 2) e = launch_vec<T, BACKWARD, 8>(p, sh, s);
-    } else if (vec == 4) {
-      e = launch_vec<T, BACKWARD, 4>(p, sh, s);
+    const int threads = std::max(sh.lpr, 256);
+    p.groups = (int)groups_for(p.rows, threads, threads / sh.lpr, sh.nv);
+    e = vec == V ? launch_vec<T, BACKWARD, V>(p, sh, s) : launch_vec<T, BACKWARD, 1>(p, sh, s);
+  } else {
+    const unsigned grid = (unsigned)std::min<int64_t>(p.rows, 1024);
+    if constexpr (!BACKWARD) {
+      hipLaunchKernelGGL((norm_forward_wide_kernel<T, V>), dim3(grid), dim3(kWideThreads), 0, s, p);
+      e = hipGetLastError();
     } else {
-      e = launch_vec<T, BACKWARD, 1>(p, sh, s);
+      if (p.d_x) {
+        hipLaunchKernelGGL((norm_backward_wide_kernel<T, V>), dim3(grid), dim3(kWideThreads), 0, s, p);
+        e = hipGetLastError();
+      }
+      if (e == hipSuccess && p.part) {
+        p.groups = (int)std::min<int64_t>(p.rows, kWideGroups);
+        hipLaunchKernelGGL((norm_columns_kernel<T, V>), dim3((p.cols + 256 * V - 1) / (256 * V), p.groups), dim3(256), 0,
+                           s, p);
+        e = hipGetLastError();
+      }
     }
-    if (e != hipSuccess) return e;
   }
-  if (BACKWARD && p.part) {
+  if (e == hipSuccess && BACKWARD && p.part) {
     hipLaunchKernelGGL(norm_reduce_kernel<T>, dim3((unsigned)((2 * (int64_t)p.cols + 31) / 32)), dim3(1024), 0, s, p);
     e = hipGetLastError();
   }
@@ -448,7 +542,7 @@ extern "C" {
 
 int64_t plh_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 1 || cols > (1 << 24)) return -1;
-  return plh::groups_for(rows) * 2 * cols * (int64_t)sizeof(float);
+  return std::max<int64_t>(plh::groups_for(rows, 256, 1, 1), plh::kWideGroups) * 2 * cols * (int64_t)sizeof(float);
 }
 
 int plh_layer_norm_forward(int dtype, int wdtype, const void* x, int64_t stride, int64_t rows, int64_t cols,

@@ -37,6 +37,15 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
   __builtin_memcpy(p, &v, sizeof(v));
 }
 
+// A store of 16 bytes that is not to be kept in the caches.
+template <typename T, int N>
+__device__ __forceinline__ void store_vec_stream(T* p, const Vec<T, N>& v) {
+  static_assert(sizeof(v) == 16, "16 bytes");
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef u32x4 u32x4_at_any __attribute__((aligned(2)));
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4_at_any*>(p));
+}
+
 // Barrier that orders LDS traffic only: global loads and stores stay in flight across it (__syncthreads waits for them).
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
