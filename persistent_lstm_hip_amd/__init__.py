@@ -6,6 +6,7 @@ The LSTM's public surface mirrors mantuoluozk/persistent_lstm_hip's `persistent_
 """
 from .api import convert_lstm_module, convert_model_copy, convert_regressor_module, replace_lstm_inplace
 from .extension import load_extension
+from .gated import GatedScanBlock, GatedScanRegressor
 from .model import (
     NativeModuleFallback,
     PersistentLSTM,
@@ -26,6 +27,8 @@ __all__ = [
     "replace_lstm_inplace",
     "convert_model_copy",
     "load_extension",
+    "GatedScanBlock",
+    "GatedScanRegressor",
     "gated_scan",
     "gated_scan_step",
     "layer_norm",

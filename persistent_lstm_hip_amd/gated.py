@@ -1,0 +1,92 @@
+"""A recurrent forecaster that trains in parallel over time, on the block operators (ops.py):
+
+* GatedScanBlock      -- y = x + dropout(W_o scan(W_g layer_norm(x))), over a sequence or one step of it.
+* GatedScanRegressor  -- StandardLSTMRegressor's shape (x [B, T, I] -> [B, O] from a row's last step) with such blocks
+                         in the place of the stacked LSTM: trained over whole sequences, served token by token.
+
+The recurrence keeps an LSTM's forget and output gate and drops its recurrent weights, so that a sequence is one scan
+instead of a chain of matrix products.  The matrix products themselves are torch's.
+
+`python -m persistent_lstm_hip_amd.gated_demo` trains one on synthetic series, then serves it step by step.
+"""
+from __future__ import annotations
+
+from typing import List, Optional
+
+import torch
+import torch.nn as nn
+
+from .ops import dropout_add, gated_scan, gated_scan_step, layer_norm
+
+
+class GatedScanBlock(nn.Module):
+    """One residual block of width dim.  Its state is the scan's, [batch, dim] float32."""
+
+    def __init__(self, dim: int, dropout: float = 0.0):
+        super().__init__()
+        self.norm_weight = nn.Parameter(torch.ones(dim))
+        self.norm_bias = nn.Parameter(torch.zeros(dim))
+        self.gates = nn.Linear(dim, 3 * dim)
+        self.out = nn.Linear(dim, dim)
+        self.dropout = dropout
+        with torch.no_grad():  # memories from two steps to some hundred, channel by channel
+            self.gates.bias[:dim] = torch.linspace(0.5, 6.0, dim)
+
+    def forward(self, x: torch.Tensor, c0: Optional[torch.Tensor] = None, *, lengths=None, seed: int = 0,
+                offset: int = 0):
+        """x [batch, time, dim] -> (y, c_n).  (seed, offset) pick the dropout mask in training mode."""
+        gates = self.gates(layer_norm(x, self.norm_weight, self.norm_bias))
+        h, c_n = gated_scan(gates, c0, lengths=lengths)
+        p = self.dropout if self.training else 0.0
+        return dropout_add(self.out(h), x, p=p, seed=seed, offset=offset), c_n
+
+    def step(self, x: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
+        """One token x [batch, dim] -> y; c is updated in place.  For inference."""
+        gates = self.gates(layer_norm(x, self.norm_weight, self.norm_bias))
+        h, _ = gated_scan_step(gates, c, inplace=True)
+        return x + self.out(h)
+
+
+class GatedScanRegressor(nn.Module):
+    """x [batch, time, input_dim] -> [batch, output_dim], read off at every row's last step."""
+
+    def __init__(self, input_dim: int, hidden_dim: int, output_dim: int, n_layers: int, dropout: float = 0.2):
+        super().__init__()
+        self.stem = nn.Linear(input_dim, hidden_dim)
+        self.blocks = nn.ModuleList(GatedScanBlock(hidden_dim, dropout) for _ in range(n_layers))
+        self.norm_weight = nn.Parameter(torch.ones(hidden_dim))
+        self.norm_bias = nn.Parameter(torch.zeros(hidden_dim))
+        self.linear = nn.Linear(hidden_dim, output_dim)
+        self.seed = int(torch.initial_seed())
+        self._passes = 0  # training passes so far: every layer of every pass has a mask of its own
+
+    def _head(self, x: torch.Tensor) -> torch.Tensor:
+        return self.linear(layer_norm(x, self.norm_weight, self.norm_bias))
+
+    def forward(self, x: torch.Tensor, lengths=None) -> torch.Tensor:
+        if x.dim() != 3 or x.size(1) == 0:
+            raise ValueError("x must be a [batch, seq_len, input_size] tensor of at least one step")
+        if lengths is not None:
+            lengths = torch.as_tensor(lengths)
+        offset = self._passes * len(self.blocks)
+        if self.training:
+            self._passes += 1
+        y = self.stem(x)
+        for i, block in enumerate(self.blocks):
+            y, _ = block(y, lengths=lengths, seed=self.seed, offset=offset + i)
+        if lengths is None:
+            return self._head(y[:, -1])
+        last = (lengths.to(y.device, torch.int64) - 1).clamp(0, y.size(1) - 1)  # (an empty row: its first step)
+        return self._head(y[torch.arange(y.size(0), device=y.device), last])
+
+    def initial_state(self, batch: int) -> List[torch.Tensor]:
+        w = self.norm_weight
+        return [torch.zeros(batch, w.numel(), dtype=torch.float32, device=w.device) for _ in self.blocks]
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: List[torch.Tensor]) -> torch.Tensor:
+        """One token x [batch, input_dim] -> the forecast after it; state (initial_state) is updated in place."""
+        y = self.stem(x)
+        for block, c in zip(self.blocks, state):
+            y = block.step(y, c)
+        return self._head(y)
