@@ -226,8 +226,7 @@ int plh_probe_mfma_f16(double* tflops, double* clock_ghz);
  * for training and serving.  No counterpart in the reference, whose recurrence is the LSTM's alone.
  *   - dtype names the element type of the activations (PLH_F16, PLH_BF16, PLH_F32); sums, statistics and states are
  *     fp32, rounded once where an activation is written.
- *   - Pointers need the alignment of their elements only; strides are in elements.  Kernels move 16, 8, 4 or 2 bytes
- *     per lane, the widest that the pointers, the strides and the row length allow.
+ *   - Pointers need the alignment of their elements only (the workspaces: 16 bytes); strides are in elements.
  *   - Asynchronous on `stream`; no atomics, so that results are the same from call to call.  All can be captured in a
  *     HIP graph.
  */

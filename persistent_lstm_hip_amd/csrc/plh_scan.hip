@@ -34,11 +34,14 @@ constexpr int kSlabThreads = CT == 32 ? 512 : 256;
 // Channels per thread.
 inline int scan_vec(int64_t hidden) { return hidden >= 4 ? 4 : 1; }
 
-// Workgroups that a launch should have: two per CU.  With fewer slabs the time axis is split into segments, whose maps
-// a launch of its own computes first.  Forward / backward with about 512, 1024 and 2048 workgroups: 2 x 16384 x 640 bf16
-// (20 slabs) 60 / 94, 59 / 100, 56 / 95 us; 32 x 2048 x 512 (256 slabs) 83 / 125, 83 / 144, 85 / 147; 16 x 2048 x 2048
-// fp32 (512 slabs) 220 / 375 unsplit, 274 / 473 in two segments.
-constexpr int kScanGroups = 512;
+// With few slabs the time axis is split into segments, whose maps a launch of its own computes first: below so many slabs,
+// into so many workgroups in all.  Measured with 1, 2, 3 and 4 segments, us, bf16 or fp16, three gates:
+//   forward   300 slabs 111, 99, 90, 95;  384: 58, 58, 61, 64;  413: 163, 207, 203, 203;  20 slabs x 256 tiles with 256, 512
+//             and 768 workgroups 85, 57, 53;  61 x 201: 201, 151, 151
+//   backward  192 slabs 104, 110, 111, 115;  256: 109, 125, 143, 143;  20 x 256 with 256, 512 and 768: 117, 100, 95;
+//             64 x 64: 93, 76, 78
+constexpr int kSplitBelow[2] = {352, 160};  // forward, backward
+constexpr int kSplitGroups[2] = {768, 512};
 
 struct Split {
   int tiles;      // tiles of a row
@@ -53,11 +56,11 @@ int64_t slabs_of(int64_t batch, int64_t hidden) {
   return (pieces_of(batch, hidden) + ct - 1) / ct;
 }
 
-Split split_for(int64_t batch, int64_t seq_len, int64_t hidden) {
+Split split_for(int64_t batch, int64_t seq_len, int64_t hidden, bool backward) {
   Split s;
   s.tiles = (int)((seq_len + kTile - 1) / kTile);
   const int64_t slabs = std::max<int64_t>(slabs_of(batch, hidden), 1);
-  const int want = (int)std::max<int64_t>(1, (kScanGroups + slabs / 2) / slabs);
+  const int want = slabs < kSplitBelow[backward] ? (int)((kSplitGroups[backward] + slabs / 2) / slabs) : 1;
   s.seg_tiles = std::max(1, (s.tiles + want - 1) / want);
   s.segs = std::max(1, (s.tiles + s.seg_tiles - 1) / s.seg_tiles);
   return s;
@@ -729,8 +732,8 @@ int check_scan(const char* what, int dtype, const void* gates, int64_t stride_b,
 
 template <typename T>
 ScanArgs<T> scan_args(const void* gates, int64_t stride_b, int64_t stride_t, int64_t batch, int64_t seq_len, int hidden,
-                      const int32_t* lengths, void* workspace) {
-  const Split sp = split_for(batch, seq_len, hidden);
+                      const int32_t* lengths, void* workspace, bool backward) {
+  const Split sp = split_for(batch, seq_len, hidden, backward);
   ScanArgs<T> p = {};
   p.gates = (const T*)gates;
   p.stride_b = stride_b, p.stride_t = stride_t;
@@ -754,9 +757,10 @@ int64_t plh_gated_scan_states(int64_t seq_len) { return seq_len < 0 ? -1 : (seq_
 
 int64_t plh_gated_scan_workspace_bytes(int64_t batch, int64_t seq_len, int hidden) {
   if (batch < 0 || seq_len < 0 || hidden < 1 || seq_len > (1 << 30) || batch > (1 << 29)) return -1;
-  const plh::Split s = plh::split_for(batch, seq_len, hidden);
-  if (s.segs <= 1) return 0;
-  return 2 * ((batch * hidden * s.segs + 3) / 4 * 4) * (int64_t)sizeof(float);
+  const int64_t segs = std::max(plh::split_for(batch, seq_len, hidden, false).segs,
+                                plh::split_for(batch, seq_len, hidden, true).segs);
+  if (segs <= 1) return 0;
+  return 2 * ((batch * hidden * segs + 3) / 4 * 4) * (int64_t)sizeof(float);
 }
 
 int plh_gated_scan_forward(int dtype, int output_gate, const void* gates, int64_t stride_b, int64_t stride_t,
@@ -772,7 +776,7 @@ int plh_gated_scan_forward(int dtype, int output_gate, const void* gates, int64_
   hipError_t e = hipSuccess;
   plh::with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
-    auto p = plh::scan_args<T>(gates, stride_b, stride_t, batch, seq_len, hidden, lengths, workspace);
+    auto p = plh::scan_args<T>(gates, stride_b, stride_t, batch, seq_len, hidden, lengths, workspace, false);
     p.c0 = c0, p.out = (T*)out, p.c_n = c_n, p.states = states;
     e = plh::launch_scan<T, false>(p, output_gate != 0, (hipStream_t)stream);
   });
@@ -793,7 +797,7 @@ int plh_gated_scan_backward(int dtype, int output_gate, const void* gates, int64
   hipError_t e = hipSuccess;
   plh::with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
-    auto p = plh::scan_args<T>(gates, stride_b, stride_t, batch, seq_len, hidden, lengths, workspace);
+    auto p = plh::scan_args<T>(gates, stride_b, stride_t, batch, seq_len, hidden, lengths, workspace, true);
     p.states = const_cast<float*>(states), p.d_out = (const T*)d_out, p.d_cn = d_cn;
     p.d_gates = (T*)d_gates, p.d_c0 = d_c0;
     e = plh::launch_scan<T, true>(p, output_gate != 0, (hipStream_t)stream);

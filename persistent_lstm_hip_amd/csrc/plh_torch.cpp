@@ -71,6 +71,9 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
 
+// A gradient as the kernels read it: of the output's type, contiguous.
+Tensor incoming(const Tensor& grad, at::ScalarType type) { return grad.to(type).contiguous(); }
+
 // In a node below, needs_input_grad counts the tensors that it was given (an optional that holds none is not counted).
 
 // What a node's backward pass returns can be differentiated no further: asked for a second derivative it raises.
@@ -161,9 +164,9 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     const int64_t B = gates.size(0), T = gates.size(1), H = states.size(2);
     const at::Device device = gates.device();
     const c10::DeviceGuard guard(device);
-    const Tensor d_out =
-        grads[0].defined() ? grads[0].contiguous() : at::zeros({B, T, H}, at::TensorOptions().dtype(gates.scalar_type()).device(device));
-    const Tensor d_cn = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor d_out = grads[0].defined() ? incoming(grads[0], gates.scalar_type())
+                                            : at::zeros({B, T, H}, at::TensorOptions().dtype(gates.scalar_type()).device(device));
+    const Tensor d_cn = grads[1].defined() ? incoming(grads[1], at::kFloat) : Tensor();
     Tensor d_gates = empty(gates.sizes(), gates.scalar_type(), device), d_c0;
     if (ctx->saved_data["has_c0"].toBool() && ctx->needs_input_grad(1)) d_c0 = empty({B, H}, at::kFloat, device);
     const Tensor ws = scan_workspace(B, T, H, device);
@@ -264,7 +267,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto wtype = (at::ScalarType)ctx->saved_data["wdtype"].toInt();
     const at::Device device = m.device();
     const c10::DeviceGuard guard(device);
-    const Tensor d_y = grads[0].contiguous();
+    const Tensor d_y = incoming(grads[0], m.scalar_type());
     Tensor d_x, d_w, d_b, ws;
     if (ctx->needs_input_grad(0)) d_x = empty(ctx->saved_data["shape"].toIntVector(), m.scalar_type(), device);
     if ((has & 1) && ctx->needs_input_grad(1)) d_w = empty({cols}, wtype, device);
@@ -321,6 +324,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     ctx->save_for_backward({off});
     ctx->saved_data["mask"] = std::vector<int64_t>{threshold, seed, offset};
     ctx->saved_data["has_residual"] = residual.has_value();
+    ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
     return dropout(x, given(residual), Mask{(int)threshold, (uint64_t)seed, (uint64_t)offset}, off);
   }
 
@@ -328,10 +332,11 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     const std::vector<int64_t> m = ctx->saved_data["mask"].toIntVector();
     const variable_list saved = ctx->get_saved_variables();
     const c10::DeviceGuard guard(grads[0].device());
+    const Tensor d_out = incoming(grads[0], (at::ScalarType)ctx->saved_data["dtype"].toInt());
     Tensor d_x, d_r;
     if (ctx->needs_input_grad(0))
-      d_x = dropout(grads[0].contiguous(), Tensor(), Mask{(int)m[0], (uint64_t)m[1], (uint64_t)m[2]}, saved[0]);
-    if (ctx->saved_data["has_residual"].toBool() && ctx->needs_input_grad(1)) d_r = grads[0];
+      d_x = dropout(d_out, Tensor(), Mask{(int)m[0], (uint64_t)m[1], (uint64_t)m[2]}, saved[0]);
+    if (ctx->saved_data["has_residual"].toBool() && ctx->needs_input_grad(1)) d_r = d_out;
     return once({d_x, d_r, Tensor(), Tensor(), Tensor(), Tensor()}, grads, "dropout_add");
   }
 };

@@ -600,6 +600,20 @@ def test_operators_refuse_on_the_device(gpu):
             bad()
 
 
+def test_gradients_of_another_type_are_converted(gpu):
+    _say("gradient types")
+    x = torch.randn(4, 24, device="cuda").half().requires_grad_(True)
+    d = torch.randn(4, 24, device="cuda")
+    for f in (lambda: P.layer_norm(x), lambda: P.dropout_add(x, p=0.1, seed=1),
+              lambda: P.gated_scan(x.view(2, 2, 24), output_gate=False)[0]):
+        y = f()
+        dy = d.view(-1)[:y.numel()].view(y.shape)
+        assert torch.equal(torch.autograd.grad(f(), x, dy)[0], torch.autograd.grad(f(), x, dy.half())[0])
+    z = x.detach().float().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(P.layer_norm(z), z, d.half())[0],
+                       torch.autograd.grad(P.layer_norm(z), z, d.half().float())[0])
+
+
 def test_gradients_are_once_differentiable(gpu):
     _say("double backward")
     x = torch.randn(3, 8, device="cuda", requires_grad=True)

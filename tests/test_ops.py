@@ -81,6 +81,17 @@ def test_host_tensors_are_refused(call):
         call(lambda *shape: [0.0])
 
 
+def test_a_missing_front_end_is_an_error_that_names_it(tmp_path, monkeypatch):
+    from persistent_lstm_hip_amd import extension
+
+    monkeypatch.setattr(extension, "TORCH_PATH", str(tmp_path / "plh_torch.so"))
+    with pytest.raises(RuntimeError, match="plh_torch.so.*persistent_lstm_hip_amd.build"):
+        extension.require_torch_ops.__wrapped__()
+    (tmp_path / "plh_torch.so").write_bytes(b"not a library")
+    with pytest.raises(RuntimeError, match="plh_torch.so"):
+        extension.require_torch_ops.__wrapped__()
+
+
 # ---- the C ABI refuses before it touches a device ------------------------------------------------
 
 ANY = ctypes.c_void_p(256)  # never dereferenced
