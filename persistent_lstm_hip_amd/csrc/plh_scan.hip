@@ -608,55 +608,139 @@ __global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArg
   if (at.on && at.tg == 0 && seg == 0 && p.d_c0) store_carry(p.d_c0, at, carry);
 }
 
-constexpr int kStepThreads = 256;
+// ---- a few steps ----
+// One step (serving) or up to eight: a thread carries VEC channels through them one after the other, nothing to scan.
+// The tiled kernels leave most of a tile idle there: 1000 rows of 2 x 512 fp16 forward / backward 41 / 69 us, here
+// 5.1 / 6.1; 400 x 8 x 400 fp32 15 / 37 and 7.3 / 9.2.  With more steps the chain of loads takes over: 300 x 16 x 512
+// bf16 forward 14.7 and 13.9 us, 8 x 16 x 512 4.2 and 8.3.
+constexpr int kShort = 8;
+constexpr int kShortThreads = 256;
 
-// One step of every row, for serving: a thread per VEC channels, nothing to scan.  (The tiled kernel would leave 63 of
-// 64 steps idle: 20.4 us for 512 rows of 512 channels in bfloat16.)
-template <typename T, int VEC, bool GATED>
-__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanArgs<T> p) {
-  const uint32_t piece = blockIdx.x * kStepThreads + threadIdx.x, per = (p.H + VEC - 1) / VEC;
+// A thread's channels: f(integral constant N, b, h) for N of them from h on.  A row's last piece goes one channel at a
+// time where it is not full: c_n may be c0, so that no channel may be another thread's too.
+template <int VEC, typename T, typename F>
+__device__ __forceinline__ void short_pieces(const ScanArgs<T>& p, F&& f) {
+  const uint32_t piece = blockIdx.x * kShortThreads + threadIdx.x, per = (p.H + VEC - 1) / VEC;
   if (piece >= p.pieces) return;
   const int64_t b = piece / per;
   const int h = (int)(piece % per) * VEC;
-  const bool on = !p.lengths || p.lengths[b] > 0;
-  const auto step = [&](auto width, int h) __attribute__((always_inline)) {
-    constexpr int N = decltype(width)::value;
+  if (h + VEC <= p.H) {
+    f(std::integral_constant<int, VEC>(), b, h);
+  } else {
+    for (int k = h; k < p.H; ++k) f(std::integral_constant<int, 1>(), b, k);
+  }
+}
+
+template <typename T, int VEC, bool GATED>
+__global__ void __launch_bounds__(kShortThreads) scan_forward_short_kernel(ScanArgs<T> p) {
+  short_pieces<VEC>(p, [&](auto width, int64_t b, int h) __attribute__((always_inline)) {
+    constexpr int N = decltype(width)::value, U = 4;  // U steps are loaded at a time
+    const int len = p.lengths ? min(max(p.lengths[b], 0), p.T_) : p.T_;
     const int64_t n = b * p.H + h;
     Vec<float, N> c = {};
     if (p.c0) c = load_vec<float, N>(p.c0 + n);
     if (p.states) store_vec(p.states + n, c);
-    Vec<T, N> y = {};
-    if (on) {
-      const T* const src = p.gates + b * p.stride_b + h;
-      const Vec<T, N> f = load_vec<T, N>(src), g = load_vec<T, N>(src + p.H);
-      Vec<T, N> o = {};
-      if (GATED) o = load_vec<T, N>(src + 2 * p.H);
-      float out[N];
+    const T* src = p.gates + b * p.stride_b + h;
+    T* dst = p.out + b * p.T_ * p.H + h;
+    for (int t = 0; t < p.T_; t += U) {
+      Vec<T, N> f[U] = {}, g[U] = {}, o[U] = {};
+#pragma unroll
+      for (int r = 0; r < U; ++r) {
+        if (t + r < len) {
+          f[r] = load_vec<T, N>(src), g[r] = load_vec<T, N>(src + p.H);
+          if (GATED) o[r] = load_vec<T, N>(src + 2 * p.H);
+        }
+        src += p.stride_t;
+      }
+#pragma unroll
+      for (int r = 0; r < U; ++r) {
+        if (t + r < p.T_) {
+          float y[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            float a, na;
+            logistic((float)f[r].v[j], a, na);
+            const float next = fmaf(a, c.v[j], na * (float)g[r].v[j]);
+            c.v[j] = t + r < len ? next : c.v[j];
+            y[j] = GATED ? next * sigmoid((float)o[r].v[j]) : next;
+          }
+          store_vec(dst, zero_unless(t + r < len, round_to<T, N>(y)));
+        }
+        dst += p.H;
+      }
+    }
+    if (p.c_n) store_vec(p.c_n + n, c);
+  });
+}
+
+template <typename T, int VEC, bool GATED>
+__global__ void __launch_bounds__(kShortThreads) scan_backward_short_kernel(ScanArgs<T> p) {
+  short_pieces<VEC>(p, [&](auto width, int64_t b, int h) __attribute__((always_inline)) {
+    constexpr int N = decltype(width)::value, R = kShort, kParts = GATED ? 3 : 2;
+    const int len = p.lengths ? min(max(p.lengths[b], 0), p.T_) : p.T_;
+    const int64_t n = b * p.H + h;
+    Vec<T, N> f[R] = {}, g[R] = {}, o[R] = {}, d[R] = {};
+    const T* src = p.gates + b * p.stride_b + h;
+    const T* grad = p.d_out + b * p.T_ * p.H + h;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r < len) {
+        f[r] = load_vec<T, N>(src), g[r] = load_vec<T, N>(src + p.H);
+        if (GATED) o[r] = load_vec<T, N>(src + 2 * p.H);
+        d[r] = load_vec<T, N>(grad);
+      }
+      src += p.stride_t, grad += p.H;
+    }
+    Vec<float, N> c = load_vec<float, N>(p.states + n), e = {};
+    if (p.d_cn) e = load_vec<float, N>(p.d_cn + n);
+    float before[R][N];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         float a, na;
-        logistic((float)f.v[j], a, na);
-        c.v[j] = fmaf(a, c.v[j], na * (float)g.v[j]);
-        out[j] = GATED ? c.v[j] * sigmoid((float)o.v[j]) : c.v[j];
+        logistic((float)f[r].v[j], a, na);
+        before[r][j] = c.v[j];
+        c.v[j] = fmaf(a, c.v[j], na * (float)g[r].v[j]);  // (past the row's end it is not used)
       }
-      y = round_to<T, N>(out);
     }
-    if (p.c_n) store_vec(p.c_n + n, c);
-    store_vec(p.out + n, y);
-  };
-  if (h + VEC <= p.H) {
-    step(std::integral_constant<int, VEC>(), h);
-  } else {  // (c_n may be c0, so no channel may be another thread's too)
-    for (int k = h; k < p.H; ++k) step(std::integral_constant<int, 1>(), k);
-  }
+    T* const dst = p.d_gates + b * p.T_ * (kParts * p.H) + h;
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r) {
+      if (r >= p.T_) continue;
+      const bool live = r < len;
+      float df[N], dg[N], d_o[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float a, na, u = (float)d[r].v[j];
+        const float gv = (float)g[r].v[j];
+        logistic((float)f[r].v[j], a, na);
+        if (GATED) {
+          float s, ns;
+          logistic_fast((float)o[r].v[j], s, ns);
+          u *= s;
+          d_o[j] = ns * u * fmaf(a, before[r][j], na * gv);
+        }
+        const float D = u + e.v[j], k = na * D;
+        if (live) e.v[j] = a * D;
+        dg[j] = k;
+        df[j] = a * k * (before[r][j] - gv);
+      }
+      T* const q = dst + (int64_t)r * (kParts * p.H);
+      store_vec(q, zero_unless(live, round_to<T, N>(df)));
+      store_vec(q + p.H, zero_unless(live, round_to<T, N>(dg)));
+      if (GATED) store_vec(q + 2 * p.H, zero_unless(live, round_to<T, N>(d_o)));
+    }
+    if (p.d_c0) store_vec(p.d_c0 + n, e);
+  });
 }
 
 template <typename T, int VEC, bool GATED>
 hipError_t launch_forward(const ScanArgs<T>& p, hipStream_t s) {
   constexpr int CT = VEC == 4 ? 16 : 64, kThreads = Place<VEC, CT>::THREADS;
-  if (p.T_ == 1) {
-    hipLaunchKernelGGL((scan_step_kernel<T, VEC, GATED>), dim3((p.pieces + kStepThreads - 1) / kStepThreads),
-                       dim3(kStepThreads), 0, s, p);
+  if (p.T_ >= 1 && p.T_ <= kShort) {
+    hipLaunchKernelGGL((scan_forward_short_kernel<T, VEC, GATED>), dim3((p.pieces + kShortThreads - 1) / kShortThreads),
+                       dim3(kShortThreads), 0, s, p);
     return hipGetLastError();
   }
   if (p.segs > 1) {
@@ -682,6 +766,11 @@ bool wide_slabs(const ScanArgs<T>& p) {
 template <typename T, int VEC, bool GATED>
 hipError_t launch_backward(ScanArgs<T> p, hipStream_t s) {
   constexpr int CT = VEC == 4 ? 16 : 64, kThreads = Place<VEC, CT>::THREADS;
+  if (p.T_ >= 1 && p.T_ <= kShort) {
+    hipLaunchKernelGGL((scan_backward_short_kernel<T, VEC, GATED>), dim3((p.pieces + kShortThreads - 1) / kShortThreads),
+                       dim3(kShortThreads), 0, s, p);
+    return hipGetLastError();
+  }
   if constexpr (sizeof(T) == 2 && VEC == 4) {
     if (wide_slabs(p)) {
       p.slabs = (p.pieces + 31) / 32;
