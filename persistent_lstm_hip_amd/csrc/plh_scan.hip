@@ -25,7 +25,7 @@ namespace {
 // the row: its channels are then carried by two threads, which compute and store the same.  Pieces are numbered row
 // after row, so that slabs are full whatever H is.
 //   VEC 4, CT 16: 256 threads, 64 channels, 4 steps each (the usual slab)
-//   VEC 4, CT 32: 512 threads, 128 channels, 4 steps each (backward, see wide_slabs)
+//   VEC 4, CT 32: 512 threads, 128 channels, 4 steps each (see wide_slabs)
 //   VEC 1, CT 64: 256 threads, 64 channels, 16 steps each (H < 4)
 constexpr int kTile = 64;  // steps
 template <int CT>
@@ -40,7 +40,7 @@ inline int scan_vec(int64_t hidden) { return hidden >= 4 ? 4 : 1; }
 //             and 768 workgroups 85, 57, 53;  61 x 201: 201, 151, 151
 //   backward  192 slabs 104, 110, 111, 115;  256: 109, 125, 143, 143;  20 x 256 with 256, 512 and 768: 117, 100, 95;
 //             64 x 64: 93, 76, 78
-constexpr int kSplitBelow[2] = {352, 160};  // forward, backward
+constexpr unsigned kSplitBelow[2] = {352, 160};  // forward, backward
 constexpr int kSplitGroups[2] = {768, 512};
 
 struct Split {
@@ -243,6 +243,57 @@ __device__ __forceinline__ void fold_waves(const P& at, const TileMaps<P, SUMS>&
   for (int j = 0; j < VEC; ++j) mine[j] = fmaf(pa[j], before[j], pb[j]);
 }
 
+// Forward, the carry goes from wave to wave, and from the last one to the first one's next tile: slot[w] holds what wave w starts
+// its part of a tile from, tag[w] the number of the tile (from 1 on, in the order of the scan) that it is for.  A wave waits for
+// the one before it alone, so that the waves of a workgroup do not run in step as they would around a barrier: half of
+// them load and store while the others compute (16 x 4096 x 2048 bf16 forward 243 -> 235 us, and with 128-channel
+// slabs, which lose without it, 215).  (The backward pass, where c and E go through a tile in opposite directions, would
+// wait for both in turn: 32 x 2048 x 512 109 -> 127 us.  It composes a tile's maps around one barrier.)  A slot is written for the next tile only after the wave that reads it has sent on what
+// it read.  All waves of a workgroup are resident, so every wait ends.
+template <typename P>
+struct Relay {
+  float slot[P::WAVES][P::SLAB];
+  uint32_t tag[P::WAVES];
+};
+template <typename P, int VEC = P::VEC>
+__device__ __forceinline__ void relay_put(const P& at, Relay<P>& relay, int wave, uint32_t tag, const float (&c)[VEC]) {
+  if (at.lane < P::CT) put_lds<VEC>(&relay.slot[wave][at.ct * VEC], c);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  if (at.lane == 0) __hip_atomic_store(&relay.tag[wave], tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+template <typename P, int VEC = P::VEC>
+__device__ __forceinline__ void relay_get(const P& at, Relay<P>& relay, uint32_t tag, float (&c)[VEC]) {
+  while (__hip_atomic_load(&relay.tag[at.wave], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) != tag) {
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  const Vec<float, VEC> v = get_lds<VEC>(&relay.slot[at.wave][at.ct * VEC]);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) c[j] = v.v[j];
+}
+// One wave's part of a tile: takes the carry, gives the next wave what the map (A, B) of its own steps makes of it (the
+// last wave gives it to the next tile's first), and returns what a thread starts from, by its map (pa, pb).
+template <typename P, int VEC = P::VEC>
+__device__ __forceinline__ void relay_pass(const P& at, Relay<P>& relay, uint32_t round, const float (&A)[VEC],
+                                           const float (&B)[VEC], const float (&pa)[VEC], const float (&pb)[VEC],
+                                           float (&carry)[VEC], float (&mine)[VEC]) {
+  relay_get(at, relay, round, carry);
+  float after[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    after[j] = fmaf(A[j], carry[j], B[j]);
+    mine[j] = fmaf(pa[j], carry[j], pb[j]);
+  }
+  if (at.wave + 1 < P::WAVES)
+    relay_put(at, relay, at.wave + 1, round, after);
+  else
+    relay_put(at, relay, 0, round + 1, after);
+}
+// Empties the relay (all threads; a barrier follows).
+template <typename P>
+__device__ __forceinline__ void relay_clear(Relay<P>& relay) {
+  if (threadIdx.x < P::WAVES) relay.tag[threadIdx.x] = 0;
+}
+
 // The carry at a segment's start: the maps of the n segments before it, segment `first` + i `step` for i = 0 .. n - 1 in
 // this order, applied to `carry`.  Each time group composes a run of them, and the runs are composed as a tile's are.
 // (One thread after the other through the same maps, an L2 latency each, took 60 us for 255 segments.)
@@ -433,13 +484,18 @@ template <typename T, int VEC, int CT, bool GATED>
 __global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan_forward_kernel(ScanArgs<T> p) {
   using P = Place<VEC, CT>;
   constexpr int R = P::R;
-  __shared__ alignas(16) WaveMaps<P, 1> lds;
+  __shared__ alignas(16) TileMaps<P, 1> lds;
+  __shared__ alignas(16) Relay<P> relay;
   const int seg = blockIdx.x / p.slabs;
   const P at(p, slab_of(blockIdx.x % p.slabs, p.slabs));
   float carry[VEC];
   load_carry(p.c0, at, carry);
   const int tile_first = seg * p.seg_tiles, tile_end = min(p.tiles, (seg + 1) * p.seg_tiles);
-  fold_segments<T, P, 1>(p, at, 0, 1, seg, lds[(tile_first + 1) & 1], carry);
+  fold_segments<T, P, 1>(p, at, 0, 1, seg, lds, carry);
+  relay_clear(relay);
+  lds_barrier();
+  if (at.wave == 0) relay_put(at, relay, 0, 1, carry);
+  uint32_t round = 0;
   using Tile = Rows<T, P, true, GATED, false>;
   const auto process = [&](const Tile& x, int tile) __attribute__((always_inline)) {
     const int t0 = tile * kTile + at.tg * R;
@@ -458,12 +514,9 @@ __global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan
       }
     }
     wave_maps<P, 1, false>(at.lane, A, B, pa, pb);
-    auto& maps = lds[tile & 1];
-    put_maps<P, 1>(at, maps, A, B);
-    lds_barrier();
-    if (p.states && at.on && at.tg == 0) store_carry(p.states + (int64_t)tile * p.channels, at, carry);
     float c[VEC];
-    fold_waves<P, 1, 0, false>(at, maps, pa[0], pb[0], carry, c);
+    relay_pass(at, relay, ++round, A, B[0], pa[0], pb[0], carry, c);
+    if (p.states && at.on && at.tg == 0) store_carry(p.states + (int64_t)tile * p.channels, at, carry);
     if (!at.on) return;
     T* dst = p.out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h;
     Vec<T, VEC> y[R];
@@ -495,7 +548,10 @@ __global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan
     process(x, tile);
   }
   zero_tiles<1>(p.out, p, at, max(tile_first, live_end), tile_end);
-  if (at.on && at.tg == 0 && seg == p.segs - 1 && p.c_n) store_carry(p.c_n, at, carry);
+  if (at.wave == 0) {
+    relay_get(at, relay, round + 1, carry);
+    if (at.on && at.tg == 0 && seg == p.segs - 1 && p.c_n) store_carry(p.c_n, at, carry);
+  }
 }
 
 // Backward: tiles from the last to the first.
@@ -735,8 +791,20 @@ __global__ void __launch_bounds__(kShortThreads) scan_backward_short_kernel(Scan
   });
 }
 
+// Whether to take slabs of 128 channels in 512 threads: rows of 16-bit elements are then read 256 bytes at a time instead
+// of 128 (as 32-bit ones are in the usual slabs).  Not where the time axis has to be split (33 x 1001 x 333, 174
+// slabs: backward 60 -> 77 us), nor where the last round of workgroups, one per CU of 256, would be far from full.
+// Forward / backward, usual -> wide, us: 16 x 4096 x 2048 bf16 (256 wide slabs) 235 / 411 -> 216 / 353; B x 1000 x 256 bf16
+// with 180 wide slabs 58 / 84 -> 53 / 76, with 256 61 / 101 -> 59 / 99, 300 76 / 138 -> 85 / 153, 400 107 / 172 -> 97 / 158, 600
+// 151 / 230 -> 152 / 244, 1000 233 / 371 -> 228 / 363; rows that no line divides, 300 x 2493 x 88 fp16: 158 / 348 -> 145 / 277.
+template <typename T>
+bool wide_slabs(const ScanArgs<T>& p) {
+  const unsigned wide = (p.pieces + 31) / 32, rounds = (wide + 255) / 256;
+  return sizeof(T) == 2 && p.slabs >= kSplitBelow[0] && (rounds == 1 || 4 * wide >= 3 * 256 * rounds);
+}
+
 template <typename T, int VEC, bool GATED>
-hipError_t launch_forward(const ScanArgs<T>& p, hipStream_t s) {
+hipError_t launch_forward(ScanArgs<T> p, hipStream_t s) {
   constexpr int CT = VEC == 4 ? 16 : 64, kThreads = Place<VEC, CT>::THREADS;
   if (p.T_ >= 1 && p.T_ <= kShort) {
     hipLaunchKernelGGL((scan_forward_short_kernel<T, VEC, GATED>), dim3((p.pieces + kShortThreads - 1) / kShortThreads),
@@ -749,18 +817,16 @@ hipError_t launch_forward(const ScanArgs<T>& p, hipStream_t s) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
+  if constexpr (sizeof(T) == 2 && VEC == 4) {
+    if (wide_slabs(p)) {
+      p.slabs = (p.pieces + 31) / 32;
+      hipLaunchKernelGGL((scan_forward_kernel<T, 4, 32, GATED>), dim3(p.slabs), dim3(Place<4, 32>::THREADS), 0, s, p);
+      return hipGetLastError();
+    }
+  }
   hipLaunchKernelGGL((scan_forward_kernel<T, VEC, CT, GATED>), dim3(p.slabs * (unsigned)p.segs), dim3(kThreads), 0, s,
                      p);
   return hipGetLastError();
-}
-
-// Whether the backward pass takes slabs of 128 channels in 512 threads: rows of 16-bit elements are then read 256 bytes
-// at a time instead of 128, with one workgroup per CU and no split.  16 x 4096 x 2048 bf16: 411 -> 353 us.  Rows that
-// are hardly longer gain nothing (512 x 1000 x 128: 189 and 190 us), a time axis that has to be split loses (33 x
-// 1001 x 333: 70 and 77 us), and the forward pass loses too (243 and 269 us).
-template <typename T>
-bool wide_slabs(const ScanArgs<T>& p) {
-  return sizeof(T) == 2 && p.H >= 256 && p.slabs >= 512 && p.segs == 1;
 }
 
 template <typename T, int VEC, bool GATED>
