@@ -1,5 +1,6 @@
 /*
- * persistent_lstm_hip.h -- C ABI of the MI355X (gfx950) stacked LSTM + Linear inference forward.
+ * persistent_lstm_hip.h -- C ABI of the MI355X (gfx950) stacked LSTM + Linear inference forward and of the operators of
+ * a residual block around a recurrence that is parallel over time (at the end).
  *
  * Library: persistent_lstm_hip_amd/lib/libpersistent_lstm_hip.so
  *

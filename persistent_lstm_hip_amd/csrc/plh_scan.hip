@@ -25,7 +25,7 @@ namespace {
 // the row: its channels are then carried by two threads, which compute and store the same.  Pieces are numbered row
 // after row, so that slabs are full whatever H is.
 //   VEC 4, CT 16: 256 threads, 64 channels, 4 steps each (the usual slab)
-//   VEC 4, CT 32: 512 threads, 128 channels, 4 steps each (see wide_slabs)
+//   VEC 4, CT 32: 512 threads, 128 channels, 4 steps each (see layout_for)
 //   VEC 1, CT 64: 256 threads, 64 channels, 16 steps each (H < 4)
 constexpr int kTile = 64;  // steps
 template <int CT>
@@ -34,36 +34,55 @@ constexpr int kSlabThreads = CT == 32 ? 512 : 256;
 // Channels per thread.
 inline int scan_vec(int64_t hidden) { return hidden >= 4 ? 4 : 1; }
 
-// With few slabs the time axis is split into segments, whose maps a launch of its own computes first: below so many slabs,
-// into so many workgroups in all.  Measured with 1, 2, 3 and 4 segments, us, bf16 or fp16, three gates:
-//   forward   300 slabs 111, 99, 90, 95;  384: 58, 58, 61, 64;  413: 163, 207, 203, 203;  20 slabs x 256 tiles with 256, 512
-//             and 768 workgroups 85, 57, 53;  61 x 201: 201, 151, 151
-//   backward  192 slabs 104, 110, 111, 115;  256: 109, 125, 143, 143;  20 x 256 with 256, 512 and 768: 117, 100, 95;
-//             64 x 64: 93, 76, 78
-constexpr unsigned kSplitBelow[2] = {352, 160};  // forward, backward
-constexpr int kSplitGroups[2] = {768, 512};
+int64_t pieces_of(int64_t batch, int64_t hidden) { return batch * ((hidden + scan_vec(hidden) - 1) / scan_vec(hidden)); }
 
-struct Split {
+// How a call is laid out on the device.
+struct Layout {
+  bool wide;      // slabs of 128 channels
+  int64_t slabs;
   int tiles;      // tiles of a row
   int seg_tiles;  // ... of a segment
-  int segs;
+  int segs;       // segments of the time axis
 };
 
-int64_t pieces_of(int64_t batch, int64_t hidden) { return batch * ((hidden + scan_vec(hidden) - 1) / scan_vec(hidden)); }
-// Slabs of the usual kind.
-int64_t slabs_of(int64_t batch, int64_t hidden) {
+// With few slabs the time axis is split into segments, whose maps a launch of its own computes first.  Rows of 16-bit
+// elements may be read 256 bytes at a time, in wide slabs, instead of 128 (as 32-bit ones are in the usual slabs).
+// Measured, us, on 256 CUs, by the number of usual slabs (forward / backward; bf16 or fp16 with output gate):
+//   352 and more: no split; wide slabs, but not where the last round of their workgroups, one per CU, would be far from
+//     full.  usual -> wide: 512 slabs 235 / 411 -> 216 / 353 (16 x 4096 x 2048), B x 1000 x 256 with 360 slabs 58 / 84 -> 53 / 76,
+//     512 61 / 101 -> 59 / 99, 600 76 / 138 -> 85 / 153, 800 107 / 172 -> 97 / 158, 1200 151 / 230 -> 152 / 244, 2000
+//     233 / 371 -> 219 / 359;  rows that no line divides, 300 x 2493 x 88 (413): 158 / 348 -> 145 / 277, in two segments
+//     207 / 401
+//   160 to 351: usual slabs; forward about 768 workgroups (300 slabs with 1, 2, 3, 4 segments: 111, 99, 90, 95), backward
+//     no split (256: 109, 125, 143, 143; 192: 104, 110, 111, 115)
+//   32 to 159: wide slabs for 16 bits; forward 512 workgroups, backward 256.  usual -> wide: 64 slabs 46 / 76 -> 40 / 72, 128
+//     62 / 108 -> 57 / 93, 61 (4 x 12837 x 968) 152 / 289 -> 150 / 254
+//   fewer: usual slabs, 768 and 512 workgroups.  20 slabs (2 x 16384 x 640) with 256, 512, 768 workgroups: 85 / 117,
+//     57 / 100, 53 / 95; in wide slabs 54 / 109
+Layout layout_for(int elem_bytes, int64_t batch, int64_t seq_len, int64_t hidden, bool backward) {
+  Layout l;
+  const int64_t pieces = std::max<int64_t>(pieces_of(batch, hidden), 1);
   const int ct = hidden >= 4 ? 16 : 64;
-  return (pieces_of(batch, hidden) + ct - 1) / ct;
-}
-
-Split split_for(int64_t batch, int64_t seq_len, int64_t hidden, bool backward) {
-  Split s;
-  s.tiles = (int)((seq_len + kTile - 1) / kTile);
-  const int64_t slabs = std::max<int64_t>(slabs_of(batch, hidden), 1);
-  const int want = slabs < kSplitBelow[backward] ? (int)((kSplitGroups[backward] + slabs / 2) / slabs) : 1;
-  s.seg_tiles = std::max(1, (s.tiles + want - 1) / want);
-  s.segs = std::max(1, (s.tiles + s.seg_tiles - 1) / s.seg_tiles);
-  return s;
+  const int64_t usual = (pieces + ct - 1) / ct, wide = (pieces + 31) / 32, rounds = (wide + 255) / 256;
+  const bool may = elem_bytes == 2 && hidden >= 4;
+  int groups = 0;  // (no split)
+  l.wide = false;
+  if (usual >= 352) {
+    l.wide = may && (rounds == 1 || 4 * wide >= 3 * 256 * rounds);
+  } else if (usual >= 160) {
+    if (!backward) groups = 768;
+  } else if (usual >= 32 && may) {
+    l.wide = true;
+    groups = backward ? 256 : 512;
+  } else {
+    groups = backward ? 512 : 768;
+  }
+  l.slabs = l.wide ? wide : usual;
+  l.tiles = (int)((seq_len + kTile - 1) / kTile);
+  const int want = std::max(1, (int)((groups + l.slabs / 2) / l.slabs));
+  l.seg_tiles = std::max(1, (l.tiles + want - 1) / want);
+  l.segs = std::max(1, (l.tiles + l.seg_tiles - 1) / l.seg_tiles);
+  return l;
 }
 
 template <typename T>
@@ -73,6 +92,7 @@ struct ScanArgs {
   int64_t channels;            // B H
   int T_, H, tiles, seg_tiles, segs;
   unsigned slabs, pieces;
+  bool wide;
   const int32_t* lengths;
   const float* c0;
   T* out;         // [B][T][H]
@@ -791,78 +811,43 @@ __global__ void __launch_bounds__(kShortThreads) scan_backward_short_kernel(Scan
   });
 }
 
-// Whether to take slabs of 128 channels in 512 threads: rows of 16-bit elements are then read 256 bytes at a time instead
-// of 128 (as 32-bit ones are in the usual slabs).  Not where the time axis has to be split (33 x 1001 x 333, 174
-// slabs: backward 60 -> 77 us), nor where the last round of workgroups, one per CU of 256, would be far from full.
-// Forward / backward, usual -> wide, us: 16 x 4096 x 2048 bf16 (256 wide slabs) 235 / 411 -> 216 / 353; B x 1000 x 256 bf16
-// with 180 wide slabs 58 / 84 -> 53 / 76, with 256 61 / 101 -> 59 / 99, 300 76 / 138 -> 85 / 153, 400 107 / 172 -> 97 / 158, 600
-// 151 / 230 -> 152 / 244, 1000 233 / 371 -> 228 / 363; rows that no line divides, 300 x 2493 x 88 fp16: 158 / 348 -> 145 / 277.
-template <typename T>
-bool wide_slabs(const ScanArgs<T>& p) {
-  const unsigned wide = (p.pieces + 31) / 32, rounds = (wide + 255) / 256;
-  return sizeof(T) == 2 && p.slabs >= kSplitBelow[0] && (rounds == 1 || 4 * wide >= 3 * 256 * rounds);
-}
-
-template <typename T, int VEC, bool GATED>
-hipError_t launch_forward(ScanArgs<T> p, hipStream_t s) {
-  constexpr int CT = VEC == 4 ? 16 : 64, kThreads = Place<VEC, CT>::THREADS;
-  if (p.T_ >= 1 && p.T_ <= kShort) {
-    hipLaunchKernelGGL((scan_forward_short_kernel<T, VEC, GATED>), dim3((p.pieces + kShortThreads - 1) / kShortThreads),
-                       dim3(kShortThreads), 0, s, p);
-    return hipGetLastError();
-  }
+template <typename T, int VEC, int CT, bool GATED, bool BACKWARD>
+hipError_t launch_slabs(const ScanArgs<T>& p, hipStream_t s) {
+  const dim3 block(Place<VEC, CT>::THREADS);
   if (p.segs > 1) {
-    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, false, false>), dim3(p.slabs * (unsigned)(p.segs - 1)),
-                       dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, BACKWARD, BACKWARD && GATED>), dim3(p.slabs * (unsigned)(p.segs - 1)),
+                       block, 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if constexpr (sizeof(T) == 2 && VEC == 4) {
-    if (wide_slabs(p)) {
-      p.slabs = (p.pieces + 31) / 32;
-      hipLaunchKernelGGL((scan_forward_kernel<T, 4, 32, GATED>), dim3(p.slabs), dim3(Place<4, 32>::THREADS), 0, s, p);
-      return hipGetLastError();
-    }
-  }
-  hipLaunchKernelGGL((scan_forward_kernel<T, VEC, CT, GATED>), dim3(p.slabs * (unsigned)p.segs), dim3(kThreads), 0, s,
-                     p);
+  const dim3 grid(p.slabs * (unsigned)p.segs);
+  if constexpr (BACKWARD)
+    hipLaunchKernelGGL((scan_backward_kernel<T, VEC, CT, GATED>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((scan_forward_kernel<T, VEC, CT, GATED>), grid, block, 0, s, p);
   return hipGetLastError();
 }
 
-template <typename T, int VEC, bool GATED>
-hipError_t launch_backward(ScanArgs<T> p, hipStream_t s) {
-  constexpr int CT = VEC == 4 ? 16 : 64, kThreads = Place<VEC, CT>::THREADS;
+template <typename T, int VEC, bool GATED, bool BACKWARD>
+hipError_t launch_vec(const ScanArgs<T>& p, hipStream_t s) {
   if (p.T_ >= 1 && p.T_ <= kShort) {
-    hipLaunchKernelGGL((scan_backward_short_kernel<T, VEC, GATED>), dim3((p.pieces + kShortThreads - 1) / kShortThreads),
-                       dim3(kShortThreads), 0, s, p);
+    const dim3 grid((p.pieces + kShortThreads - 1) / kShortThreads), block(kShortThreads);
+    if constexpr (BACKWARD)
+      hipLaunchKernelGGL((scan_backward_short_kernel<T, VEC, GATED>), grid, block, 0, s, p);
+    else
+      hipLaunchKernelGGL((scan_forward_short_kernel<T, VEC, GATED>), grid, block, 0, s, p);
     return hipGetLastError();
   }
-  if constexpr (sizeof(T) == 2 && VEC == 4) {
-    if (wide_slabs(p)) {
-      p.slabs = (p.pieces + 31) / 32;
-      hipLaunchKernelGGL((scan_backward_kernel<T, 4, 32, GATED>), dim3(p.slabs), dim3(Place<4, 32>::THREADS), 0, s, p);
-      return hipGetLastError();
-    }
-  }
-  if (p.segs > 1) {
-    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, true, GATED>), dim3(p.slabs * (unsigned)(p.segs - 1)),
-                       dim3(kThreads), 0, s, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  hipLaunchKernelGGL((scan_backward_kernel<T, VEC, CT, GATED>), dim3(p.slabs * (unsigned)p.segs), dim3(kThreads), 0, s,
-                     p);
-  return hipGetLastError();
+  if constexpr (sizeof(T) == 2 && VEC == 4)
+    if (p.wide) return launch_slabs<T, 4, 32, GATED, BACKWARD>(p, s);
+  return launch_slabs<T, VEC, VEC == 4 ? 16 : 64, GATED, BACKWARD>(p, s);
 }
 
 template <typename T, bool BACKWARD>
 hipError_t launch_scan(const ScanArgs<T>& p, bool gated, hipStream_t s) {
   const auto go = [&](auto vec) {
     constexpr int V = decltype(vec)::value;
-    if constexpr (BACKWARD)
-      return gated ? launch_backward<T, V, true>(p, s) : launch_backward<T, V, false>(p, s);
-    else
-      return gated ? launch_forward<T, V, true>(p, s) : launch_forward<T, V, false>(p, s);
+    return gated ? launch_vec<T, V, true, BACKWARD>(p, s) : launch_vec<T, V, false, BACKWARD>(p, s);
   };
   return scan_vec(p.H) == 4 ? go(std::integral_constant<int, 4>()) : go(std::integral_constant<int, 1>());
 }
@@ -888,18 +873,18 @@ int check_scan(const char* what, int dtype, const void* gates, int64_t stride_b,
 template <typename T>
 ScanArgs<T> scan_args(const void* gates, int64_t stride_b, int64_t stride_t, int64_t batch, int64_t seq_len, int hidden,
                       const int32_t* lengths, void* workspace, bool backward) {
-  const Split sp = split_for(batch, seq_len, hidden, backward);
+  const Layout l = layout_for(sizeof(T), batch, seq_len, hidden, backward);
   ScanArgs<T> p = {};
   p.gates = (const T*)gates;
   p.stride_b = stride_b, p.stride_t = stride_t;
   p.channels = batch * hidden;
   p.T_ = (int)seq_len, p.H = hidden;
-  p.tiles = sp.tiles, p.seg_tiles = sp.seg_tiles, p.segs = sp.segs;
-  p.slabs = (unsigned)slabs_of(batch, hidden);
+  p.tiles = l.tiles, p.seg_tiles = l.seg_tiles, p.segs = l.segs;
+  p.slabs = (unsigned)l.slabs, p.wide = l.wide;
   p.pieces = (unsigned)pieces_of(batch, hidden);
   p.lengths = lengths;
   p.seg_a = (float*)workspace;
-  p.seg_b = p.seg_a ? p.seg_a + (p.channels * sp.segs + 3) / 4 * 4 : nullptr;
+  p.seg_b = p.seg_a ? p.seg_a + (p.channels * l.segs + 3) / 4 * 4 : nullptr;
   return p;
 }
 
@@ -912,8 +897,9 @@ int64_t plh_gated_scan_states(int64_t seq_len) { return seq_len < 0 ? -1 : (seq_
 
 int64_t plh_gated_scan_workspace_bytes(int64_t batch, int64_t seq_len, int hidden) {
   if (batch < 0 || seq_len < 0 || hidden < 1 || seq_len > (1 << 30) || batch > (1 << 29)) return -1;
-  const int64_t segs = std::max(plh::split_for(batch, seq_len, hidden, false).segs,
-                                plh::split_for(batch, seq_len, hidden, true).segs);
+  int segs = 1;  // the most of any type, in either direction
+  for (int elem : {2, 4})
+    for (bool backward : {false, true}) segs = std::max(segs, plh::layout_for(elem, batch, seq_len, hidden, backward).segs);
   if (segs <= 1) return 0;
   return 2 * ((batch * hidden * segs + 3) / 4 * 4) * (int64_t)sizeof(float);
 }
