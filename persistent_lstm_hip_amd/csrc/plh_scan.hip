@@ -586,7 +586,9 @@ __global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArg
   float carry[VEC];
   load_carry(p.d_cn, at, carry);
   const int tile_first = seg * p.seg_tiles, tile_last = min(p.tiles, (seg + 1) * p.seg_tiles) - 1;
-  fold_segments<T, P, 2>(p, at, p.segs - 1, -1, p.segs - 1 - seg, lds[(tile_last + 1) & 1], carry);
+  const int live_last = min(tile_last, at.live_tiles - 1);
+  // in the half that the first tile, live_last, does not write: no barrier follows
+  fold_segments<T, P, 2>(p, at, p.segs - 1, -1, p.segs - 1 - seg, lds[(live_last + 1) & 1], carry);
   struct Tile : Rows<T, P, true, GATED, true> {
     float start[VEC];  // c before the tile, from the forward pass
     __device__ __forceinline__ void load(const ScanArgs<T>& p, const P& at, int tile) {
@@ -673,7 +675,6 @@ __global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArg
     }
   };
   zero_tiles<kParts>(p.d_gates, p, at, max(tile_first, at.live_tiles), tile_last + 1);
-  const int live_last = min(tile_last, at.live_tiles - 1);
   Tile x, next;  // (as in the forward kernel)
   if (live_last >= tile_first) next.load(p, at, live_last);
   for (int tile = live_last; tile >= tile_first; --tile) {

@@ -92,6 +92,16 @@ def test_scan(gpu, B, T, H, gated, dtype):
     _check_scan(_gates(B, T, H, gated, dtype, 7), None, _lengths("ragged", B, T), gated, what="ragged")
 
 
+@pytest.mark.parametrize("B,T,H", [(2, 3000, 700), (2, 4100, 1000)])
+def test_scan_rows_that_end_anywhere_in_a_segment(gpu, B, T, H):
+    """A time axis that is split into segments of three tiles, or of five: all rows end in each tile of a segment in
+    turn, and the gradient of c_n comes through the steps past them as it is."""
+    _say(f"scan segments' ends {B} {T} {H}")
+    z, c0 = _gates(B, T, H, True, BF16), _rand(B, H, seed=1)
+    for tiles in range(10, 16):
+        _check_scan(z, c0, torch.full((B,), 64 * tiles + 1), True, what=f"{64 * tiles + 1} steps")
+
+
 @pytest.mark.parametrize("place", ["list", "int32 on the device", "int64 on the device"])
 def test_scan_lengths_from_anywhere(gpu, place):
     _say(f"scan lengths {place}")
