@@ -524,7 +524,8 @@ hipError_t launch_norm(NormArgs p, hipStream_t s) {
   return e;
 }
 
-int check_norm(const char* what, int dtype, int wdtype, int64_t stride, int64_t rows, int64_t cols, const void* x) noexcept {
+int check_norm(const char* what, int dtype, int wdtype, int64_t stride, int64_t rows, int64_t cols,
+               const void* x) noexcept {
   if (dtype != PLH_F16 && dtype != PLH_BF16 && dtype != PLH_F32)
     return op_error(PLH_ERR_INVALID, what, "dtype must be PLH_F16, PLH_BF16 or PLH_F32");
   if (wdtype != dtype && wdtype != PLH_F32) return op_error(PLH_ERR_INVALID, what, "wdtype must be dtype or PLH_F32");

@@ -49,14 +49,14 @@ struct Layout {
 // elements may be read 256 bytes at a time, in wide slabs, instead of 128 (as 32-bit ones are in the usual slabs).
 // Measured, us, on 256 CUs, by the number of usual slabs (forward / backward; bf16 or fp16 with output gate):
 //   352 and more: no split; wide slabs, but not where the last round of their workgroups, one per CU, would be far from
-//     full.  usual -> wide: 512 slabs 235 / 411 -> 216 / 353 (16 x 4096 x 2048), B x 1000 x 256 with 360 slabs 58 / 84 -> 53 / 76,
-//     512 61 / 101 -> 59 / 99, 600 76 / 138 -> 85 / 153, 800 107 / 172 -> 97 / 158, 1200 151 / 230 -> 152 / 244, 2000
-//     233 / 371 -> 219 / 359;  rows that no line divides, 300 x 2493 x 88 (413): 158 / 348 -> 145 / 277, in two segments
-//     207 / 401
-//   160 to 351: usual slabs; forward about 768 workgroups (300 slabs with 1, 2, 3, 4 segments: 111, 99, 90, 95), backward
-//     no split (256: 109, 125, 143, 143; 192: 104, 110, 111, 115)
-//   32 to 159: wide slabs for 16 bits; forward 512 workgroups, backward 256.  usual -> wide: 64 slabs 46 / 76 -> 40 / 72, 128
-//     62 / 108 -> 57 / 93, 61 (4 x 12837 x 968) 152 / 289 -> 150 / 254
+//     full.  usual -> wide: 512 slabs 235 / 411 -> 216 / 353 (16 x 4096 x 2048), B x 1000 x 256 with 360 slabs
+//     58 / 84 -> 53 / 76, 512 61 / 101 -> 59 / 99, 600 76 / 138 -> 85 / 153, 800 107 / 172 -> 97 / 158, 1200
+//     151 / 230 -> 152 / 244, 2000 233 / 371 -> 219 / 359;  rows that no line divides, 300 x 2493 x 88 (413):
+//     158 / 348 -> 145 / 277, in two segments 207 / 401
+//   160 to 351: usual slabs; forward about 768 workgroups (300 slabs with 1, 2, 3, 4 segments: 111, 99, 90, 95),
+//     backward no split (256: 109, 125, 143, 143; 192: 104, 110, 111, 115)
+//   32 to 159: wide slabs for 16 bits; forward 512 workgroups, backward 256.  usual -> wide: 64 slabs 46 / 76 ->
+//     40 / 72, 128 62 / 108 -> 57 / 93, 61 (4 x 12837 x 968) 152 / 289 -> 150 / 254
 //   fewer: usual slabs, 768 and 512 workgroups.  20 slabs (2 x 16384 x 640) with 256, 512, 768 workgroups: 85 / 117,
 //     57 / 100, 53 / 95; in wide slabs 54 / 109
 Layout layout_for(int elem_bytes, int64_t batch, int64_t seq_len, int64_t hidden, bool backward) {
@@ -263,13 +263,14 @@ __device__ __forceinline__ void fold_waves(const P& at, const TileMaps<P, SUMS>&
   for (int j = 0; j < VEC; ++j) mine[j] = fmaf(pa[j], before[j], pb[j]);
 }
 
-// Forward, the carry goes from wave to wave, and from the last one to the first one's next tile: slot[w] holds what wave w starts
-// its part of a tile from, tag[w] the number of the tile (from 1 on, in the order of the scan) that it is for.  A wave waits for
-// the one before it alone, so that the waves of a workgroup do not run in step as they would around a barrier: half of
-// them load and store while the others compute (16 x 4096 x 2048 bf16 forward 243 -> 235 us, and with 128-channel
-// slabs, which lose without it, 215).  (The backward pass, where c and E go through a tile in opposite directions, would
-// wait for both in turn: 32 x 2048 x 512 109 -> 127 us.  It composes a tile's maps around one barrier.)  A slot is written for the next tile only after the wave that reads it has sent on what
-// it read.  All waves of a workgroup are resident, so every wait ends.
+// Forward, the carry goes from wave to wave, and from the last one to the first one's next tile: slot[w] holds what
+// wave w starts its part of a tile from, tag[w] the number of the tile (from 1 on, in the order of the scan) that it is
+// for.  A wave waits for the one before it alone, so that the waves of a workgroup do not run in step as they would
+// around a barrier: half of them load and store while the others compute (16 x 4096 x 2048 bf16 forward 243 -> 235 us,
+// and with 128-channel slabs, which lose without it, 215).  (The backward pass, where c and E go through a tile in
+// opposite directions, would wait for both in turn: 32 x 2048 x 512 109 -> 127 us.  It composes a tile's maps around one
+// barrier.)  A slot is written for the next tile only after the wave that reads it has sent on what it read.  All waves
+// of a workgroup are resident, so every wait ends.
 template <typename P>
 struct Relay {
   float slot[P::WAVES][P::SLAB];
@@ -816,8 +817,8 @@ template <typename T, int VEC, int CT, bool GATED, bool BACKWARD>
 hipError_t launch_slabs(const ScanArgs<T>& p, hipStream_t s) {
   const dim3 block(Place<VEC, CT>::THREADS);
   if (p.segs > 1) {
-    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, BACKWARD, BACKWARD && GATED>), dim3(p.slabs * (unsigned)(p.segs - 1)),
-                       block, 0, s, p);
+    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, BACKWARD, BACKWARD && GATED>),
+                       dim3(p.slabs * (unsigned)(p.segs - 1)), block, 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -900,7 +901,8 @@ int64_t plh_gated_scan_workspace_bytes(int64_t batch, int64_t seq_len, int hidde
   if (batch < 0 || seq_len < 0 || hidden < 1 || seq_len > (1 << 30) || batch > (1 << 29)) return -1;
   int segs = 1;  // the most of any type, in either direction
   for (int elem : {2, 4})
-    for (bool backward : {false, true}) segs = std::max(segs, plh::layout_for(elem, batch, seq_len, hidden, backward).segs);
+    for (bool backward : {false, true})
+      segs = std::max(segs, plh::layout_for(elem, batch, seq_len, hidden, backward).segs);
   if (segs <= 1) return 0;
   return 2 * ((batch * hidden * segs + 3) / 4 * 4) * (int64_t)sizeof(float);
 }

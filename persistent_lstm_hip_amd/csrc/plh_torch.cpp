@@ -112,6 +112,11 @@ Tensor device_lengths(const MaybeTensor& lengths, int64_t batch, int64_t seq_len
   TORCH_CHECK_VALUE(n.dim() == 1 && n.numel() == batch && at::isIntegralType(n.scalar_type(), /*includeBool=*/false),
                     "lengths must be a 1-D integer tensor with one entry per batch row");
   if (n.device().is_cpu()) {
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    TORCH_CHECK(hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device.index()), &capturing) == hipSuccess,
+                "the stream's capture status is not known");
+    TORCH_CHECK_VALUE(capturing == hipStreamCaptureStatusNone, "lengths must be on ", device,
+                      " while a graph is captured: its replays would copy them from host memory that is freed by then");
     n = n.to(at::kLong).contiguous();
     const int64_t* v = n.const_data_ptr<int64_t>();
     for (int64_t i = 0; i < batch; ++i)
@@ -164,8 +169,8 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     const int64_t B = gates.size(0), T = gates.size(1), H = states.size(2);
     const at::Device device = gates.device();
     const c10::DeviceGuard guard(device);
-    const Tensor d_out = grads[0].defined() ? incoming(grads[0], gates.scalar_type())
-                                            : at::zeros({B, T, H}, at::TensorOptions().dtype(gates.scalar_type()).device(device));
+    const auto like_gates = at::TensorOptions().dtype(gates.scalar_type()).device(device);
+    const Tensor d_out = grads[0].defined() ? incoming(grads[0], gates.scalar_type()) : at::zeros({B, T, H}, like_gates);
     const Tensor d_cn = grads[1].defined() ? incoming(grads[1], at::kFloat) : Tensor();
     Tensor d_gates = empty(gates.sizes(), gates.scalar_type(), device), d_c0;
     if (ctx->saved_data["has_c0"].toBool() && ctx->needs_input_grad(1)) d_c0 = empty({B, H}, at::kFloat, device);

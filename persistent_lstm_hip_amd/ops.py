@@ -40,7 +40,8 @@ def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, *,
     hidden] of gates' type, c_n [batch, hidden] float32).  c0: the state before the first step, [batch, hidden]
     (default: zeros).  lengths: row b runs lengths[b] steps, as in a packed sequence: its c_n is the state after them,
     its outputs are zero from there on and what gates holds there, NaN included, changes nothing.  A list or a host
-    tensor is checked; a tensor on the device is not (it would synchronise) but taken as clamped to [0, time].
+    tensor is checked; a tensor on the device is not (it would synchronise) but taken as clamped to [0, time].  While a
+    graph is captured lengths must be on the device.
 
     gates may have any batch and time strides, so a time-major projection's transpose runs without a copy.
     Differentiable in gates and c0.

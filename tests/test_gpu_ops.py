@@ -550,6 +550,26 @@ def test_dropout_beyond_32_bits(gpu):
 # ---- together -------------------------------------------------------------------------------------
 
 
+def test_lengths_on_the_host_are_refused_in_a_capture(gpu):
+    """Their copy's source would be freed before a replay."""
+    _say("graph, host lengths")
+    z = _gates(2, 70, 8, True, F16).cuda()
+    n = torch.tensor([70, 3], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        want = P.gated_scan(z, lengths=n)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for host in ([70, 3], torch.tensor([70, 3])):
+                with pytest.raises(ValueError, match="captured"):
+                    P.gated_scan(z, lengths=host)
+            got = P.gated_scan(z, lengths=n)
+        for _ in range(3):
+            got[0].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_operators_in_a_captured_graph(gpu):
     """Every forward in one graph, replayed several times with eager work between the replays, against eager calls;
     the dropout's offset advances on the device."""
