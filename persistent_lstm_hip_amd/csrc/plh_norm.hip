@@ -48,6 +48,25 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
   return v;
 }
 
+// Two sums of a row at once, with one barrier; the buffers are taken in turn, as above.
+template <int LPR>
+__device__ __forceinline__ void row_sums(float& u, float& v, float (*lds)[2]) {
+  constexpr int W = LPR < kWave ? LPR : kWave;
+#pragma unroll
+  for (int d = 1; d < W; d *= 2) {
+    u += __shfl_xor(u, d);
+    v += __shfl_xor(v, d);
+  }
+  if constexpr (LPR > kWave) {
+    constexpr int N = LPR / kWave;
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave][0] = u, lds[threadIdx.x / kWave][1] = v;
+    lds_barrier();
+    u = v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) u += lds[i][0], v += lds[i][1];
+  }
+}
+
 // sum / cols, corrected by its remainder: the mean of equal values is that value.
 __device__ __forceinline__ float mean_of(float sum, const NormArgs& p) {
   const float m = sum * p.inv_cols;
@@ -173,7 +192,7 @@ __global__ void __launch_bounds__(kNormThreads<LPR>, sizeof(T) == 2 || LPR == 10
     norm_backward_kernel(NormArgs p) {
   constexpr int kThreads = kNormThreads<LPR>, kRows = kThreads / LPR;
   constexpr bool kAhead = LPR < (VEC * NV * sizeof(T) > 32 ? 512 : 1024);
-  __shared__ float lds[2][kThreads / kWave];
+  __shared__ alignas(8) float lds[2][kThreads / kWave][2];
   const Pieces<VEC, LPR, NV> at(p.cols);
   float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
 #pragma unroll
@@ -226,7 +245,8 @@ __global__ void __launch_bounds__(kNormThreads<LPR>, sizeof(T) == 2 || LPR == 10
         }
       }
     }
-    const float m1 = row_sum<LPR>(s1, lds[0]) * p.inv_cols, m2 = row_sum<LPR>(s2, lds[1]) * p.inv_cols;
+    row_sums<LPR>(s1, s2, lds[k & 1]);
+    const float m1 = s1 * p.inv_cols, m2 = s2 * p.inv_cols;
     if (!on || !p.d_x) continue;
     T* const dst = static_cast<T*>(p.d_x) + r * p.cols;
 #pragma unroll
