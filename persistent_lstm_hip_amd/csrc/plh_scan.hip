@@ -19,71 +19,20 @@
 namespace plh {
 namespace {
 
-// A workgroup carries a slab of channels through time, 64 steps (a tile) at a time.  A thread has VEC neighbouring
-// channels for R consecutive steps; CT threads side by side read one step of the slab, the groups of so many threads
-// are consecutive in time.  A row's channels are cut into pieces of VEC, the last of which is moved back to end with
-// the row: its channels are then carried by two threads, which compute and store the same.  Pieces are numbered row
-// after row, so that slabs are full whatever H is.
-//   VEC 4, CT 16: 256 threads, 64 channels, 4 steps each (the usual slab)
-//   VEC 4, CT 32: 512 threads, 128 channels, 4 steps each (see layout_for)
-//   VEC 1, CT 64: 256 threads, 64 channels, 16 steps each (H < 4)
-constexpr int kTile = 64;  // steps
-template <int CT>
-constexpr int kSlabThreads = CT == 32 ? 512 : 256;
-
-// Channels per thread.
-inline int scan_vec(int64_t hidden) { return hidden >= 4 ? 4 : 1; }
-
-int64_t pieces_of(int64_t batch, int64_t hidden) { return batch * ((hidden + scan_vec(hidden) - 1) / scan_vec(hidden)); }
-
-// How a call is laid out on the device.
-struct Layout {
-  bool wide;      // slabs of 128 channels
-  int64_t slabs;
-  int tiles;      // tiles of a row
-  int seg_tiles;  // ... of a segment
-  int segs;       // segments of the time axis
-};
-
-// With few slabs the time axis is split into segments, whose maps a launch of its own computes first.  Rows of 16-bit
-// elements may be read 256 bytes at a time, in wide slabs, instead of 128 (as 32-bit ones are in the usual slabs).
-// Measured, us, on 256 CUs, by the number of usual slabs (forward / backward; bf16 or fp16 with output gate):
-//   352 and more: no split; wide slabs, but not where the last round of their workgroups, one per CU, would be far from
-//     full.  usual -> wide: 512 slabs 235 / 411 -> 216 / 353 (16 x 4096 x 2048), B x 1000 x 256 with 360 slabs
-//     58 / 84 -> 53 / 76, 512 61 / 101 -> 59 / 99, 600 76 / 138 -> 85 / 153, 800 107 / 172 -> 97 / 158, 1200
-//     151 / 230 -> 152 / 244, 2000 233 / 371 -> 219 / 359;  rows that no line divides, 300 x 2493 x 88 (413):
-//     158 / 348 -> 145 / 277, in two segments 207 / 401
-//   160 to 351: usual slabs; forward about 768 workgroups (300 slabs with 1, 2, 3, 4 segments: 111, 99, 90, 95),
-//     backward no split (256: 109, 125, 143, 143; 192: 104, 110, 111, 115)
-//   32 to 159: wide slabs for 16 bits; forward 512 workgroups, backward 256.  usual -> wide: 64 slabs 46 / 76 ->
-//     40 / 72, 128 62 / 108 -> 57 / 93, 61 (4 x 12837 x 968) 152 / 289 -> 150 / 254
-//   fewer: usual slabs, 768 and 512 workgroups.  20 slabs (2 x 16384 x 640) with 256, 512, 768 workgroups: 85 / 117,
-//     57 / 100, 53 / 95; in wide slabs 54 / 109
-Layout layout_for(int elem_bytes, int64_t batch, int64_t seq_len, int64_t hidden, bool backward) {
-  Layout l;
-  const int64_t pieces = std::max<int64_t>(pieces_of(batch, hidden), 1);
-  const int ct = hidden >= 4 ? 16 : 64;
-  const int64_t usual = (pieces + ct - 1) / ct, wide = (pieces + 31) / 32, rounds = (wide + 255) / 256;
-  const bool may = elem_bytes == 2 && hidden >= 4;
-  int groups = 0;  // (no split)
-  l.wide = false;
-  if (usual >= 352) {
-    l.wide = may && (rounds == 1 || 4 * wide >= 3 * 256 * rounds);
-  } else if (usual >= 160) {
-    if (!backward) groups = 768;
-  } else if (usual >= 32 && may) {
-    l.wide = true;
-    groups = backward ? 256 : 512;
-  } else {
-    groups = backward ? 512 : 768;
-  }
-  l.slabs = l.wide ? wide : usual;
-  l.tiles = (int)((seq_len + kTile - 1) / kTile);
-  const int want = std::max(1, (int)((groups + l.slabs / 2) / l.slabs));
-  l.seg_tiles = std::max(1, (l.tiles + want - 1) / want);
-  l.segs = std::max(1, (l.tiles + l.seg_tiles - 1) / l.seg_tiles);
-  return l;
-}
+// A workgroup carries a slab of channels through time, a tile of steps at a time.  A thread has VEC neighbouring channels
+// for R consecutive steps; CT threads side by side read one step of the slab, the TG groups of so many threads are
+// consecutive in time.  A row's channels are cut into pieces of VEC, the last of which is moved back to end with the
+// row: its channels are then carried by two threads, which compute and store the same.  Pieces are numbered row after
+// row, so that slabs are full whatever H is.
+constexpr int kTile = 64;  // steps of a tile where there can be several (MANY): its loads are then in flight one ahead
+template <int VEC, int CT, int TG, int R, bool MANY>
+struct Place;
+using Usual = Place<4, 16, 16, 4, true>;     // 256 threads, 64 channels, 64 steps
+using Wide = Place<4, 32, 16, 4, true>;      // 512 threads, 128 channels, 64 steps (see layout_for)
+using Narrow = Place<1, 64, 4, 16, true>;    // 256 threads, 64 channels, 64 steps: H < 4
+using Steps64 = Place<4, 16, 16, 4, false>;  // 256 threads and one tile: 64 channels, 64 steps,
+using Steps32 = Place<4, 32, 8, 4, false>;   // 128 channels, 32 steps,
+using Steps16 = Place<4, 64, 4, 4, false>;   // 256 channels, 16 steps
 
 template <typename T>
 struct ScanArgs {
@@ -92,7 +41,7 @@ struct ScanArgs {
   int64_t channels;            // B H
   int T_, H, tiles, seg_tiles, segs;
   unsigned slabs, pieces;
-  bool wide;
+  int ct;
   const int32_t* lengths;
   const float* c0;
   T* out;         // [B][T][H]
@@ -114,14 +63,13 @@ __device__ __forceinline__ unsigned slab_of(unsigned i, unsigned n) {
 }
 
 // Where a thread stands: its channels, its place among the time groups, its row's length.
-template <int VEC_, int CT_>
+template <int VEC_, int CT_, int TG_, int R_, bool MANY_>
 struct Place {
-  static constexpr int VEC = VEC_, CT = CT_;
-  static constexpr int TG = VEC == 4 ? 16 : 4;          // time groups
-  static constexpr int R = kTile / TG;                  // steps of a thread
-  static constexpr int THREADS = kSlabThreads<CT>, WAVES = THREADS / kWave, SLAB = CT * VEC;
-  static_assert(THREADS == CT * TG && ((VEC == 4 && (CT == 16 || CT == 32)) || (VEC == 1 && CT == 64)),
-                "four, two or one time groups in a wave");
+  static constexpr int VEC = VEC_, CT = CT_, TG = TG_, R = R_;
+  static constexpr bool MANY = MANY_;
+  static constexpr int TILE = TG * R, THREADS = CT * TG, WAVES = THREADS / kWave, SLAB = CT * VEC;
+  static_assert(CT == 16 || CT == 32 || CT == 64, "four, two or one time groups in a wave");
+  static_assert(TILE == kTile || (!MANY && TILE < kTile), "states are stored every kTile steps");
   int lane, wave, ct, tg;
   bool on;
   int64_t b, n;  // row; first channel, counted over all rows
@@ -146,9 +94,72 @@ struct Place {
     int most = len;
 #pragma unroll
     for (int d = 1; d < CT; d *= 2) most = max(most, __shfl_xor(most, d));
-    live_tiles = __builtin_amdgcn_readfirstlane((most + kTile - 1) / kTile);
+    live_tiles = __builtin_amdgcn_readfirstlane((most + TILE - 1) / TILE);
   }
 };
+
+// Channels per thread.
+inline int scan_vec(int64_t hidden) { return hidden >= 4 ? 4 : 1; }
+
+int64_t pieces_of(int64_t batch, int64_t hidden) { return batch * ((hidden + scan_vec(hidden) - 1) / scan_vec(hidden)); }
+
+// How a call is laid out on the device.
+struct Layout {
+  int ct;         // the slabs' CT
+  int64_t slabs;
+  int tiles;      // tiles of a row
+  int seg_tiles;  // ... of a segment
+  int segs;       // segments of the time axis
+};
+
+// Up to 64 steps take one tile of a size that they fill (forward / backward us; where every call has tiles of 64 steps and
+// room for the next one's loads, and here): 300 rows of 512 bf16, 16 steps 15.7 / 24.5 and 7.3 / 11.1, 32 steps
+// 16.5 / 27.9 and 10.2 / 17.6, 33 steps 16.9 / 28.1 and 14.8 / 23.2, 64 steps 19.6 / 36.2 and 18.3 / 35.8; 400 x 15 x 400
+// fp32 17.0 / 36.0 and 7.8 / 12.2.
+// More steps: with few slabs the time axis is split into segments, whose maps a launch of its own computes first.  Rows of 16-bit
+// elements may be read 256 bytes at a time, in wide slabs, instead of 128 (as 32-bit ones are in the usual slabs).
+// Measured, us, on 256 CUs, by the number of usual slabs (forward / backward; bf16 or fp16 with output gate):
+//   352 and more: no split; wide slabs, but not where the last round of their workgroups, one per CU, would be far from
+//     full.  usual -> wide: 512 slabs 235 / 411 -> 216 / 353 (16 x 4096 x 2048), B x 1000 x 256 with 360 slabs
+//     58 / 84 -> 53 / 76, 512 61 / 101 -> 59 / 99, 600 76 / 138 -> 85 / 153, 800 107 / 172 -> 97 / 158, 1200
+//     151 / 230 -> 152 / 244, 2000 233 / 371 -> 219 / 359;  rows that no line divides, 300 x 2493 x 88 (413):
+//     158 / 348 -> 145 / 277, in two segments 207 / 401
+//   160 to 351: usual slabs; forward about 768 workgroups (300 slabs with 1, 2, 3, 4 segments: 111, 99, 90, 95),
+//     backward no split (256: 109, 125, 143, 143; 192: 104, 110, 111, 115)
+//   32 to 159: wide slabs for 16 bits; forward 512 workgroups, backward 256.  usual -> wide: 64 slabs 46 / 76 ->
+//     40 / 72, 128 62 / 108 -> 57 / 93, 61 (4 x 12837 x 968) 152 / 289 -> 150 / 254
+//   fewer: usual slabs, 768 and 512 workgroups.  20 slabs (2 x 16384 x 640) with 256, 512, 768 workgroups: 85 / 117,
+//     57 / 100, 53 / 95; in wide slabs 54 / 109
+Layout layout_for(int elem_bytes, int64_t batch, int64_t seq_len, int64_t hidden, bool backward) {
+  const int64_t pieces = std::max<int64_t>(pieces_of(batch, hidden), 1);
+  if (hidden >= 4 && seq_len <= kTile) {
+    const int ct = seq_len <= Steps16::TILE ? Steps16::CT : seq_len <= Steps32::TILE ? Steps32::CT : Steps64::CT;
+    return {ct, (pieces + ct - 1) / ct, seq_len > 0, 1, 1};
+  }
+  Layout l;
+  l.ct = hidden >= 4 ? Usual::CT : Narrow::CT;
+  const int64_t usual = (pieces + l.ct - 1) / l.ct, wide = (pieces + 31) / 32, rounds = (wide + 255) / 256;
+  const bool may = elem_bytes == 2 && hidden >= 4;
+  int groups = 0;  // (no split)
+  bool take_wide = false;
+  if (usual >= 352) {
+    take_wide = may && (rounds == 1 || 4 * wide >= 3 * 256 * rounds);
+  } else if (usual >= 160) {
+    if (!backward) groups = 768;
+  } else if (usual >= 32 && may) {
+    take_wide = true;
+    groups = backward ? 256 : 512;
+  } else {
+    groups = backward ? 512 : 768;
+  }
+  if (take_wide) l.ct = Wide::CT;
+  l.slabs = take_wide ? wide : usual;
+  l.tiles = (int)((seq_len + kTile - 1) / kTile);
+  const int want = std::max(1, (int)((groups + l.slabs / 2) / l.slabs));
+  l.seg_tiles = std::max(1, (l.tiles + want - 1) / want);
+  l.segs = std::max(1, (l.tiles + l.seg_tiles - 1) / l.seg_tiles);
+  return l;
+}
 
 // v of the even and of the odd time group of a pair of groups, in both (one exchange per level and value).
 template <int LEVEL>
@@ -355,7 +366,7 @@ struct Rows {
   Vec<T, VEC> f[R], g[R], o[R], d[R];
 
   __device__ __forceinline__ void load(const ScanArgs<T>& p, const P& at, int tile) {
-    const int t0 = tile * kTile + at.tg * R;
+    const int t0 = tile * P::TILE + at.tg * R;
     const T* src = p.gates + at.b * p.stride_b + (int64_t)t0 * p.stride_t + at.h;
     const T* grad = D ? p.d_out + (at.b * p.T_ + t0) * (int64_t)p.H + at.h : nullptr;
     const auto row = [&](int r) {
@@ -402,8 +413,8 @@ template <int PARTS, typename P, typename T>
 __device__ __forceinline__ void zero_tiles(T* dst, const ScanArgs<T>& p, const P& at, int first, int end) {
   if (!at.on) return;
   const Vec<T, P::VEC> zero = {};
-  const int t_end = min(end * kTile, p.T_);
-  for (int t = first * kTile + at.tg; t < t_end; t += P::TG) {
+  const int t_end = min(end * P::TILE, p.T_);
+  for (int t = first * P::TILE + at.tg; t < t_end; t += P::TG) {
     T* const q = dst + (at.b * p.T_ + t) * (int64_t)(PARTS * p.H) + at.h;
 #pragma unroll
     for (int k = 0; k < PARTS; ++k) store_vec(q + k * p.H, zero);
@@ -430,17 +441,16 @@ __device__ __forceinline__ void store_carry(float* dst, const P& at, const float
 
 // The maps of the segments, for the launch that follows: of all but the last in order (of c), or of all but the first
 // in reverse order (of E).  Each time group composes a run of the segment, and the runs are composed once at the end.
-template <typename T, int VEC, int CT, bool REVERSE, bool GATED>
-__global__ void __launch_bounds__(kSlabThreads<CT>) scan_maps_kernel(ScanArgs<T> p) {
-  using P = Place<VEC, CT>;
-  constexpr int R = P::R;
+template <typename T, typename P, bool REVERSE, bool GATED>
+__global__ void __launch_bounds__(P::THREADS) scan_maps_kernel(ScanArgs<T> p) {
+  constexpr int VEC = P::VEC, R = P::R;
   __shared__ alignas(16) TileMaps<P, 1> lds;
   const int seg = blockIdx.x / p.slabs + (REVERSE ? 1 : 0);
   const P at(p, slab_of(blockIdx.x % p.slabs, p.slabs));
   float A[VEC], B[1][VEC], pa[1][VEC], pb[1][VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = 0.0f;
-  const int run = p.seg_tiles * R, first = seg * p.seg_tiles * kTile + at.tg * run;
+  const int run = p.seg_tiles * R, first = seg * p.seg_tiles * P::TILE + at.tg * run;
   const int steps = min(run, at.len - first);
   const T* const src = p.gates + at.b * p.stride_b + (int64_t)first * p.stride_t + at.h;
   const T* const grad = REVERSE ? p.d_out + (at.b * p.T_ + first) * (int64_t)p.H + at.h : nullptr;
@@ -501,10 +511,9 @@ __global__ void __launch_bounds__(kSlabThreads<CT>) scan_maps_kernel(ScanArgs<T>
   store_carry(p.seg_b + (int64_t)seg * p.channels, at, sum);
 }
 
-template <typename T, int VEC, int CT, bool GATED>
-__global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan_forward_kernel(ScanArgs<T> p) {
-  using P = Place<VEC, CT>;
-  constexpr int R = P::R;
+template <typename T, typename P, bool GATED>
+__global__ void __launch_bounds__(P::THREADS, sizeof(T) == 2 ? 4 : 1) scan_forward_kernel(ScanArgs<T> p) {
+  constexpr int VEC = P::VEC, R = P::R;
   __shared__ alignas(16) TileMaps<P, 1> lds;
   __shared__ alignas(16) Relay<P> relay;
   const int seg = blockIdx.x / p.slabs;
@@ -519,7 +528,7 @@ __global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan
   uint32_t round = 0;
   using Tile = Rows<T, P, true, GATED, false>;
   const auto process = [&](const Tile& x, int tile) __attribute__((always_inline)) {
-    const int t0 = tile * kTile + at.tg * R;
+    const int t0 = tile * P::TILE + at.tg * R;
     float a[R][VEC], b[R][VEC], A[VEC], B[1][VEC], pa[1][VEC], pb[1][VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[0][j] = 0.0f;
@@ -565,7 +574,7 @@ __global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan
   if (tile_first < live_end) next.load(p, at, tile_first);
   for (int tile = tile_first; tile < live_end; ++tile) {
     x = next;
-    if (tile + 1 < live_end) next.load(p, at, tile + 1);
+    if (P::MANY && tile + 1 < live_end) next.load(p, at, tile + 1);
     process(x, tile);
   }
   zero_tiles<1>(p.out, p, at, max(tile_first, live_end), tile_end);
@@ -576,10 +585,9 @@ __global__ void __launch_bounds__(kSlabThreads<CT>, sizeof(T) == 2 ? 4 : 1) scan
 }
 
 // Backward: tiles from the last to the first.
-template <typename T, int VEC, int CT, bool GATED>
-__global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArgs<T> p) {
-  using P = Place<VEC, CT>;
-  constexpr int R = P::R;
+template <typename T, typename P, bool GATED>
+__global__ void __launch_bounds__(P::THREADS) scan_backward_kernel(ScanArgs<T> p) {
+  constexpr int VEC = P::VEC, R = P::R;
   constexpr int kParts = GATED ? 3 : 2;
   __shared__ alignas(16) WaveMaps<P, 2> lds;
   const int seg = blockIdx.x / p.slabs;
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArg
     }
   };
   const auto process = [&](const Tile& x, int tile) __attribute__((always_inline)) {
-    const int t0 = tile * kTile + at.tg * R;
+    const int t0 = tile * P::TILE + at.tg * R;
     float a[R][VEC], na[R][VEC], u[R][VEC], w[R][VEC];  // a, 1 - a, u = s dh, w = (1 - s) u
     float A[VEC], B[2][VEC], pa[2][VEC], pb[2][VEC];    // sums in order (for c) and in reverse order (for E)
 #pragma unroll
@@ -680,7 +688,7 @@ __global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArg
   if (live_last >= tile_first) next.load(p, at, live_last);
   for (int tile = live_last; tile >= tile_first; --tile) {
     x = next;
-    if (tile > tile_first) next.load(p, at, tile - 1);
+    if (P::MANY && tile > tile_first) next.load(p, at, tile - 1);
     process(x, tile);
   }
   if (at.on && at.tg == 0 && seg == 0 && p.d_c0) store_carry(p.d_c0, at, carry);
@@ -688,9 +696,9 @@ __global__ void __launch_bounds__(kSlabThreads<CT>) scan_backward_kernel(ScanArg
 
 // ---- a few steps ----
 // One step (serving) or up to eight: a thread carries VEC channels through them one after the other, nothing to scan.
-// The tiled kernels leave most of a tile idle there: 1000 rows of 2 x 512 fp16 forward / backward 41 / 69 us, here
-// 5.1 / 6.1; 400 x 8 x 400 fp32 15 / 37 and 7.3 / 9.2.  With more steps the chain of loads takes over: 300 x 16 x 512
-// bf16 forward 14.7 and 13.9 us, 8 x 16 x 512 4.2 and 8.3.
+// In tiles of 16 steps and here, forward / backward us: 199 x 5 x 2048 bf16 9.9 / 15.4 and 7.7 / 8.8, 2000 x 8 x 256
+// 11.5 / 18.8 and 10.5 / 12.3, 400 x 8 x 400 fp32 7.0 / 11.1 and 7.4 / 9.3.  With more steps the chain of loads takes
+// over: 300 x 16 x 512 bf16 forward 7.3 and 13.9.
 constexpr int kShort = 8;
 constexpr int kShortThreads = 256;
 
@@ -813,20 +821,22 @@ __global__ void __launch_bounds__(kShortThreads) scan_backward_short_kernel(Scan
   });
 }
 
-template <typename T, int VEC, int CT, bool GATED, bool BACKWARD>
+template <typename T, typename P, bool GATED, bool BACKWARD>
 hipError_t launch_slabs(const ScanArgs<T>& p, hipStream_t s) {
-  const dim3 block(Place<VEC, CT>::THREADS);
-  if (p.segs > 1) {
-    hipLaunchKernelGGL((scan_maps_kernel<T, VEC, CT, BACKWARD, BACKWARD && GATED>),
-                       dim3(p.slabs * (unsigned)(p.segs - 1)), block, 0, s, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+  const dim3 block(P::THREADS);
+  if constexpr (P::MANY) {
+    if (p.segs > 1) {
+      hipLaunchKernelGGL((scan_maps_kernel<T, P, BACKWARD, BACKWARD && GATED>),
+                         dim3(p.slabs * (unsigned)(p.segs - 1)), block, 0, s, p);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
   }
   const dim3 grid(p.slabs * (unsigned)p.segs);
   if constexpr (BACKWARD)
-    hipLaunchKernelGGL((scan_backward_kernel<T, VEC, CT, GATED>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((scan_backward_kernel<T, P, GATED>), grid, block, 0, s, p);
   else
-    hipLaunchKernelGGL((scan_forward_kernel<T, VEC, CT, GATED>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((scan_forward_kernel<T, P, GATED>), grid, block, 0, s, p);
   return hipGetLastError();
 }
 
@@ -840,9 +850,16 @@ hipError_t launch_vec(const ScanArgs<T>& p, hipStream_t s) {
       hipLaunchKernelGGL((scan_forward_short_kernel<T, VEC, GATED>), grid, block, 0, s, p);
     return hipGetLastError();
   }
-  if constexpr (sizeof(T) == 2 && VEC == 4)
-    if (p.wide) return launch_slabs<T, 4, 32, GATED, BACKWARD>(p, s);
-  return launch_slabs<T, VEC, VEC == 4 ? 16 : 64, GATED, BACKWARD>(p, s);
+  if constexpr (VEC == 1) {
+    return launch_slabs<T, Narrow, GATED, BACKWARD>(p, s);
+  } else {
+    if (p.T_ <= Steps16::TILE) return launch_slabs<T, Steps16, GATED, BACKWARD>(p, s);
+    if (p.T_ <= Steps32::TILE) return launch_slabs<T, Steps32, GATED, BACKWARD>(p, s);
+    if (p.T_ <= Steps64::TILE) return launch_slabs<T, Steps64, GATED, BACKWARD>(p, s);
+    if constexpr (sizeof(T) == 2)
+      if (p.ct == Wide::CT) return launch_slabs<T, Wide, GATED, BACKWARD>(p, s);
+    return launch_slabs<T, Usual, GATED, BACKWARD>(p, s);
+  }
 }
 
 template <typename T, bool BACKWARD>
@@ -882,7 +899,7 @@ ScanArgs<T> scan_args(const void* gates, int64_t stride_b, int64_t stride_t, int
   p.channels = batch * hidden;
   p.T_ = (int)seq_len, p.H = hidden;
   p.tiles = l.tiles, p.seg_tiles = l.seg_tiles, p.segs = l.segs;
-  p.slabs = (unsigned)l.slabs, p.wide = l.wide;
+  p.slabs = (unsigned)l.slabs, p.ct = l.ct;
   p.pieces = (unsigned)pieces_of(batch, hidden);
   p.lengths = lengths;
   p.seg_a = (float*)workspace;

@@ -36,10 +36,12 @@ def _gates(B, T, H, gated, dtype, seed=0):
 
 
 # (B, T, H): one of everything; no steps; odd; one and several tiles; a time axis that is split; many rows; a few steps;
-# rows of few channels; as many rows as it takes for slabs of either width, split in both directions, in one, or not
+# rows of few channels; as many rows as it takes for slabs of either width, split in both directions, in one, or not;
+# one tile of each size
 SCAN_SHAPES = [(1, 1, 1), (3, 0, 5), (0, 4, 3), (2, 64, 64), (2, 65, 60), (5, 129, 7), (1, 2500, 24), (2, 700, 130),
                (70, 33, 61), (300, 5, 200), (9, 8, 51), (9, 9, 51), (40, 2, 2), (2, 300, 3),
-               (33, 70, 1000), (24, 130, 1000), (8, 700, 402), (45, 200, 264), (75, 70, 512)]
+               (33, 70, 1000), (24, 130, 1000), (8, 700, 402), (45, 200, 264), (75, 70, 512),
+               (3, 16, 260), (30, 12, 70), (5, 17, 130), (2, 32, 517), (1, 63, 1030)]
 
 
 def _lengths(kind, B, T):
