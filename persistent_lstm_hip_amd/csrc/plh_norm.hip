@@ -48,7 +48,8 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
   return v;
 }
 
-// Two sums of a row at once, with one barrier; the buffers are taken in turn, as above.
+// Two sums of a row at once, with one barrier; the buffers are taken in turn, as above.  (A row's two barriers cost the
+// backward pass of 16384 x 8192 bf16 14 us of 166, and 4000 x 12000 fp32, whose workgroup fills a CU, 50 of 171.)
 template <int LPR>
 __device__ __forceinline__ void row_sums(float& u, float& v, float (*lds)[2]) {
   constexpr int W = LPR < kWave ? LPR : kWave;
@@ -501,7 +502,8 @@ hipError_t launch_vec(const NormArgs& p, const Shape& sh, hipStream_t s) {
 // Workgroups of the backward pass, of `threads` threads with `side` rows side by side, each with a row of partial sums:
 // 1024 threads per CU with one piece per thread, 512 with more (longer rows, whose partial sums weigh more), one
 // workgroup at least.  With 512 and 1024 threads per CU: 512000 x 128 fp16 83 and 79 us, 300000 x 129 84 and 68,
-// 65536 x 1024 bf16 77 and 82, 7301 x 1001 fp16 16.9 and 18.3, 30000 x 2048 fp32 137 and 145.
+// 65536 x 1024 bf16 77 and 82, 7301 x 1001 fp16 16.6 and 18.5, 30000 x 2048 fp32 137 and 145, 16384 x 8192 bf16 153 and
+// 163.
 int64_t groups_for(int64_t rows, int threads, int side, int nv) {
   const int64_t most = std::max(256, 256 * (nv == 1 ? 1024 : 512) / threads);
   return std::max<int64_t>(1, std::min<int64_t>((rows + side - 1) / side, most));
