@@ -95,7 +95,9 @@ int64_t hidden_of(const Tensor& gates, bool output_gate) {
   const int64_t width = gates.size(-1), parts = output_gate ? 3 : 2;
   TORCH_CHECK_VALUE(width > 0 && width % parts == 0, "gates needs ", parts, " * hidden columns (f, g",
                     output_gate ? ", o" : "", "), not ", width);
-  return width / parts;
+  const int64_t hidden = width / parts;  // (an int in the C ABI, which checks what fits one)
+  TORCH_CHECK_VALUE(hidden <= 1 << 24, "hidden must not exceed 2^24, not ", hidden);
+  return hidden;
 }
 
 // gates itself where its last dimension is dense (any other strides), else a copy.

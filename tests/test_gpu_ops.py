@@ -634,6 +634,16 @@ def test_operators_refuse_on_the_device(gpu):
             bad()
 
 
+def test_hidden_beyond_an_int_is_refused(gpu):
+    _say("hidden beyond an int")  # 2^32 + 4 would be 4 in 32 bits; expanded, so that nothing of the size exists
+    z, c = torch.zeros(1, 1, 1, device="cuda"), torch.zeros(1, 1, device="cuda")
+    for hidden in ((1 << 24) + 1, 1 << 31, (1 << 32) + 4):
+        with pytest.raises(ValueError, match="hidden"):
+            P.gated_scan(z.expand(1, 1, 3 * hidden))
+        with pytest.raises(ValueError, match="hidden"):
+            P.gated_scan_step(z[0].expand(1, 3 * hidden), c.expand(1, hidden))
+
+
 def test_gradients_of_another_type_are_converted(gpu):
     _say("gradient types")
     x = torch.randn(4, 24, device="cuda").half().requires_grad_(True)
