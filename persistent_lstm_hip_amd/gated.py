@@ -48,7 +48,11 @@ class GatedScanBlock(nn.Module):
 
 
 class GatedScanRegressor(nn.Module):
-    """x [batch, time, input_dim] -> [batch, output_dim], read off at every row's last step."""
+    """x [batch, time, input_dim] -> [batch, output_dim], read off at every row's last step.
+
+    In training mode every layer of every pass draws a dropout mask of its own under `seed` (torch.initial_seed() unless
+    set).  The passes are counted from the model's construction on and are not in its state_dict: a resumed run, or a
+    second model of a process, sets another seed."""
 
     def __init__(self, input_dim: int, hidden_dim: int, output_dim: int, n_layers: int, dropout: float = 0.2):
         super().__init__()

@@ -74,6 +74,30 @@ def test_model_and_its_gradients(gpu, H, L, ragged):
         assert (a.cpu().double() - b).abs().max() <= tol * max(1.0, b.abs().max().item()), name
 
 
+def test_model_under_autocast(gpu):
+    """fp32 parameters and fp16 products: the block's operators take a mixture of the two as autocast makes it."""
+    _say("autocast")
+    B, T, I, H, L, O, p = 5, 70, 3, 61, 2, 4, 0.25
+    m = _model(I, H, O, L, p)
+    g = torch.Generator().manual_seed(1)
+    x, d = torch.randn(B, T, I, generator=g), torch.randn(B, O, generator=g)
+    lengths = torch.tensor([70, 1, 64, 0, 33])
+    with torch.autocast("cuda", dtype=torch.float16):
+        out = m(x.cuda(), lengths)
+    assert out.dtype == torch.float16
+    grads = torch.autograd.grad(out.float(), list(m.parameters()), d.cuda())
+    params = {n: t.detach().cpu().double().requires_grad_(True) for n, t in m.named_parameters()}
+    want = _plain_forward(params, x.double(), lengths, L, p, m.seed, 0)
+    want_grads = torch.autograd.grad(want, list(params.values()), d.double())
+    # 6 L + 3 = 15 stages rounded to 11 bits, weights too, each amplified by at most a few by the norms behind it: 64
+    # units; the gradients go through as many again
+    u16 = 2.0 ** -11
+    assert (out.detach().cpu().double() - want.detach()).abs().max() <= 64 * u16 * max(1.0, want.abs().max().item())
+    for name, a, b in zip(params, grads, want_grads):
+        assert a.dtype == torch.float32, name
+        assert (a.cpu().double() - b).abs().max() <= 128 * u16 * max(1.0, b.abs().max().item()), name
+
+
 @pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-4), (torch.float16, 2e-2)])
 def test_serving_step_by_step_is_the_forward_pass(gpu, dtype, tol):
     _say(f"serve {dtype}")
