@@ -6,7 +6,9 @@
 // No kernel is in this file, and the library itself does not depend on torch.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -76,17 +78,28 @@ Tensor incoming(const Tensor& grad, at::ScalarType type) { return grad.to(type).
 
 // In a node below, needs_input_grad counts the tensors that it was given (an optional that holds none is not counted).
 
-// What a node's backward pass returns can be differentiated no further: asked for a second derivative it raises.
-variable_list once(variable_list grads, const variable_list& incoming, const char* what) {
+// What the backward pass of the node that runs returns can be differentiated no further: asked for a second derivative it
+// raises.  Gradients depend on the incoming ones and, where the node is not linear in its first input, on its first
+// `inputs` inputs: with a loss that is linear in the output only those are tracked.  The raising node is linked to all of
+// them, as a derivative's own would be: the engine leaves out what does not lead to the tensors that it is asked for.
+// Where nothing is tracked the gradients are constants.
+variable_list once(variable_list grads, const variable_list& incoming, uint32_t inputs, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::edge_list edges = torch::autograd::collect_next_edges(incoming);
+  const auto node = torch::autograd::get_current_node();
+  if (inputs > 0 && node->next_edge(0).is_valid())
+    for (uint32_t i = 0; i < inputs; ++i) edges.push_back(node->next_edge(i));
   bool any = false;
-  for (const Tensor& g : incoming) any = any || tracks(g);
+  for (const auto& e : edges) any = any || e.is_valid();
   if (!any) return grads;
-  for (Tensor& g : grads)
-    if (g.defined()) g = g.detach().requires_grad_(true);
-  auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once only",
-                                                              (int64_t)grads.size());
-  return (*node)(std::move(grads));
+  const auto raises =
+      std::make_shared<torch::autograd::Error>(std::string(what) + " is differentiable once only", std::move(edges));
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    torch::autograd::create_gradient_edge(g, raises);
+  }
+  return grads;
 }
 
 // ---- gated linear recurrence --------------------------------------------------------------------
@@ -182,7 +195,8 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
                                   ptr<float>(d_cn), ptr(d_gates), ptr<float>(d_c0), ptr(ws),
                                   ws.defined() ? ws.numel() : 0, stream_of(gates)),
           "gated_scan backward");
-    return once({d_gates, d_c0, Tensor(), Tensor()}, grads, "gated_scan");
+    // (linear in c0 alone)
+    return once({d_gates, d_c0, Tensor(), Tensor()}, grads, ctx->saved_data["has_c0"].toBool() ? 2 : 1, "gated_scan");
   }
 };
 
@@ -285,7 +299,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                                   ptr(w), mean, mean ? mean + rows : nullptr, ptr(d_y), ptr(d_x), ptr(d_w), ptr(d_b),
                                   ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(m)),
           "layer_norm backward");
-    return once({d_x, d_w, d_b, Tensor()}, grads, "layer_norm");
+    // (linear in weight and bias alone; no gradient depends on the bias)
+    return once({d_x, d_w, d_b, Tensor()}, grads, has & 1 ? 2 : 1, "layer_norm");
   }
 };
 
@@ -344,7 +359,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     if (ctx->needs_input_grad(0))
       d_x = dropout(d_out, Tensor(), Mask{(int)m[0], (uint64_t)m[1], (uint64_t)m[2]}, saved[0]);
     if (ctx->saved_data["has_residual"].toBool() && ctx->needs_input_grad(1)) d_r = d_out;
-    return once({d_x, d_r, Tensor(), Tensor(), Tensor(), Tensor()}, grads, "dropout_add");
+    return once({d_x, d_r, Tensor(), Tensor(), Tensor(), Tensor()}, grads, 0, "dropout_add");  // (linear in both)
   }
 };
 
