@@ -34,17 +34,25 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
+// A dual tensor of forward-mode differentiation need not have requires_grad: its tangent would be dropped.
+void check_no_tangent(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(!t._fw_grad(/*level=*/0).defined(), name,
+                    " carries a forward-mode tangent: the block operators have reverse-mode gradients only");
+}
+
 int check_tensor(const Tensor& t, const char* name, int64_t dims = -1) {
   TORCH_CHECK_VALUE(t.is_cuda(), name, " must be on a HIP device: this library has no CPU path");
   const int code = dtype_code(t.scalar_type());
   TORCH_CHECK_VALUE(code >= 0, name, " must be float16, bfloat16 or float32, not ", t.scalar_type());
   TORCH_CHECK_VALUE(dims < 0 || t.dim() == dims, name, " must have ", dims, " dimensions, not ", t.dim());
+  check_no_tangent(t, name);
   return code;
 }
 
 void check_like(const Tensor& t, const char* name, at::IntArrayRef shape, at::Device device) {
   TORCH_CHECK_VALUE(t.sizes() == shape, name, " must be a tensor of shape ", shape, ", not ", t.sizes());
   TORCH_CHECK_VALUE(t.device() == device, name, " must be on ", device);
+  check_no_tangent(t, name);
 }
 
 void check(int rc, const char* what) {
@@ -74,7 +82,10 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
 }
 
 // A gradient as the kernels read it: of the output's type, contiguous.
-Tensor incoming(const Tensor& grad, at::ScalarType type) { return grad.to(type).contiguous(); }
+Tensor incoming(const Tensor& grad, at::ScalarType type) {
+  check_no_tangent(grad, "an incoming gradient");
+  return grad.to(type).contiguous();
+}
 
 // In a node below, needs_input_grad counts the tensors that it was given (an optional that holds none is not counted).
 

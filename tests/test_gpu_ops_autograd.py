@@ -1,9 +1,10 @@
 """What the block operators' autograd nodes do beside a first gradient on the GPU: second derivatives of every kind of
-loss, and where a gradient is a constant."""
+loss, where a gradient is a constant, and forward mode."""
 from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 import ops_plain as plain
 import persistent_lstm_hip_amd as P
@@ -112,3 +113,60 @@ def test_a_state_may_be_overwritten_before_the_backward_pass(gpu):
     _, c_n = P.gated_scan(z, c0)
     c0.copy_(c_n.detach())
     assert torch.equal(torch.autograd.grad(c_n, z, d)[0], want)
+
+
+# ---- forward mode ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", range(10))
+def test_forward_mode_tangents_are_refused(gpu, which, grad):
+    """A dual tensor has no requires_grad of its own; its tangent would be dropped."""
+    _say(f"tangent {which} grad={grad}")
+    x, w, c = _x(3, 8), _x(8, seed=1), _x(3, 4, seed=2)
+    z = x.view(3, 1, 8)
+    name, t, call = [
+        ("x", x, lambda t: P.layer_norm(t, w, w)), ("weight", w, lambda t: P.layer_norm(x, t, w)),
+        ("bias", w, lambda t: P.layer_norm(x, w, t)),
+        ("x", x, lambda t: P.dropout_add(t, x, p=0.1, seed=1)), ("residual", x, lambda t: P.dropout_add(x, t, p=0.1, seed=1)),
+        ("gates", z, lambda t: P.gated_scan(t, c, output_gate=False)),
+        ("c0", c, lambda t: P.gated_scan(z, t, output_gate=False)),
+        ("gates", x, lambda t: P.gated_scan_step(t, c, output_gate=False)),
+        ("c", c, lambda t: P.gated_scan_step(x, t, output_gate=False)),
+        ("c", c, lambda t: P.gated_scan_step(x, t, output_gate=False, inplace=True)),
+    ][which]
+    before = c.clone()
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        with pytest.raises(ValueError, match=f"^{name} carries a forward-mode tangent"):
+            call(fw.make_dual(t, torch.ones_like(t)))
+        call(t)  # (as it is without one)
+    if which < 9:
+        assert torch.equal(c, before)
+
+
+def test_a_tangent_of_an_incoming_gradient_is_refused(gpu):
+    _say("tangent of a gradient")
+    x = _x(3, 8).requires_grad_(True)
+    for f in (P.layer_norm, lambda t: P.dropout_add(t, p=0.1, seed=1),
+              lambda t: P.gated_scan(t.view(1, 3, 8), output_gate=False)[0],
+              lambda t: P.gated_scan(t.view(1, 3, 8), output_gate=False)[1]):
+        with fw.dual_level():
+            y = f(x)
+            with pytest.raises(ValueError, match="incoming gradient carries a forward-mode tangent"):
+                torch.autograd.grad(y, x, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("transform", ["grad", "jvp", "vmap"])
+def test_function_transforms_raise(gpu, transform):
+    """torch.func's wrappers hold no storage: an error, never a value without its derivative."""
+    _say(f"torch.func.{transform}")
+    x = _x(3, 8)
+    for f in (P.layer_norm, lambda t: P.dropout_add(t, p=0.1, seed=1),
+              lambda t: P.gated_scan(t.view(1, 3, 8), output_gate=False)[0]):
+        with pytest.raises((RuntimeError, ValueError)):
+            if transform == "grad":
+                torch.func.grad(lambda t: f(t).sum())(x)
+            elif transform == "jvp":
+                torch.func.jvp(f, (x,), (torch.ones_like(x),))
+            else:
+                torch.func.vmap(f)(x.expand(2, 3, 8))
