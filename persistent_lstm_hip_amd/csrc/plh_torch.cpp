@@ -5,6 +5,7 @@
 // function a layer norm of one row took 11 us, and a training step of a small one, whose kernels run for 25 us, 125 us.
 // No kernel is in this file, and the library itself does not depend on torch.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -242,6 +243,9 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& gates_in, const Tensor&
   TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(tracks(gates_in) || tracks(c_in)),
                     "gated_scan_step is not differentiable: call it under torch.no_grad(), or gated_scan");
   const c10::DeviceGuard guard(device);
+  // (before the kernel runs: torch would raise for the version only after it)
+  TORCH_CHECK_VALUE(!inplace || !c_in.is_inference() || c10::InferenceMode::is_enabled(),
+                    "c is an inference tensor: it can be updated in place in inference mode only");
   const Tensor c = c_in.contiguous(), gates = dense_rows(gates_in);
   Tensor out = empty({B, H}, gates.scalar_type(), device), c_n = inplace ? c_in : empty({B, H}, at::kFloat, device);
   check(plh_gated_scan_forward(code, output_gate, ptr(gates), gates.stride(0), 0, B, 1, (int)H, nullptr, ptr<float>(c),
