@@ -82,10 +82,15 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
 
+// t with its values in its storage (torch may hold a real tensor as the storage's negative, as the imaginary part of a
+// conjugate) and contiguous.
+Tensor values(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return values(t).contiguous(); }
+
 // A gradient as the kernels read it: of the output's type, contiguous.
 Tensor incoming(const Tensor& grad, at::ScalarType type) {
   check_no_tangent(grad, "an incoming gradient");
-  return grad.to(type).contiguous();
+  return dense(grad.to(type));
 }
 
 // In a node below, needs_input_grad counts the tensors that it was given (an optional that holds none is not counted).
@@ -127,7 +132,7 @@ int64_t hidden_of(const Tensor& gates, bool output_gate) {
 
 // gates itself where its last dimension is dense (any other strides), else a copy.
 Tensor dense_rows(const Tensor& gates) {
-  return gates.stride(-1) == 1 || gates.size(-1) == 1 ? gates : gates.contiguous();
+  return gates.stride(-1) == 1 || gates.size(-1) == 1 ? values(gates) : gates.contiguous();
 }
 
 // int32 on the device.  Host lengths are checked; lengths on the device are not (that would synchronise the stream):
@@ -222,7 +227,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& gates_in, const MaybeTensor&
   if (c0_in.has_value()) {
     check_tensor(*c0_in, "c0");
     check_like(*c0_in, "c0", {B, H}, device);
-    c0 = c0_in->to(at::kFloat).contiguous();
+    c0 = dense(c0_in->to(at::kFloat));
   }
   const Tensor n = device_lengths(lengths, B, T, device), gates = dense_rows(gates_in);
   if (at::GradMode::is_enabled() && (tracks(gates) || tracks(given(c0)))) {
@@ -239,14 +244,15 @@ std::tuple<Tensor, Tensor> gated_scan_step(const Tensor& gates_in, const Tensor&
   const at::Device device = gates_in.device();
   check_like(c_in, "c", {B, H}, device);
   TORCH_CHECK_VALUE(c_in.scalar_type() == at::kFloat, "c must be float32, not ", c_in.scalar_type());
-  TORCH_CHECK_VALUE(!inplace || c_in.is_contiguous(), "c must be contiguous to be updated in place");
+  TORCH_CHECK_VALUE(!inplace || (c_in.is_contiguous() && !c_in.is_neg()),
+                    "c must be contiguous (and no lazily negated view) to be updated in place");
   TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(tracks(gates_in) || tracks(c_in)),
                     "gated_scan_step is not differentiable: call it under torch.no_grad(), or gated_scan");
   const c10::DeviceGuard guard(device);
   // (before the kernel runs: torch would raise for the version only after it)
   TORCH_CHECK_VALUE(!inplace || !c_in.is_inference() || c10::InferenceMode::is_enabled(),
                     "c is an inference tensor: it can be updated in place in inference mode only");
-  const Tensor c = c_in.contiguous(), gates = dense_rows(gates_in);
+  const Tensor c = dense(c_in), gates = dense_rows(gates_in);
   Tensor out = empty({B, H}, gates.scalar_type(), device), c_n = inplace ? c_in : empty({B, H}, at::kFloat, device);
   check(plh_gated_scan_forward(code, output_gate, ptr(gates), gates.stride(0), 0, B, 1, (int)H, nullptr, ptr<float>(c),
                                ptr(out), ptr<float>(c_n), nullptr, nullptr, 0, stream_of(gates)),
@@ -319,15 +325,16 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 };
 
-Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
-  check_tensor(x, "x");
+Tensor layer_norm(const Tensor& x_in, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+  check_tensor(x_in, "x");
+  const Tensor x = values(x_in);
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x needs a last dimension of at least one element");
   const auto param = [&](const MaybeTensor& t, const char* name) -> MaybeTensor {
     if (!t.has_value()) return t;
     check_like(*t, name, {x.size(-1)}, x.device());
     TORCH_CHECK_VALUE(t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat, name, " must be ",
                       x.scalar_type(), " or float32, not ", t->scalar_type());
-    return t->contiguous();
+    return dense(*t);
   };
   const MaybeTensor w = param(weight, "weight"), b = param(bias, "bias");
   TORCH_CHECK_VALUE(!w.has_value() || !b.has_value() || w->scalar_type() == b->scalar_type(),
@@ -393,9 +400,9 @@ Tensor dropout_add(const Tensor& x_in, const MaybeTensor& residual_in, double p,
                     "a tensor offset must be one int64 on ", device);
   const c10::DeviceGuard guard(device);
   const Mask m{(int)std::floor(p * 65536.0 + 0.5), seed, offset};
-  const Tensor x = x_in.contiguous();
+  const Tensor x = dense(x_in);
   MaybeTensor residual;
-  if (residual_in.has_value()) residual = residual_in->contiguous();
+  if (residual_in.has_value()) residual = dense(*residual_in);
   if (at::GradMode::is_enabled() && (tracks(x) || tracks(given(residual))))
     return DropoutAdd::apply(x, residual, (int64_t)m.threshold, (int64_t)seed, (int64_t)offset, offset_dev);
   return dropout(x, given(residual), m, given(offset_dev));
