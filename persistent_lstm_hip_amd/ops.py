@@ -15,6 +15,7 @@ reference has no counterpart.
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -27,6 +28,14 @@ _U64 = (1 << 64) - 1
 def _tensor(t, name: str) -> None:
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
+
+
+def _u64(v, name: str) -> int:
+    """An integer of any type modulo 2^64 (numpy's do not take the mask as one of theirs)."""
+    try:
+        return operator.index(v) & _U64
+    except TypeError:
+        raise ValueError(f"{name} must be an integer, not {type(v).__name__}") from None
 
 
 def gated_scan(gates: torch.Tensor, c0: Optional[torch.Tensor] = None, *,
@@ -90,5 +99,5 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, *, p: 
     if residual is not None:
         _tensor(residual, "residual")
     if isinstance(offset, torch.Tensor):
-        return require_torch_ops().dropout_add(x, residual, p, seed & _U64, 0, offset)
-    return require_torch_ops().dropout_add(x, residual, p, seed & _U64, offset & _U64, None)
+        return require_torch_ops().dropout_add(x, residual, p, _u64(seed, "seed"), 0, offset)
+    return require_torch_ops().dropout_add(x, residual, p, _u64(seed, "seed"), _u64(offset, "offset"), None)
