@@ -510,17 +510,31 @@ int64_t groups_for(int64_t rows, int threads, int side, int nv) {
 }
 constexpr int kWideGroups = 64;  // runs of rows of norm_columns_kernel
 
+// How a call with pieces of `v` columns (16 bytes) is laid out.
+struct NormLayout {
+  int vec;      // columns of a piece: v, or one where a row is shorter than that
+  Shape shape;  // {0, 0}: a workgroup per row
+  int groups;   // rows of partial sums of the backward pass, one at least
+};
+NormLayout norm_layout(int v, int64_t rows, int64_t cols) {
+  NormLayout l;
+  l.vec = cols >= v ? v : 1;
+  l.shape = shape_for((cols + l.vec - 1) / l.vec, l.vec);
+  const int threads = std::max(l.shape.lpr, 256);
+  l.groups = l.shape.lpr ? (int)groups_for(rows, threads, threads / l.shape.lpr, l.shape.nv)
+                         : (int)std::max<int64_t>(1, std::min<int64_t>(rows, kWideGroups));
+  return l;
+}
+
 template <typename T, bool BACKWARD>
 hipError_t launch_norm(NormArgs p, hipStream_t s) {
   constexpr int V = kNormVec<T>;
-  const int vec = p.cols >= V ? V : 1;
-  const Shape sh = shape_for((p.cols + vec - 1) / vec, vec);
+  const NormLayout l = norm_layout(V, p.rows, p.cols);
+  p.groups = l.groups;
   if (BACKWARD && !p.d_weight && !p.d_bias) p.part = nullptr;
   hipError_t e = hipSuccess;
-  if (sh.lpr) {
-    const int threads = std::max(sh.lpr, 256);
-    p.groups = (int)groups_for(p.rows, threads, threads / sh.lpr, sh.nv);
-    e = vec == V ? launch_vec<T, BACKWARD, V>(p, sh, s) : launch_vec<T, BACKWARD, 1>(p, sh, s);
+  if (l.shape.lpr) {
+    e = l.vec == V ? launch_vec<T, BACKWARD, V>(p, l.shape, s) : launch_vec<T, BACKWARD, 1>(p, l.shape, s);
   } else {
     const unsigned grid = (unsigned)std::min<int64_t>(p.rows, 1024);
     if constexpr (!BACKWARD) {
@@ -532,7 +546,6 @@ hipError_t launch_norm(NormArgs p, hipStream_t s) {
         e = hipGetLastError();
       }
       if (e == hipSuccess && p.part) {
-        p.groups = (int)std::min<int64_t>(p.rows, kWideGroups);
         hipLaunchKernelGGL((norm_columns_kernel<T, V>), dim3((p.cols + 256 * V - 1) / (256 * V), p.groups), dim3(256), 0,
                            s, p);
         e = hipGetLastError();
@@ -565,7 +578,10 @@ extern "C" {
 
 int64_t plh_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 1 || cols > (1 << 24)) return -1;
-  return std::max<int64_t>(plh::groups_for(rows, 256, 1, 1), plh::kWideGroups) * 2 * cols * (int64_t)sizeof(float);
+  int groups = 0;  // the most of any type
+  for (int v : {plh::kNormVec<_Float16>, plh::kNormVec<float>})
+    groups = std::max(groups, plh::norm_layout(v, rows, cols).groups);
+  return groups * 2 * cols * (int64_t)sizeof(float);
 }
 
 int plh_layer_norm_forward(int dtype, int wdtype, const void* x, int64_t stride, int64_t rows, int64_t cols,
