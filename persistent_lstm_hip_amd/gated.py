@@ -38,7 +38,8 @@ class GatedScanBlock(nn.Module):
         gates = self.gates(layer_norm(x, self.norm_weight, self.norm_bias))
         h, c_n = gated_scan(gates, c0, lengths=lengths)
         p = self.dropout if self.training else 0.0
-        return dropout_add(self.out(h), x, p=p, seed=seed, offset=offset), c_n
+        # (under autocast a product is of the lower type; the residual stream keeps its own)
+        return dropout_add(self.out(h).to(x.dtype), x, p=p, seed=seed, offset=offset), c_n
 
     def step(self, x: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
         """One token x [batch, dim] -> y; c is updated in place.  For inference."""
