@@ -11,12 +11,17 @@ instead of a chain of matrix products.  The matrix products themselves are torch
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import torch
 import torch.nn as nn
 
 from .ops import dropout_add, gated_scan, gated_scan_step, layer_norm
+
+
+def _draw() -> int:
+    """62 bits of torch's host generator, which activation checkpointing restores for its recomputation."""
+    return int(torch.randint(1 << 62, (), device="cpu"))
 
 
 class GatedScanBlock(nn.Module):
@@ -33,11 +38,14 @@ class GatedScanBlock(nn.Module):
             self.gates.bias[:dim] = torch.linspace(0.5, 6.0, dim)
 
     def forward(self, x: torch.Tensor, c0: Optional[torch.Tensor] = None, *, lengths=None, seed: int = 0,
-                offset: int = 0):
-        """x [batch, time, dim] -> (y, c_n).  (seed, offset) pick the dropout mask in training mode."""
+                offset: Union[int, torch.Tensor, None] = None):
+        """x [batch, time, dim] -> (y, c_n).  (seed, offset) pick the dropout mask in training mode, as in dropout_add.
+        Without an offset one is drawn from torch's generator, so that every call has a mask of its own."""
         gates = self.gates(layer_norm(x, self.norm_weight, self.norm_bias))
         h, c_n = gated_scan(gates, c0, lengths=lengths)
         p = self.dropout if self.training else 0.0
+        if offset is None:
+            offset = _draw() if p > 0.0 else 0
         # (under autocast a product is of the lower type; the residual stream keeps its own)
         return dropout_add(self.out(h).to(x.dtype), x, p=p, seed=seed, offset=offset), c_n
 
