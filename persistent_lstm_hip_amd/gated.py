@@ -60,8 +60,12 @@ class GatedScanRegressor(nn.Module):
     """x [batch, time, input_dim] -> [batch, output_dim], read off at every row's last step.
 
     In training mode every layer of every pass draws a dropout mask of its own under `seed` (torch.initial_seed() unless
-    set).  The passes are counted from the model's construction on and are not in its state_dict: a resumed run, or a
-    second model of a process, sets another seed."""
+    set).  The passes are counted from the model's construction on and are not in its state_dict: a resumed run, a
+    second model of a process, or the ranks of a data-parallel job that share a manual seed set other seeds.  A pass
+    that finds torch's host generator where an earlier one found it is that pass once more, with its masks: activation
+    checkpointing, which restores the generator, recomputes what it computed."""
+
+    _REMEMBERED = 4096  # passes that a recomputation may go back
 
     def __init__(self, input_dim: int, hidden_dim: int, output_dim: int, n_layers: int, dropout: float = 0.2):
         super().__init__()
@@ -72,6 +76,16 @@ class GatedScanRegressor(nn.Module):
         self.linear = nn.Linear(hidden_dim, output_dim)
         self.seed = int(torch.initial_seed())
         self._passes = 0  # training passes so far: every layer of every pass has a mask of its own
+        self._numbers = {}  # of the last passes, by what they drew from torch's generator
+
+    def _pass_number(self) -> int:
+        drawn = _draw()
+        if drawn not in self._numbers:
+            if len(self._numbers) == self._REMEMBERED:
+                del self._numbers[next(iter(self._numbers))]  # (the oldest)
+            self._numbers[drawn] = self._passes
+            self._passes += 1
+        return self._numbers[drawn]
 
     def _head(self, x: torch.Tensor) -> torch.Tensor:
         return self.linear(layer_norm(x, self.norm_weight, self.norm_bias))
@@ -81,9 +95,8 @@ class GatedScanRegressor(nn.Module):
             raise ValueError("x must be a [batch, seq_len, input_size] tensor of at least one step")
         if lengths is not None:
             lengths = torch.as_tensor(lengths)
-        offset = self._passes * len(self.blocks)
-        if self.training:
-            self._passes += 1
+        drops = self.training and any(block.dropout > 0.0 for block in self.blocks)
+        offset = self._pass_number() * len(self.blocks) if drops else 0
         y = self.stem(x)
         for i, block in enumerate(self.blocks):
             y, _ = block(y, lengths=lengths, seed=self.seed, offset=offset + i)

@@ -1,4 +1,4 @@
-"""Which dropout masks the block draws: their offsets, with the operators' formulas in torch on the CPU."""
+"""Which dropout masks the block and the forecaster draw: their offsets, with the operators' formulas in torch on the CPU."""
 from __future__ import annotations
 
 import pytest
@@ -6,7 +6,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import ops_plain as plain
-from persistent_lstm_hip_amd import GatedScanBlock, gated
+from persistent_lstm_hip_amd import GatedScanBlock, GatedScanRegressor, gated
 
 
 def _scan(gates, c0=None, *, lengths=None):
@@ -86,3 +86,55 @@ def test_a_checkpointed_block_recomputes_its_own_mask(masks, reentrant):
     assert masks[2] == first != masks[1]
     want = torch.autograd.grad(block(x, offset=first[1])[0].square().sum(), x)
     assert torch.allclose(got[0], want[0])
+
+
+def _model(p=0.5, layers=2):
+    torch.manual_seed(1)
+    return GatedScanRegressor(3, 8, 2, layers, p)
+
+
+def test_the_forecasters_passes_are_numbered(masks):
+    m, x = _model(), torch.randn(2, 6, 3)
+    m(x), m(x)
+    assert masks == [(m.seed, i) for i in range(4)]
+    m.eval()
+    m(x)
+    assert len(masks) == 4
+    m.train()
+    m(x)
+    assert masks[4:] == [(m.seed, 4), (m.seed, 5)]
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_forecaster_recomputes_its_own_masks(masks, reentrant):
+    """Two passes are outstanding when the first is recomputed; their gradients are those without checkpointing."""
+    m = _model()
+    xs = [torch.randn(2, 6, 3, requires_grad=True) for _ in range(2)]
+    ys = [checkpoint(m, x, use_reentrant=reentrant) for x in xs]
+    for p in m.parameters():
+        p.grad = None
+    sum(y.square().sum() for y in ys).backward()
+    assert sorted(masks[:4]) == sorted(masks[4:]) == [(m.seed, i) for i in range(4)]
+    got = [p.grad.clone() for p in m.parameters()]
+    fresh = _model()
+    sum(fresh(x).square().sum() for x in xs).backward()
+    for a, b in zip(got, fresh.parameters()):
+        assert torch.allclose(a, b.grad, atol=1e-6)
+    del masks[:]
+    m(xs[0])
+    assert masks == [(m.seed, 4), (m.seed, 5)]  # (the recomputations are no passes of their own)
+
+
+def test_a_forecaster_without_dropout_leaves_torchs_generator_alone(masks):
+    m, x = _model(0.0), torch.randn(2, 6, 3)
+    state = torch.get_rng_state()
+    m(x)
+    assert torch.equal(torch.get_rng_state(), state) and masks == []
+
+
+def test_what_a_forecaster_remembers_is_bounded(masks, monkeypatch):
+    monkeypatch.setattr(GatedScanRegressor, "_REMEMBERED", 3)
+    m, x = _model(layers=1), torch.randn(2, 2, 3)
+    for _ in range(7):
+        m(x)
+    assert len(m._numbers) == 3 and masks == [(m.seed, i) for i in range(7)]
