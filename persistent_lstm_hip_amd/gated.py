@@ -11,7 +11,7 @@ instead of a chain of matrix products.  The matrix products themselves are torch
 """
 from __future__ import annotations
 
-from typing import List, Optional, Union
+from typing import List, Optional, Sequence, Union
 
 import torch
 import torch.nn as nn
@@ -19,8 +19,11 @@ import torch.nn as nn
 from .ops import dropout_add, gated_scan, gated_scan_step, layer_norm
 
 
-def _draw() -> int:
-    """62 bits of torch's host generator, which activation checkpointing restores for its recomputation."""
+def _draw(device: torch.device) -> Union[int, torch.Tensor]:
+    """62 bits of torch's host generator, which activation checkpointing restores for its recomputation.  While a graph is
+    captured, which would keep them for all its replays, of the device's, in a tensor that every replay draws again."""
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        return torch.randint(1 << 62, (1,), device=device)
     return int(torch.randint(1 << 62, (), device="cpu"))
 
 
@@ -40,12 +43,13 @@ class GatedScanBlock(nn.Module):
     def forward(self, x: torch.Tensor, c0: Optional[torch.Tensor] = None, *, lengths=None, seed: int = 0,
                 offset: Union[int, torch.Tensor, None] = None):
         """x [batch, time, dim] -> (y, c_n).  (seed, offset) pick the dropout mask in training mode, as in dropout_add.
-        Without an offset one is drawn from torch's generator, so that every call has a mask of its own."""
+        Without an offset one is drawn from torch's generator, so that every call (and every replay of a captured
+        one) has a mask of its own."""
         gates = self.gates(layer_norm(x, self.norm_weight, self.norm_bias))
         h, c_n = gated_scan(gates, c0, lengths=lengths)
         p = self.dropout if self.training else 0.0
         if offset is None:
-            offset = _draw() if p > 0.0 else 0
+            offset = _draw(x.device) if p > 0.0 else 0
         # (under autocast a product is of the lower type; the residual stream keeps its own)
         return dropout_add(self.out(h).to(x.dtype), x, p=p, seed=seed, offset=offset), c_n
 
@@ -63,7 +67,9 @@ class GatedScanRegressor(nn.Module):
     set).  The passes are counted from the model's construction on and are not in its state_dict: a resumed run, a
     second model of a process, or the ranks of a data-parallel job that share a manual seed set other seeds.  A pass
     that finds torch's host generator where an earlier one found it is that pass once more, with its masks: activation
-    checkpointing, which restores the generator, recomputes what it computed."""
+    checkpointing, which restores the generator, recomputes what it computed.  forward's `offset` gives the pass its
+    number in the place of the count: an int, or a one-element int64 tensor on the device, which a captured graph may
+    advance.  A captured pass without one draws its number on the device in every replay."""
 
     _REMEMBERED = 4096  # passes that a recomputation may go back
 
@@ -78,8 +84,10 @@ class GatedScanRegressor(nn.Module):
         self._passes = 0  # training passes so far: every layer of every pass has a mask of its own
         self._numbers = {}  # of the last passes, by what they drew from torch's generator
 
-    def _pass_number(self) -> int:
-        drawn = _draw()
+    def _pass_number(self, device: torch.device) -> Union[int, torch.Tensor]:
+        drawn = _draw(device)
+        if isinstance(drawn, torch.Tensor):
+            return drawn
         if drawn not in self._numbers:
             if len(self._numbers) == self._REMEMBERED:
                 del self._numbers[next(iter(self._numbers))]  # (the oldest)
@@ -90,16 +98,28 @@ class GatedScanRegressor(nn.Module):
     def _head(self, x: torch.Tensor) -> torch.Tensor:
         return self.linear(layer_norm(x, self.norm_weight, self.norm_bias))
 
-    def forward(self, x: torch.Tensor, lengths=None) -> torch.Tensor:
+    def _offsets(self, offset, device) -> Sequence[Union[int, torch.Tensor]]:
+        """The layers' offsets in dropout_add of pass number `offset`."""
+        n = len(self.blocks)
+        if not isinstance(offset, torch.Tensor):
+            return range(offset * n, (offset + 1) * n)
+        if offset.numel() != 1 or offset.dtype != torch.int64 or offset.device != device:
+            raise ValueError(f"a tensor offset must be one int64 on {device}")
+        return (offset.reshape(1, 1) * n + torch.arange(n, device=device).unsqueeze(1)).unbind()
+
+    def forward(self, x: torch.Tensor, lengths=None, offset: Union[int, torch.Tensor, None] = None) -> torch.Tensor:
         if x.dim() != 3 or x.size(1) == 0:
             raise ValueError("x must be a [batch, seq_len, input_size] tensor of at least one step")
         if lengths is not None:
             lengths = torch.as_tensor(lengths)
         drops = self.training and any(block.dropout > 0.0 for block in self.blocks)
-        offset = self._pass_number() * len(self.blocks) if drops else 0
+        if not drops:
+            offset = 0
+        elif offset is None:
+            offset = self._pass_number(x.device)
         y = self.stem(x)
-        for i, block in enumerate(self.blocks):
-            y, _ = block(y, lengths=lengths, seed=self.seed, offset=offset + i)
+        for block, mask in zip(self.blocks, self._offsets(offset, x.device)):
+            y, _ = block(y, lengths=lengths, seed=self.seed, offset=mask)
         if lengths is None:
             return self._head(y[:, -1])
         last = (lengths.to(y.device, torch.int64) - 1).clamp(0, y.size(1) - 1)  # (an empty row: its first step)

@@ -138,3 +138,23 @@ def test_what_a_forecaster_remembers_is_bounded(masks, monkeypatch):
     for _ in range(7):
         m(x)
     assert len(m._numbers) == 3 and masks == [(m.seed, i) for i in range(7)]
+
+
+@pytest.mark.parametrize("kind", [int, lambda v: torch.tensor([v]), torch.tensor])
+def test_a_forecaster_takes_the_pass_number_that_it_is_given(masks, kind):
+    m, x = _model(), torch.randn(2, 6, 3)
+    state = torch.get_rng_state()
+    a = m(x, None, kind(7))
+    assert masks == [(m.seed, 14), (m.seed, 15)]
+    assert torch.equal(torch.get_rng_state(), state) and m._passes == 0
+    assert torch.equal(m(x, offset=7), a)
+    y = checkpoint(m, x.requires_grad_(True), None, kind(7), use_reentrant=False)
+    y.sum().backward()
+    assert masks[4:] == [(m.seed, 14), (m.seed, 15)] * 2
+
+
+def test_pass_numbers_that_are_refused(masks):
+    m, x = _model(), torch.randn(2, 6, 3)
+    for bad in (torch.tensor([1, 2]), torch.tensor([1.0]), torch.tensor([1], dtype=torch.int32)):
+        with pytest.raises(ValueError, match="one int64"):
+            m(x, offset=bad)
