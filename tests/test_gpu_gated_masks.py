@@ -108,3 +108,36 @@ def test_replays_draw_masks_by_themselves(gpu, kind, monkeypatch):
             for a, b in zip(got, step(offset=given)):
                 assert torch.allclose(a, b, rtol=1e-5, atol=1e-5), f"replay {i}"
     assert len(numbers) == 4 and len(drawn) == 1
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_pass_in_a_captured_step(gpu, reentrant, monkeypatch):
+    """The recomputation draws the pass' own number in every replay."""
+    _say(f"captured checkpoint reentrant={reentrant}")
+    m, x = _model(), torch.randn(4, 70, 2, device="cuda", requires_grad=True)
+    drawn, draw = [], gated._draw
+    monkeypatch.setattr(gated, "_draw", lambda device: drawn.append(draw(device)) or drawn[-1])
+
+    def step():
+        y = checkpoint(m, x, use_reentrant=reentrant)
+        y.sum().backward()
+        return y
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    del drawn[:]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    seen = set()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        first, again = (int(v) for v in drawn)
+        assert first == again
+        seen.add(first)
+        m(x, offset=0)
+    assert len(seen) == 3
