@@ -161,6 +161,16 @@ Layout layout_for(int elem_bytes, int64_t batch, int64_t seq_len, int64_t hidden
   return l;
 }
 
+// A factor of a map that is composed of several steps.  Every step's own is positive (at least 2^-126, see logistic()), so
+// that an infinite state stays infinite; their product may underflow, and 0 * inf would be NaN.  Held at 2^-126 it moves
+// a finite state by less than 2^-126 of what it was.  (A NaN factor is dropped here: the map's sum holds it as well.)
+__device__ __forceinline__ float factor(float a) { return __builtin_fmaxf(a, 0x1p-126f); }
+template <int VEC>
+__device__ __forceinline__ void hold_factors(float (&A)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) A[j] = factor(A[j]);
+}
+
 // v of the even and of the odd time group of a pair of groups, in both (one exchange per level and value).
 template <int LEVEL>
 __device__ __forceinline__ void pair_of(float v, float& even, float& odd) {
@@ -203,11 +213,11 @@ __device__ __forceinline__ void wave_maps(int lane, float (&A)[VEC], float (&B)[
         const float fa = rev ? a1 : a0, fb = rev ? b1 : b0, sa = rev ? a0 : a1, sb = rev ? b0 : b1;
         if (odd != rev) {
           pb[k][j] = fmaf(pa[k][j], fb, pb[k][j]);
-          pa[k][j] *= fa;
+          pa[k][j] = factor(pa[k][j] * fa);
         }
         B[k][j] = fmaf(sa, fb, sb);
       }
-      A[j] = a0 * a1;
+      A[j] = factor(a0 * a1);
     }
   };
   if constexpr (P::CT == 16) level(std::integral_constant<int, 0>());
@@ -348,6 +358,7 @@ __device__ __forceinline__ void fold_segments(const ScanArgs<T>& p, const P& at,
         A[j] *= a.v[j];
       }
     }
+    hold_factors(A);
   }
   wave_maps<P, 1, false>(at.lane, A, B, pa, pb);
   if (at.lane < P::CT) {
@@ -493,6 +504,7 @@ __global__ void __launch_bounds__(P::THREADS) scan_maps_kernel(ScanArgs<T> p) {
     for (; t + 4 <= steps; t += 4) rows(t, Many());
     for (; t < steps; ++t) rows(t, One());
   }
+  hold_factors(A);
   wave_maps<P, 1, REVERSE>(at.lane, A, B, pa, pb);
   put_maps<P, 1>(at, lds, A, B);
   lds_barrier();
@@ -506,6 +518,7 @@ __global__ void __launch_bounds__(P::THREADS) scan_maps_kernel(ScanArgs<T> p) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) prod[j] *= a.v[j];
   }
+  hold_factors(prod);
   fold_waves<P, 1, 0, REVERSE>(at, lds, pa[0], pb[0], sum, none);
   store_carry(p.seg_a + (int64_t)seg * p.channels, at, prod);
   store_carry(p.seg_b + (int64_t)seg * p.channels, at, sum);
@@ -543,6 +556,7 @@ __global__ void __launch_bounds__(P::THREADS, sizeof(T) == 2 ? 4 : 1) scan_forwa
         A[j] *= a[r][j];
       }
     }
+    hold_factors(A);
     wave_maps<P, 1, false>(at.lane, A, B, pa, pb);
     float c[VEC];
     relay_pass(at, relay, ++round, A, B[0], pa[0], pb[0], carry, c);
@@ -631,6 +645,7 @@ __global__ void __launch_bounds__(P::THREADS) scan_backward_kernel(ScanArgs<T> p
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) B[0][j] = fmaf(a[r][j], B[0][j], na[r][j] * (float)x.g[r].v[j]);
+    hold_factors(A);
     wave_maps<P, 2, false>(at.lane, A, B, pa, pb);
     auto& maps = lds[tile & 1];
     put_maps<P, 2>(at, maps, A, B);
