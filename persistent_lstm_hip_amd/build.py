@@ -57,7 +57,9 @@ def host_compiler() -> str:
 
 
 def build(verbose: bool = False) -> str:
-    """Compile every source for gfx950 and link the shared library.  Always recompiles."""
+    """Compile every source for gfx950 and link the shared library, its native driver and the torch front end.  Always
+    recompiles.  The front end comes last: without a C++ compiler or Python's headers for it this raises, with the
+    library and its driver built."""
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
 
@@ -67,7 +69,7 @@ def build(verbose: bool = False) -> str:
         proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         out = "\n".join(l for l in proc.stdout.splitlines() if "packed-fp32-ops" not in l)
         if proc.returncode != 0:
-            raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{out}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({proc.returncode}):\n{out}")
         if verbose and out.strip():
             print(out, flush=True)
 
@@ -76,39 +78,34 @@ def build(verbose: bool = False) -> str:
         run([hipcc()] + HIPCC_FLAGS + ["-c", os.path.join(CSRC, source), "-o", obj])
         return obj
 
-    import torch
+    def compile_front(obj: str) -> list:
+        """Compiles the torch front end; the command that links it."""
+        import torch
 
-    torch_dir = os.path.dirname(torch.__file__)
-    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+        torch_dir = os.path.dirname(torch.__file__)
+        rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+        include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                   os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
+        run([host_compiler(), "-std=c++17", "-O2", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-DTORCH_EXTENSION_NAME=plh_torch"] + [a for d in include for a in ("-isystem", d)] +
+            ["-c", os.path.join(CSRC, "plh_torch.cpp"), "-o", obj])
+        return [host_compiler(), "-shared", obj, "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu",
+                "-ltorch", "-ltorch_python", "-L" + LIB_DIR, "-lpersistent_lstm_hip", "-Wl,-rpath,$ORIGIN"]
+
     with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(4) as pool:
-        front_obj = os.path.join(objects, "plh_torch.o")
-        front = pool.submit(run, [host_compiler(), "-std=c++17", "-O2", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1",
-                                  "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=plh_torch"] +
-                            [a for d in (os.path.join(torch_dir, "include"),
-                                         os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
-                                         os.path.join(rocm, "include"), sysconfig.get_paths()["include"])
-                             for a in ("-isystem", d)] +
-                            ["-c", os.path.join(CSRC, "plh_torch.cpp"), "-o", front_obj])
+        front = pool.submit(compile_front, os.path.join(objects, "plh_torch.o"))
         objs = list(pool.map(lambda s: compile_one(s, objects), SOURCES))
         run([hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}"] + objs + LINK_FLAGS + ["-o", tmp])
         os.replace(tmp, LIB_PATH)
-        front.result()
-        run([host_compiler(), "-shared", front_obj, "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_hip",
-             "-ltorch_cpu", "-ltorch", "-ltorch_python", "-L" + LIB_DIR, "-lpersistent_lstm_hip", "-Wl,-rpath,$ORIGIN",
-             "-o", TORCH_PATH + ".tmp"])
-    os.replace(TORCH_PATH + ".tmp", TORCH_PATH)
-    # Native driver of the C ABI (profiling target and integration example), linked to the library.
-    # (plh_issue_probe.hip: a developer probe kernel of plh_bench --issue, not part of the library.)
-    cmd = [hipcc(), "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
-           "-packed-fp32-ops", "-Wno-unused-command-line-argument", os.path.join(CSRC, "plh_bench_main.cpp"),
-           os.path.join(CSRC, "plh_issue_probe.hip"), "-L" + LIB_DIR, "-lpersistent_lstm_hip", "-Wl,-rpath,$ORIGIN",
-           "-o", BENCH_PATH + ".tmp"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc (plh_bench) failed ({proc.returncode}):\n{proc.stdout}")
-    os.replace(BENCH_PATH + ".tmp", BENCH_PATH)
+        # Native driver of the C ABI (profiling target and integration example), linked to the library.
+        # (plh_issue_probe.hip: a developer probe kernel of plh_bench --issue, not part of the library.)
+        run([hipcc(), "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
+             "-packed-fp32-ops", "-Wno-unused-command-line-argument", os.path.join(CSRC, "plh_bench_main.cpp"),
+             os.path.join(CSRC, "plh_issue_probe.hip"), "-L" + LIB_DIR, "-lpersistent_lstm_hip", "-Wl,-rpath,$ORIGIN",
+             "-o", BENCH_PATH + ".tmp"])
+        os.replace(BENCH_PATH + ".tmp", BENCH_PATH)
+        run(front.result() + ["-o", TORCH_PATH + ".tmp"])
+        os.replace(TORCH_PATH + ".tmp", TORCH_PATH)
     return LIB_PATH
 
 
