@@ -280,7 +280,8 @@ int plh_layer_norm_forward(int dtype, int wdtype, const void* x, int64_t stride,
                            void* stream);
 /*
  * Its gradient: d_x [rows][cols] (contiguous), d_weight and d_bias [cols] of wdtype, each of the three or NULL.
- * d_y [rows][cols] contiguous.  workspace as above, of plh_layer_norm_workspace_bytes(...) bytes.
+ * d_y [rows][cols] contiguous.  workspace as above, of plh_layer_norm_workspace_bytes(...) bytes (partial sums of d_weight
+ * and d_bias: at most 1024 rows, 64 where cols > 16384).
  */
 int64_t plh_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
 int plh_layer_norm_backward(int dtype, int wdtype, const void* x, int64_t stride, int64_t rows, int64_t cols,

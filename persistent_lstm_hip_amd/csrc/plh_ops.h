@@ -85,7 +85,8 @@ constexpr float kOpLog2e = 1.4426950408889634f;
 
 // The logistic function and its complement, s = 1 / (1 + e) and 1 - s = e s with e = 2^min(-z log2 e, 126): the
 // complement keeps its relative precision where s is close to 1, and the cap keeps e s from being inf * 0 (it moves s
-// by less than 2^-126).  The minimum returns NaN for a NaN argument.
+// by less than 2^-126).  The minimum returns NaN for a NaN argument.  The exponent is one rounded product, so that e, and
+// with it the smaller of the two, is within (8 + 1.5 |z|) 2^-24 of its value, relative; absolutely both are within 8 2^-24.
 __device__ __forceinline__ void logistic_fast(float z, float& s, float& not_s) {
   const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(z * -kOpLog2e, 126.0f));
   s = __builtin_amdgcn_rcpf(1.0f + e);

@@ -598,7 +598,9 @@ __global__ void __launch_bounds__(P::THREADS, sizeof(T) == 2 ? 4 : 1) scan_forwa
   }
 }
 
-// Backward: tiles from the last to the first.
+// Backward: tiles from the last to the first.  With an output gate 236 to 254 registers for 16-bit elements, two waves per
+// SIMD, and 256 and 16 accumulation registers for 32-bit ones, one wave.  Either moves its bytes at the copy's rate
+// (5.2 TB/s): 16 x 4096 x 2048 bf16 353 us, at that rate 361; 16 x 2048 x 2048 fp32 365 and 361.
 template <typename T, typename P, bool GATED>
 __global__ void __launch_bounds__(P::THREADS) scan_backward_kernel(ScanArgs<T> p) {
   constexpr int VEC = P::VEC, R = P::R;

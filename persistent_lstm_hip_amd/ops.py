@@ -8,7 +8,8 @@
 * dropout_add      -- dropout from a counter-based generator, with the residual added in the same pass.
 
 All take float16, bfloat16 and float32 tensors on a HIP device, keep sums, statistics and states in float32, run on
-the device's current stream and are differentiable once.  As for the LSTM there is no CPU path: a missing library
+the device's current stream and are differentiable once, in reverse mode: a second derivative raises RuntimeError, a
+tensor with a forward-mode tangent ValueError.  As for the LSTM there is no CPU path: a missing library
 raises RuntimeError, an argument that the operators do not take, such as a tensor that is not on a HIP device,
 ValueError.  The arguments are checked, the outputs allocated and the kernels called in csrc/plh_torch.cpp.  The
 reference has no counterpart.
