@@ -300,6 +300,102 @@ int plh_layer_norm_backward(int dtype, int wdtype, const void* x, int64_t stride
 int plh_dropout_add(int dtype, const void* x, const void* residual, void* out, int64_t n, int threshold, uint64_t seed,
                     uint64_t offset, const int64_t* offset_dev, void* stream);
 
+/*
+ * Operators of a block around a selective state space scan, y = x + W_out scan(silu(conv(u)), dt, A, B, C, D, z), for
+ * training and serving.  Conventions as above.
+ */
+
+/*
+ * Causal convolution along time, a filter of `width` taps (1 to 8) per channel:
+ *     acc[b, t, c] = bias[c] + sum_k weight[c, k] x[b, t - width + 1 + k, c]      y = silu(acc), or acc (silu = 0)
+ *   x             element (b, t, c) at b * stride_b + t * stride_t + c
+ *   weight, bias  [channels][width] and [channels] of wdtype (PLH_F32 or dtype); bias may be NULL (zeros)
+ *   state         [batch][width - 1][channels]: the inputs before the first step, the oldest first, or NULL for zeros
+ *   lengths       device int32 [batch] or NULL, as for the gated scan: y is zero past a row's length, x is not read there
+ *   y             [batch][seq_len][channels], contiguous
+ *   state_n       [batch][width - 1][channels]: the last width - 1 inputs of every row (of its state, where it is shorter);
+ *                 not the memory of state
+ * The step takes one input per row and a state; its state_n may be state (in place).
+ * Limits: channels <= 2^24, batch * channels <= 2^28, batch * channels * seq_len <= 2^35.
+ */
+int plh_causal_conv_forward(int dtype, int wdtype, const void* x, int64_t stride_b, int64_t stride_t, int64_t batch,
+                            int64_t seq_len, int64_t channels, int width, const void* weight, const void* bias,
+                            const void* state, const int32_t* lengths, int silu, void* y, void* state_n, void* stream);
+int plh_causal_conv_step(int dtype, int wdtype, const void* x, int64_t stride_b, int64_t batch, int64_t channels,
+                         int width, const void* weight, const void* bias, const void* state, int silu, void* y,
+                         void* state_n, void* stream);
+/*
+ * Its gradient from d_y [batch][seq_len][channels] (contiguous; not read past a row's length) and d_state_n (or NULL for
+ * zeros): d_x [batch][seq_len][channels] (contiguous, zero past a row's length), d_weight, d_bias (of wdtype) and d_state
+ * (seq_len > 0), each of the four or NULL.  The workspace holds partial sums of d_weight and d_bias.
+ */
+int64_t plh_causal_conv_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int width);
+int plh_causal_conv_backward(int dtype, int wdtype, const void* x, int64_t stride_b, int64_t stride_t, int64_t batch,
+                             int64_t seq_len, int64_t channels, int width, const void* weight, const void* bias,
+                             const void* state, const int32_t* lengths, int silu, const void* d_y,
+                             const void* d_state_n, void* d_x, void* d_weight, void* d_bias, void* d_state,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Selective state space scan, for every row b, channel d and state n:
+ *     dt = softplus(raw + dt_bias[d]), or raw + dt_bias[d] (softplus = 0)
+ *     h_n <- exp(dt A[d, n]) h_n + dt u B[n]      y = sum_n C[n] h_n + D[d] u      out = y silu(z), or y (z NULL)
+ *   u, dt, z       [batch][seq_len][channels], element (b, t, d) at b * stride[0] + t * stride[1] + d; dt holds raw
+ *   B, C           [batch][seq_len][states], likewise
+ *   A              [channels][states], not positive (a decay); D, dt_bias [channels], either may be NULL (zeros);
+ *                  all of wdtype (PLH_F32 or dtype)
+ *   lengths        device int32 [batch] or NULL, as for the gated scan: h stays as it is past a row's length, out is
+ *                  zero there, and nothing is read
+ *   h0, h_n        device fp32 [batch][channels][states], either may be NULL (zeros; not wanted)
+ *   out            [batch][seq_len][channels], contiguous
+ *   states_out     device fp32 [plh_selective_scan_states(seq_len)][batch][channels][states] or NULL: what the backward
+ *                  pass needs
+ * The step is seq_len = 1 without lengths, from h to h_n, which may be the same memory.
+ * Limits: 1 <= states <= 64, channels <= 2^24, seq_len <= 2^30, batch * ceil(channels / 8) <= 2^23,
+ * batch * seq_len * states <= 2^30.
+ */
+typedef struct plh_selective_scan_args {
+  int dtype, wdtype;
+  const void *u, *dt, *z, *B, *C;
+  int64_t u_stride[2], dt_stride[2], z_stride[2], B_stride[2], C_stride[2];
+  const void *A, *D, *dt_bias;
+  const int32_t* lengths;
+  int64_t batch, seq_len, channels;
+  int states, softplus;
+} plh_selective_scan_args;
+
+int64_t plh_selective_scan_states(int64_t seq_len);
+int64_t plh_selective_scan_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int states, int backward);
+int plh_selective_scan_forward(const plh_selective_scan_args* args, const float* h0, void* out, float* h_n,
+                               float* states_out, void* workspace, int64_t workspace_bytes, void* stream);
+int plh_selective_scan_step(const plh_selective_scan_args* args, const float* h, void* out, float* h_n, void* stream);
+/*
+ * Its gradient from d_out [batch][seq_len][channels] (contiguous; not read past a row's length) and d_hn (fp32, or NULL for
+ * zeros), with the args and the states of the forward call.  d_u, d_dt, d_z (required with z) [batch][seq_len][channels],
+ * contiguous; d_B, d_C [batch][seq_len][states], contiguous; all zero past a row's length.  d_A, d_D, d_dt_bias of wdtype;
+ * d_h0 fp32.  All but d_u, d_dt and d_z may be NULL.
+ */
+typedef struct plh_selective_scan_grads {
+  void *d_u, *d_dt, *d_z, *d_B, *d_C;
+  void *d_A, *d_D, *d_dt_bias;
+  float* d_h0;
+} plh_selective_scan_grads;
+int plh_selective_scan_backward(const plh_selective_scan_args* args, const float* states, const void* d_out,
+                                const float* d_hn, const plh_selective_scan_grads* grads, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/*
+ * The Euclidean norm of all elements of `count` tensors together, and the tensors times min(1, max_norm / (norm + 1e-6)).
+ *   dtypes, in, out, numel   host arrays of `count`; tensor i has numel[i] elements of dtypes[i], dense.  out[i] may be
+ *                            in[i] (in place); out NULL: only the norm is wanted.  Tensors must not overlap otherwise.
+ *   max_norm                 infinity: no limit
+ *   norm                     device fp32
+ * Squares are summed in 64 bits.  A norm of infinity scales by zero, of NaN by NaN.
+ */
+int64_t plh_clip_grad_norm_workspace_bytes(int64_t count, const int64_t* numel);
+int plh_clip_grad_norm(int64_t count, const int* dtypes, const void* const* in, void* const* out, const int64_t* numel,
+                       double max_norm, float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

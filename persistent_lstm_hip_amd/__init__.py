@@ -14,7 +14,17 @@ from .model import (
     PersistentLSTMRegressor,
     StandardLSTMRegressor,
 )
-from .ops import dropout_add, gated_scan, gated_scan_step, layer_norm
+from .ops import (
+    causal_conv,
+    causal_conv_step,
+    clip_grad_norm,
+    dropout_add,
+    gated_scan,
+    gated_scan_step,
+    layer_norm,
+    selective_scan,
+    selective_scan_step,
+)
 
 __all__ = [
     "PersistentLSTM",
@@ -33,4 +43,9 @@ __all__ = [
     "gated_scan_step",
     "layer_norm",
     "dropout_add",
+    "causal_conv",
+    "causal_conv_step",
+    "selective_scan",
+    "selective_scan_step",
+    "clip_grad_norm",
 ]

@@ -24,7 +24,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libpersistent_lstm_hip.so")
 TORCH_PATH = os.path.join(LIB_DIR, "plh_torch.so")
 BENCH_PATH = os.path.join(LIB_DIR, "plh_bench")
 SOURCES = ["plh_wavefront.hip", "plh_sliced.hip", "plh_rec.hip", "plh_gemm.hip", "plh_pack.hip", "plh_launch.hip",
-           "plh_probe.hip", "plh_capi.hip", "plh_scan.hip", "plh_norm.hip", "plh_dropout.hip"]
+           "plh_probe.hip", "plh_capi.hip", "plh_scan.hip", "plh_norm.hip", "plh_dropout.hip",
+           "plh_conv.hip", "plh_selective.hip", "plh_clip.hip"]
 HEADERS = ["plh_internal.h", "plh_device.h", "plh_ops.h", os.path.join("..", "..", "include", "persistent_lstm_hip.h")]
 
 ARCH = "gfx950"

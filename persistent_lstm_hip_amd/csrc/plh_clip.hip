@@ -1,0 +1,222 @@
+// plh_clip.hip -- the norm of all elements of many tensors, and the tensors scaled so that it stays within a limit.
+//
+//   norm = sqrt(sum of squares)      out = in * min(1, max_norm / (norm + 1e-6))
+//
+// Two passes, both bound by the memory traffic: one reads everything, one reads it again and writes it.  The tensors of a
+// launch are one list of chunks, of which every workgroup has an equal run, so that many small tensors cost one launch
+// and no more than a chunk each.  Squares are summed in 64 bits: nothing between the smallest and the largest fp32 value
+// overflows or vanishes, and the conversion hides under the loads.  The workgroups' sums are added in a fixed order by
+// every workgroup of the second pass, which saves a launch in between (and a wait for one workgroup).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "plh_ops.h"
+
+namespace plh {
+namespace {
+
+constexpr int kTensors = 100;     // of a launch: their table is passed by value (a captured graph keeps it)
+constexpr int kChunk = 16384;     // elements
+constexpr int64_t kGroups = 1024;  // workgroups of all launches together, about
+
+struct ClipArgs {
+  const void* in[kTensors];
+  void* out[kTensors];
+  int64_t n[kTensors];
+  int64_t first[kTensors];  // chunk that the tensor starts at
+  uint8_t dtype[kTensors];
+  int count;
+  int64_t chunks;
+  double* part;    // the workgroups' sums of squares, of all launches
+  int64_t parts;
+  int64_t offset;  // ... of this launch
+  double max_norm;
+  float* norm;     // or null: written by another launch
+  bool stream;
+};
+
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+  lds_barrier();
+  v = 0.0;
+#pragma unroll
+  for (int i = 0; i < 256 / kWave; ++i) v += lds[i];
+  return v;
+}
+
+// f(element type, tensor, first element, elements) for every chunk of the workgroup's run.
+template <typename F>
+__device__ __forceinline__ void over_chunks(const ClipArgs& p, F&& f) {
+  const int64_t per = (p.chunks + gridDim.x - 1) / gridDim.x, begin = blockIdx.x * per, end = min(begin + per, p.chunks);
+  if (begin >= end) return;
+  int lo = 0, hi = p.count;  // the last tensor that starts at or before the first chunk
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (p.first[mid] <= begin)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  for (int64_t c = begin; c < end; ++c) {
+    while (lo + 1 < p.count && p.first[lo + 1] <= c) ++lo;
+    const int64_t at = (c - p.first[lo]) * kChunk;
+    const int n = (int)min(p.n[lo] - at, (int64_t)kChunk);
+    switch (p.dtype[lo]) {
+      case PLH_F16: f(_Float16(), lo, at, n); break;
+      case PLH_BF16: f(__bf16(), lo, at, n); break;
+      default: f(float(), lo, at, n); break;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) clip_norm_kernel(ClipArgs p) {
+  __shared__ double lds[256 / kWave];
+  double sum[2] = {0.0, 0.0};
+  over_chunks(p, [&](auto zero, int k, int64_t at, int n) __attribute__((always_inline)) {
+    using T = decltype(zero);
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const T* const src = static_cast<const T*>(p.in[k]) + at;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n / VEC; i += 256) {
+      const Vec<T, VEC> v = load_vec<T, VEC>(src + i * VEC);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const double d = (double)(float)v.v[j];
+        sum[j % 2] = fma(d, d, sum[j % 2]);
+      }
+    }
+    const int rest = n / VEC * VEC + (int)threadIdx.x;
+    if (rest < n) {
+      const double d = (double)(float)src[rest];
+      sum[0] = fma(d, d, sum[0]);
+    }
+  });
+  const double all = block_sum(sum[0] + sum[1], lds);
+  if (threadIdx.x == 0) p.part[p.offset + blockIdx.x] = all;
+}
+
+// SCALE: out = in * factor; otherwise only the norm is written.  IN_PLACE: nothing is read or written where the factor is
+// one.
+template <bool SCALE, bool IN_PLACE>
+__global__ void __launch_bounds__(256) clip_scale_kernel(ClipArgs p) {
+  __shared__ double lds[256 / kWave];
+  double sum = 0.0;
+  for (int64_t i = threadIdx.x; i < p.parts; i += 256) sum += p.part[i];
+  const double norm = sqrt(block_sum(sum, lds));
+  if (p.norm && blockIdx.x == 0 && threadIdx.x == 0) *p.norm = (float)norm;
+  if constexpr (SCALE) {
+    const double ratio = p.max_norm / (norm + 1e-6);
+    const bool whole = ratio > 1.0 || p.max_norm == __builtin_huge_val();
+    const float factor = whole ? 1.0f : (float)ratio;  // (NaN stays NaN)
+    if (IN_PLACE && factor == 1.0f) return;
+    over_chunks(p, [&](auto zero, int k, int64_t at, int n) __attribute__((always_inline)) {
+      using T = decltype(zero);
+      constexpr int VEC = 16 / (int)sizeof(T);
+      const T* const src = static_cast<const T*>(p.in[k]) + at;
+      T* const dst = static_cast<T*>(p.out[k]) + at;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n / VEC; i += 256) {
+        const Vec<T, VEC> v = load_vec<T, VEC>(src + i * VEC);
+        float y[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = (float)v.v[j] * factor;
+        if (!IN_PLACE && p.stream)
+          store_vec_stream(dst + i * VEC, round_to<T, VEC>(y));
+        else
+          store_vec(dst + i * VEC, round_to<T, VEC>(y));
+      }
+      const int rest = n / VEC * VEC + (int)threadIdx.x;
+      if (rest < n) dst[rest] = round_to<T>((float)src[rest] * factor);
+    });
+  }
+}
+
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+
+// Calls f(first tensor, tensors, chunks, workgroups, offset of its sums) for every launch; the number of sums.
+template <typename F>
+int64_t over_launches(int64_t count, const int64_t* numel, F&& f) {
+  int64_t all = 0, offset = 0;
+  for (int64_t i = 0; i < count; ++i) all += chunks_of(numel[i]);
+  int64_t i = 0;
+  do {
+    const int64_t begin = i;
+    int64_t chunks = 0;
+    for (; i < count && i - begin < kTensors; ++i) chunks += chunks_of(numel[i]);
+    const int64_t share = all > 0 ? (int64_t)((double)kGroups * (double)chunks / (double)all) : 0;
+    const int64_t groups = std::max<int64_t>(1, std::min(chunks, share));
+    f(begin, i - begin, chunks, groups, offset);
+    offset += groups;
+  } while (i < count);
+  return offset;
+}
+
+}  // namespace
+}  // namespace plh
+
+extern "C" {
+
+int64_t plh_clip_grad_norm_workspace_bytes(int64_t count, const int64_t* numel) {
+  if (count < 0 || (count > 0 && !numel)) return -1;
+  for (int64_t i = 0; i < count; ++i)
+    if (numel[i] < 0 || numel[i] > (int64_t(1) << 40)) return -1;
+  return plh::over_launches(count, numel, [](int64_t, int64_t, int64_t, int64_t, int64_t) {}) * (int64_t)sizeof(double);
+}
+
+int plh_clip_grad_norm(int64_t count, const int* dtypes, const void* const* in, void* const* out, const int64_t* numel,
+                       double max_norm, float* norm, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* const what = "clip_grad_norm";
+  const int64_t need = plh_clip_grad_norm_workspace_bytes(count, numel);
+  if (need < 0) return plh::op_error(PLH_ERR_INVALID, what, "count and numel must be non-negative, numel at most 2^40");
+  if (count > 0 && (!dtypes || !in)) return plh::op_error(PLH_ERR_INVALID, what, "dtypes and in are required");
+  if (!norm) return plh::op_error(PLH_ERR_INVALID, what, "norm is required");
+  if (!(max_norm >= 0.0)) return plh::op_error(PLH_ERR_INVALID, what, "max_norm must be non-negative");
+  bool in_place = out != nullptr;
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (dtypes[i] != PLH_F16 && dtypes[i] != PLH_BF16 && dtypes[i] != PLH_F32)
+      return plh::op_error(PLH_ERR_INVALID, what, "dtype must be PLH_F16, PLH_BF16 or PLH_F32");
+    if (numel[i] > 0 && (!in[i] || (out && !out[i])))
+      return plh::op_error(PLH_ERR_INVALID, what, "a tensor with elements is missing");
+    if (out && out[i] != in[i]) in_place = false;
+    bytes += numel[i] * (dtypes[i] == PLH_F32 ? 4 : 2);
+  }
+  if (!workspace || workspace_bytes < need || !plh::aligned(workspace, 16))
+    return plh::op_error(PLH_ERR_INVALID, what,
+                         "workspace missing, smaller than plh_clip_grad_norm_workspace_bytes() or not 16-byte aligned");
+  const hipStream_t s = (hipStream_t)stream;
+  const bool scale = out && !(in_place && max_norm == __builtin_huge_val());  // (no limit: only the norm is wanted)
+  hipError_t e = hipSuccess;
+  for (int pass = 0; pass < 2; ++pass) {
+    plh::over_launches(count, numel, [&](int64_t begin, int64_t tensors, int64_t chunks, int64_t groups, int64_t offset) {
+      if (e != hipSuccess) return;
+      plh::ClipArgs p = {};
+      int64_t first = 0;
+      for (int64_t i = 0; i < tensors; ++i) {
+        p.in[i] = in[begin + i], p.out[i] = out ? out[begin + i] : nullptr;
+        p.n[i] = numel[begin + i], p.dtype[i] = (uint8_t)dtypes[begin + i], p.first[i] = first;
+        first += plh::chunks_of(numel[begin + i]);
+      }
+      p.count = (int)tensors, p.chunks = chunks, p.part = (double*)workspace, p.offset = offset;
+      p.parts = need / (int64_t)sizeof(double), p.max_norm = max_norm, p.norm = begin == 0 ? norm : nullptr;
+      p.stream = bytes >= (32 << 20);
+      const dim3 grid((unsigned)groups), block(256);
+      if (pass == 0)
+        hipLaunchKernelGGL(plh::clip_norm_kernel, grid, block, 0, s, p);
+      else if (scale && in_place)
+        hipLaunchKernelGGL((plh::clip_scale_kernel<true, true>), grid, block, 0, s, p);
+      else if (scale)
+        hipLaunchKernelGGL((plh::clip_scale_kernel<true, false>), grid, block, 0, s, p);
+      else if (begin == 0)
+        hipLaunchKernelGGL((plh::clip_scale_kernel<false, false>), dim3(1), block, 0, s, p);
+      e = hipGetLastError();
+    });
+  }
+  return e == hipSuccess ? PLH_OK : plh::op_error(e, what);
+}
+
+}  // extern "C"

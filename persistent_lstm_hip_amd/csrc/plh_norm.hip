@@ -74,23 +74,6 @@ __device__ __forceinline__ float mean_of(float sum, const NormArgs& p) {
   return fmaf(fmaf(-m, (float)p.cols, sum), p.inv_cols, m);
 }
 
-// A parameter vector's VEC elements from column c on.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_param(const void* p, bool p32, int c, float fill, float (&v)[VEC]) {
-  if (!p) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = fill;
-  } else if (p32) {
-    const Vec<float, VEC> t = load_vec<float, VEC>(static_cast<const float*>(p) + c);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = t.v[j];
-  } else {
-    const Vec<T, VEC> t = load_vec<T, VEC>(static_cast<const T*>(p) + c);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = (float)t.v[j];
-  }
-}
-
 // LPR threads per row, each with NV pieces of VEC neighbouring columns: piece i of thread l is number i LPR + l.  The
 // last piece of a row is moved back to end with it; its first `skip` elements then belong to the piece before: they
 // are computed and stored by both, and counted once.

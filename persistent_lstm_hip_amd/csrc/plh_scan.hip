@@ -54,14 +54,6 @@ struct ScanArgs {
   float* d_c0;
 };
 
-// The slab of a launch's workgroup i of n.  Workgroups go round the eight XCDs in turn; here each XCD gets neighbouring
-// slabs, so that a cache line that two slabs share is read into one L2 (33 x 1001 x 333 fp16, no slab aligned: forward
-// 47.7 -> 40.2 us, backward 79.4 -> 68.2).
-__device__ __forceinline__ unsigned slab_of(unsigned i, unsigned n) {
-  const unsigned per = n / 8;
-  return i < per * 8 ? (i % 8) * per + i / 8 : i;
-}
-
 // Where a thread stands: its channels, its place among the time groups, its row's length.
 template <int VEC_, int CT_, int TG_, int R_, bool MANY_>
 struct Place {

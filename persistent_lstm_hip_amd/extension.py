@@ -40,6 +40,21 @@ _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 
 
+class SelectiveScanArgs(ctypes.Structure):
+    """plh_selective_scan_args."""
+
+    _fields_ = ([("dtype", _i32), ("wdtype", _i32)] + [(n, _vp) for n in ("u", "dt", "z", "B", "C")] +
+                [(n + "_stride", _i64 * 2) for n in ("u", "dt", "z", "B", "C")] +
+                [(n, _vp) for n in ("A", "D", "dt_bias", "lengths")] +
+                [(n, _i64) for n in ("batch", "seq_len", "channels")] + [("states", _i32), ("softplus", _i32)])
+
+
+class SelectiveScanGrads(ctypes.Structure):
+    """plh_selective_scan_grads."""
+
+    _fields_ = [(n, _vp) for n in ("d_u", "d_dt", "d_z", "d_B", "d_C", "d_A", "d_D", "d_dt_bias", "d_h0")]
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     lib.plh_abi_version.restype = _i32
     lib.plh_abi_version.argtypes = []
@@ -103,6 +118,31 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.plh_layer_norm_backward.argtypes = norm + [_vp] * 7 + [_i64, _vp]
     lib.plh_dropout_add.restype = _i32
     lib.plh_dropout_add.argtypes = [_i32, _vp, _vp, _vp, _i64, _i32, ctypes.c_uint64, ctypes.c_uint64, _vp, _vp]
+    conv = [_i32, _i32, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32]
+    lib.plh_causal_conv_forward.restype = _i32
+    lib.plh_causal_conv_forward.argtypes = conv + [_vp, _vp, _vp]
+    lib.plh_causal_conv_step.restype = _i32
+    lib.plh_causal_conv_step.argtypes = [_i32, _i32, _vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]
+    lib.plh_causal_conv_workspace_bytes.restype = _i64
+    lib.plh_causal_conv_workspace_bytes.argtypes = [_i64, _i64, _i64, _i32]
+    lib.plh_causal_conv_backward.restype = _i32
+    lib.plh_causal_conv_backward.argtypes = conv + [_vp] * 7 + [_i64, _vp]
+    lib.plh_selective_scan_states.restype = _i64
+    lib.plh_selective_scan_states.argtypes = [_i64]
+    lib.plh_selective_scan_workspace_bytes.restype = _i64
+    lib.plh_selective_scan_workspace_bytes.argtypes = [_i64, _i64, _i64, _i32, _i32]
+    args, grads = ctypes.POINTER(SelectiveScanArgs), ctypes.POINTER(SelectiveScanGrads)
+    lib.plh_selective_scan_forward.restype = _i32
+    lib.plh_selective_scan_forward.argtypes = [args, _vp, _vp, _vp, _vp, _vp, _i64, _vp]
+    lib.plh_selective_scan_step.restype = _i32
+    lib.plh_selective_scan_step.argtypes = [args, _vp, _vp, _vp, _vp]
+    lib.plh_selective_scan_backward.restype = _i32
+    lib.plh_selective_scan_backward.argtypes = [args, _vp, _vp, _vp, grads, _vp, _i64, _vp]
+    lib.plh_clip_grad_norm_workspace_bytes.restype = _i64
+    lib.plh_clip_grad_norm_workspace_bytes.argtypes = [_i64, ctypes.POINTER(_i64)]
+    lib.plh_clip_grad_norm.restype = _i32
+    lib.plh_clip_grad_norm.argtypes = [_i64, ctypes.POINTER(_i32), ctypes.POINTER(_vp), ctypes.POINTER(_vp),
+                                       ctypes.POINTER(_i64), ctypes.c_double, _vp, _vp, _i64, _vp]
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -1,4 +1,4 @@
-"""Operators of a residual block around a recurrence that is parallel over time, for training and serving:
+"""Operators of residual blocks around a recurrence that is parallel over time, for training and serving:
 
     y = x + dropout(W_o scan(W_g layer_norm(x)))
 
@@ -6,6 +6,19 @@
 * gated_scan_step  -- one token of it, from and to a state.
 * layer_norm       -- over the last dimension.
 * dropout_add      -- dropout from a counter-based generator, with the residual added in the same pass.
+
+or, with a state wider than its channel and decays that depend on the input,
+
+    u, z = W_in layer_norm(x)    u = causal_conv(u)    dt, B, C = W_x u    y = x + W_out selective_scan(u, dt, A, B, C, D, z)
+
+* causal_conv          -- short causal convolution along time with its activation.
+* causal_conv_step     -- one token of it, from and to a state.
+* selective_scan       -- selective state space scan over a whole sequence, with its skip and gate.
+* selective_scan_step  -- one token of it, from and to a state.
+
+and, between a backward pass and an optimizer's step,
+
+* clip_grad_norm   -- many tensors scaled to a global norm.
 
 All take float16, bfloat16 and float32 tensors on a HIP device, keep sums, statistics and states in float32, run on
 the device's current stream and are differentiable once, in reverse mode: a second derivative raises RuntimeError, a
@@ -17,7 +30,7 @@ reference has no counterpart.
 from __future__ import annotations
 
 import operator
-from typing import Optional, Sequence, Tuple, Union
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -102,3 +115,108 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor] = None, *, p: 
     if isinstance(offset, torch.Tensor):
         return require_torch_ops().dropout_add(x, residual, p, _u64(seed, "seed"), 0, offset)
     return require_torch_ops().dropout_add(x, residual, p, _u64(seed, "seed"), _u64(offset, "offset"), None)
+
+
+def _lengths(lengths):
+    return lengths if lengths is None or isinstance(lengths, torch.Tensor) else torch.as_tensor(lengths)
+
+
+def _optional(t, name: str) -> None:
+    if t is not None:
+        _tensor(t, name)
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                state: Optional[torch.Tensor] = None, *,
+                lengths: Union[torch.Tensor, Sequence[int], None] = None,
+                silu: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A causal convolution along time with a filter of its own for every channel, over x [batch, time, channels]:
+
+        acc_t = bias + sum_k weight[:, k] x_{t - width + 1 + k}        y_t = silu(acc_t), or acc_t with silu=False
+
+    weight [channels, width] with a width of 1 to 8, bias [channels], of x's type or float32 (both the same).  state: the
+    width - 1 inputs before the first step, the oldest first, [batch, width - 1, channels] of x's type (default: zeros).
+    Returns (y of x's shape, the state after the last step).  lengths: as for gated_scan; a row's state is that after
+    its last step, its outputs are zero from there on.
+
+    x may have any batch and time strides (half of a projection's output, say).  Differentiable in x, weight, bias and
+    state, from both results.
+    """
+    _tensor(x, "x")
+    _tensor(weight, "weight")
+    _optional(bias, "bias")
+    _optional(state, "state")
+    return require_torch_ops().causal_conv(x, weight, bias, state, _lengths(lengths), silu)
+
+
+def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                     silu: bool = True, inplace: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One step of causal_conv for serving: x [batch, channels], state [batch, width - 1, channels].  Returns (y, the new
+    state); with inplace=True state itself is overwritten and returned.  Not differentiable."""
+    _tensor(x, "x")
+    _tensor(state, "state")
+    _tensor(weight, "weight")
+    _optional(bias, "bias")
+    return require_torch_ops().causal_conv_step(x, state, weight, bias, silu, inplace)
+
+
+def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                   D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                   h0: Optional[torch.Tensor] = None, *, dt_bias: Optional[torch.Tensor] = None, softplus: bool = True,
+                   lengths: Union[torch.Tensor, Sequence[int], None] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The selective state space scan over u and dt [batch, time, channels], B and C [batch, time, states] (shared by all
+    channels); for every channel d and state n
+
+        s_t = softplus(dt_t + dt_bias), or dt_t + dt_bias with softplus=False
+        h_t = exp(s_t A[d, n]) h_{t-1} + s_t u_t B_t[n]        y_t = sum_n C_t[n] h_t + D[d] u_t
+
+    and out_t = y_t silu(z_t), or y_t without z [batch, time, channels].  A [channels, states] with 1 to 64 states, not
+    positive (it is a decay); D and dt_bias [channels], either may be missing; these three have u's type or float32 (all
+    the same), the others u's type.  Returns (out of u's shape and type, h_n [batch, channels, states] float32).  h0: the
+    state before the first step (default: zeros).  lengths: as for gated_scan; a row's h_n is the state after its last
+    step, its outputs are zero from there on.
+
+    u, dt, z, B and C may have any batch and time strides (parts of projections' outputs).  Differentiable in all of
+    them, A, D, dt_bias and h0, from both results.
+    """
+    for t, name in ((u, "u"), (dt, "dt"), (A, "A"), (B, "B"), (C, "C")):
+        _tensor(t, name)
+    for t, name in ((D, "D"), (z, "z"), (h0, "h0"), (dt_bias, "dt_bias")):
+        _optional(t, name)
+    return require_torch_ops().selective_scan(u, dt, A, B, C, D, z, h0, dt_bias, softplus, _lengths(lengths))
+
+
+def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                        h: torch.Tensor, D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, *,
+                        dt_bias: Optional[torch.Tensor] = None, softplus: bool = True,
+                        inplace: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One step of selective_scan for serving: u, dt and z [batch, channels], B and C [batch, states], h [batch, channels,
+    states] float32.  Returns (out, the new h); with inplace=True h itself is overwritten and returned.  Not
+    differentiable."""
+    for t, name in ((u, "u"), (dt, "dt"), (A, "A"), (B, "B"), (C, "C"), (h, "h")):
+        _tensor(t, name)
+    for t, name in ((D, "D"), (z, "z"), (dt_bias, "dt_bias")):
+        _optional(t, name)
+    return require_torch_ops().selective_scan_step(u, dt, A, B, C, h, D, z, dt_bias, softplus, inplace)
+
+
+def clip_grad_norm(grads: Iterable[Optional[torch.Tensor]], max_norm: float, *,
+                   inplace: bool = False) -> Tuple[List[Optional[torch.Tensor]], torch.Tensor]:
+    """The tensors scaled by min(1, max_norm / (norm + 1e-6)), where norm is the Euclidean norm of all their elements
+    together.  Returns (the scaled tensors, norm): new tensors, or with inplace=True `grads` themselves, overwritten; norm is
+    a float32 scalar on the device (nothing waits for it).  Entries that are None stay None, so that
+
+        clip_grad_norm([p.grad for p in model.parameters()], 1.0, inplace=True)
+
+    serves a training step.  The tensors are on one device, of any shapes, strides and mixed types; squares are summed
+    in 64 bits.  max_norm may be infinite: nothing is scaled.  A norm of infinity scales by zero and one of NaN by NaN, as
+    torch.nn.utils.clip_grad_norm_ does.  Not differentiable.
+    """
+    if isinstance(grads, torch.Tensor):
+        raise ValueError("grads must be a sequence of tensors, not a tensor")
+    grads = list(grads)
+    for g in grads:
+        _optional(g, "a gradient")
+    out, norm = require_torch_ops().clip_grad_norm([g for g in grads if g is not None], float(max_norm), inplace)
+    left = iter(out)
+    return [None if g is None else next(left) for g in grads], norm
