@@ -182,6 +182,12 @@ __device__ __forceinline__ float silu_slope(float v) {
   return s * fmaf(f, 1.0f - s, 1.0f);
 }
 
+__device__ __forceinline__ void silu(float v, float& value, float& slope) {
+  const float s = sigmoid(v), low = __builtin_elementwise_maximum(v, -3e38f);
+  value = low * s;
+  slope = s * fmaf(__builtin_elementwise_minimum(low, 3e38f), 1.0f - s, 1.0f);
+}
+
 inline bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
 
 // Calls f with a value of the element type that `dtype` names; false if it names none.

@@ -15,14 +15,16 @@
 //
 // What bounds it: per state and step one exponential and four other operations forward (eight more backward, and
 // the sums over states and channels), per channel and step four values of the activations' type forward, seven
-// backward.  With 16 states the arithmetic takes longer than the traffic, so the layout saves operations: a thread has
-// two neighbouring channels by four neighbouring states, whose B and C it reads once for both, and eight consecutive steps,
-// whose decays stay in registers between the passes over them:
+// backward.  With 16 states the arithmetic takes longer than the traffic, so the layout saves operations.  A thread has
+// up to four neighbouring states of a channel for eight consecutive steps, whose decays stay in registers between the passes
+// over them:
 //   1. the decays, and the map of the thread's eight steps
 //   2. the waves of a workgroup are consecutive in time; their maps meet in LDS around one barrier, and every wave folds
 //      those before it into its own start
 //   3. the eight steps from there, with the outputs
-// so that an exponential is taken once although four times as many waves run as there are channels for.
+// so that an exponential is taken once although four times as many waves run as there are channels for.  (Two channels
+// by four states per thread read B and C half as often, and add up dB and dC in half the operations, but take twice the
+// registers: 8 x 2048 x 2048 channels x 16 states bf16 forward 256 -> 320 us, backward 886 -> 1770, with spills.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -33,8 +35,6 @@
 namespace plh {
 namespace {
 
-constexpr int kCh = 2, kNs = 4;      // channels and states of a thread
-constexpr int kSlots = kCh * kNs;
 constexpr int kRun = 8;              // steps of a thread
 constexpr int kWaves = 4;            // waves along time
 constexpr int kTileSteps = kRun * kWaves;
@@ -69,13 +69,16 @@ struct SelArgs {
   float* part_w;          // [segs][B][D N + 2 D]: dA, dD, dbias
 };
 
-// Lanes of a wave: SL threads side by side have the states of a pair of channels, 64 / SL such pairs make a group.
-template <int SL>
-struct Wave {
-  static constexpr int PAIRS = 64 / SL, CH = PAIRS * kCh, NP = SL * kNs;  // channels, padded states
-  // How the wave reads its eight steps of CH channels: eight lanes per step with E neighbouring channels each.
-  static constexpr int E = CH / 8;
-  static_assert(kRun == 8 && CH % 8 == 0, "eight steps by eight lanes");
+// A wave's layout: SL threads side by side have the states of a channel, NS neighbouring ones each; 64 / SL channels make
+// the wave's group.
+template <int SL_, int NS_>
+struct Geo {
+  static constexpr int SL = SL_, NS = NS_;
+  static constexpr int GROUP = 64 / SL, NP = SL * NS;  // NP: states, padded
+  // How the wave reads its eight steps of GROUP channels and of NP states: eight lanes per step, with E neighbouring
+  // channels and F neighbouring states each.
+  static constexpr int E = GROUP >= 8 ? GROUP / 8 : 1, F = NP >= 8 ? NP / 8 : 1;
+  static_assert(kRun == 8, "eight steps by eight lanes");
 };
 
 // Orders the LDS accesses of a wave's lanes among each other (they run in order; this is for the compiler).
@@ -84,12 +87,14 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-struct alignas(16) F4 {
-  float v[4];
+// N floats that are moved at once, in LDS.
+template <int N>
+struct alignas(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4) Fs {
+  float v[N];
 };
-struct alignas(8) F2 {
-  float v[2];
-};
+
+template <int N>
+using FVec = Vec<float, N>;
 
 // Up to E elements, the first n of them from memory; the others zero.
 template <typename T, int E>
@@ -120,27 +125,30 @@ __device__ __forceinline__ float param(const void* p, bool p32, int64_t i, float
   return !p ? fill : p32 ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
 }
 
-// log(1 + exp(v)) = max(v, 0) + log1p(exp(-|v|)) with log1p(e) = 2 artanh(s), s = e / (2 + e) in [0, 1/3]: the
-// logarithm of a number close to one would lose the small values, which step sizes are.  The series' remainder after
-// s^15 / 15 is below 2 s^17 / 17 / (1 - s^2) < 2^-29 s.
-__device__ __forceinline__ float softplus_of(float v) {
+// softplus(v) = log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|), with log1p(e) = 2 artanh(s), s = e / (2 + e) in
+// [0, 1/3]: the logarithm of a number close to one would lose the small values, which step sizes are.  artanh(s) / s is a
+// polynomial of degree 4 in s^2, fitted over that range to a relative error of 2^-26.9 at most.  Its slope is sigmoid(v).
+__device__ __forceinline__ float log1p_of(float e) {
+  const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+  float t = fmaf(0.140891671f, q, 0.139803007f);
+  t = fmaf(t, q, 0.200124547f);
+  t = fmaf(t, q, 0.333331585f);
+  return 2.0f * fmaf(t * q, s, s);
+}
+__device__ __forceinline__ float softplus(float v) {
   const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(v) * kOpLog2e);
-  const float d = 2.0f + e, r = __builtin_amdgcn_rcpf(d), s = e * fmaf(fmaf(-d, r, 1.0f), r, r), q = s * s;
-  float t = 1.0f / 15;
-  t = fmaf(t, q, 1.0f / 13);
-  t = fmaf(t, q, 1.0f / 11);
-  t = fmaf(t, q, 1.0f / 9);
-  t = fmaf(t, q, 1.0f / 7);
-  t = fmaf(t, q, 1.0f / 5);
-  t = fmaf(t, q, 1.0f / 3);
-  t = fmaf(t * q, s, s);
-  return fmaf(2.0f, t, __builtin_elementwise_maximum(v, 0.0f));
+  return log1p_of(e) + __builtin_elementwise_maximum(v, 0.0f);
+}
+__device__ __forceinline__ void softplus(float v, float& value, float& slope) {
+  const float e = __builtin_amdgcn_exp2f(-__builtin_fabsf(v) * kOpLog2e), r = __builtin_amdgcn_rcpf(1.0f + e);
+  value = log1p_of(e) + __builtin_elementwise_maximum(v, 0.0f);
+  slope = v < 0.0f ? e * r : r;
 }
 
 // The decay of a run of steps.  Every step's own is positive; their product may underflow (or, of a growing state,
 // overflow), and 0 * inf would be NaN where the steps one after the other are not.
 __device__ __forceinline__ float run_decay(float log2_decay) {
-  return __builtin_amdgcn_exp2f(fminf(fmaxf(log2_decay, -126.0f), 127.0f));
+  return __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(log2_decay, -126.0f, 127.0f));
 }
 
 // Sum over the SL lanes that share a pair of channels, to all of them.
@@ -198,93 +206,95 @@ __device__ __forceinline__ At place(const SelArgs& p, int64_t unit, int channels
 }
 
 // The LDS of a wave.
-template <int SL>
-struct WaveLds {
-  F4 step[kRun][Wave<SL>::PAIRS];   // dt, dt u of the pair's two channels
-  F4 bc[kRun][2][SL];               // B and C
-  float y[kRun][Wave<SL>::CH];
+template <typename G>
+struct alignas(16) WaveLds {
+  Fs<2> step[kRun][G::GROUP];   // dt and dt u of every channel
+  Fs<G::NS> bc[kRun][2][G::SL];  // B and C
+  float y[kRun][G::GROUP];
 };
+// A map's factors or sums, of all threads of a wave.
+template <typename G>
 struct MapLds {
-  F4 v[kSlots / 4][64];
+  Fs<G::NS> v[64];
+  __device__ __forceinline__ void put(int lane, const float (&f)[G::NS]) {
+    Fs<G::NS> t;
+#pragma unroll
+    for (int j = 0; j < G::NS; ++j) t.v[j] = f[j];
+    v[lane] = t;
+  }
+  __device__ __forceinline__ void get(int lane, float (&f)[G::NS]) const {
+    const Fs<G::NS> t = v[lane];
+#pragma unroll
+    for (int j = 0; j < G::NS; ++j) f[j] = t.v[j];
+  }
 };
 
-// A wave's states of the pair's two channels, [B][D][N] at row b; zero outside.
-template <int SL>
+// A thread's states, in [B][D][N] at row b; zero outside.
+template <typename G>
 struct Slots {
-  int c, n;      // first channel and state
-  int channels;  // of the two that there are
+  int c, n;    // channel and first state
+  int states;  // of the NS that there are
   __device__ __forceinline__ Slots(const SelArgs& p, const At& at, int lane) {
-    c = at.c0 + lane / SL * kCh, n = lane % SL * kNs;
-    channels = min(max(p.D_ - c, 0), kCh);
+    c = at.c0 + lane / G::SL, n = lane % G::SL * G::NS;
+    states = c < p.D_ ? min(max(p.N - n, 0), G::NS) : 0;
   }
-  __device__ __forceinline__ void load(const SelArgs& p, const float* base, int64_t b, float (&v)[kSlots]) const {
+  __device__ __forceinline__ void load(const SelArgs& p, const float* base, int64_t b, float (&v)[G::NS]) const {
+    const Vec<float, G::NS> t = load_some<float, G::NS>(base + (b * p.D_ + c) * p.N + n, states);
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) {
-      Vec<float, kNs> t = {};
-      if (i < channels && n < p.N) t = load_some<float, kNs>(base + (b * p.D_ + c + i) * p.N + n, p.N - n);
-#pragma unroll
-      for (int j = 0; j < kNs; ++j) v[i * kNs + j] = t.v[j];
-    }
+    for (int j = 0; j < G::NS; ++j) v[j] = t.v[j];
   }
-  __device__ __forceinline__ void store(const SelArgs& p, float* base, int64_t b, const float (&v)[kSlots]) const {
+  __device__ __forceinline__ void store(const SelArgs& p, float* base, int64_t b, const float (&v)[G::NS]) const {
+    Vec<float, G::NS> t;
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) {
-      Vec<float, kNs> t;
+    for (int j = 0; j < G::NS; ++j) t.v[j] = v[j];
+    store_some<float, G::NS>(base + (b * p.D_ + c) * p.N + n, t, states);
+  }
+  // The decays' rates, times log2 e.
+  template <typename T>
+  __device__ __forceinline__ void rates(const SelArgs& p, float (&v)[G::NS]) const {
 #pragma unroll
-      for (int j = 0; j < kNs; ++j) t.v[j] = v[i * kNs + j];
-      if (i < channels && n < p.N) store_some<float, kNs>(base + (b * p.D_ + c + i) * p.N + n, t, p.N - n);
-    }
+    for (int j = 0; j < G::NS; ++j)
+      v[j] = j < states ? kOpLog2e * param<T>(p.A, p.w32, (int64_t)c * p.N + n + j, 0.0f) : 0.0f;
   }
 };
 
-__device__ __forceinline__ void put_map(MapLds& m, int lane, const float (&v)[kSlots]) {
-#pragma unroll
-  for (int q = 0; q < kSlots / 4; ++q) m.v[q][lane] = F4{{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]}};
-}
-__device__ __forceinline__ void get_map(const MapLds& m, int lane, float (&v)[kSlots]) {
-#pragma unroll
-  for (int q = 0; q < kSlots / 4; ++q) {
-    const F4 t = m.v[q][lane];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[4 * q + j] = t.v[j];
-  }
-}
-
-// A wave's eight steps of one activation tensor, as loaded.
-template <typename T, int SL>
+// A wave's eight steps of a tensor, N elements per lane, as loaded: the lane's place in the tensor, moved from tile to tile.
+template <typename T, int N>
 struct Rows {
-  static constexpr int E = Wave<SL>::E;
-  Vec<T, E> v;
-  __device__ __forceinline__ void load(const Strided& s, const At& at, int t, int c, int n) {
-    v = Vec<T, E>{};
-    if (t < at.len && n > 0) v = load_some<T, E>(static_cast<const T*>(s.p) + at.b * s.b + (int64_t)t * s.t + c, n);
+  const T* at;
+  int64_t step;
+  int n;  // elements that there are
+  Vec<T, N> v;
+  __device__ __forceinline__ void place(const Strided& s, int64_t b, int64_t t, int c, int count, int steps) {
+    at = static_cast<const T*>(s.p) + b * s.b + t * s.t + c, step = s.t * steps, n = count, v = {};
+  }
+  // The next tile's; nothing where `on` is false.
+  __device__ __forceinline__ void load(bool on) {
+    v = load_some<T, N>(at, on ? n : 0);
+    at += step;
   }
 };
-// ... and of B and C.
-template <typename T, int SL>
-struct Coefs {
-  static constexpr int K = kRun * Wave<SL>::NP / 64 > 0 ? kRun * Wave<SL>::NP / 64 : 1;
-  T b[K], c[K];
-  __device__ __forceinline__ void load(const SelArgs& p, const At& at, int t0, int lane) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = lane + 64 * k, t = t0 + i / Wave<SL>::NP, n = i % Wave<SL>::NP;
-      b[k] = c[k] = (T)0.0f;
-      if (i < kRun * Wave<SL>::NP && t < at.len && n < p.N) {
-        b[k] = static_cast<const T*>(p.B.p)[at.b * p.B.b + (int64_t)t * p.B.t + n];
-        c[k] = static_cast<const T*>(p.C.p)[at.b * p.C.b + (int64_t)t * p.C.t + n];
-      }
-    }
+
+// What a wave reads of a tile.
+template <typename T, typename G>
+struct TileIn {
+  Rows<T, G::E> u, dt, z;
+  Rows<T, G::F> B, C;
+  __device__ __forceinline__ void place(const SelArgs& p, const At& at, int64_t t, int c, int n, int lane, int steps) {
+    const int f = lane % 8 * G::F, states = min(max(p.N - f, 0), G::F);
+    u.place(p.u, at.b, t, c, n, steps), dt.place(p.dt, at.b, t, c, n, steps);
+    if (p.z.p) z.place(p.z, at.b, t, c, n, steps);
+    z.v = {};
+    B.place(p.B, at.b, t, f, states, steps), C.place(p.C, at.b, t, f, states, steps);
   }
-  __device__ __forceinline__ void put(WaveLds<SL>& lds, int lane) const {
+  __device__ __forceinline__ void put_coefs(WaveLds<G>& lds, int lane) const {
+    if (G::NP < 8 && lane % 8 >= G::NP) return;
+    Fs<G::F> b, c;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = lane + 64 * k, r = i / Wave<SL>::NP, n = i % Wave<SL>::NP;
-      if (i < kRun * Wave<SL>::NP) {
-        lds.bc[r][0][n / 4].v[n % 4] = (float)b[k];
-        lds.bc[r][1][n / 4].v[n % 4] = (float)c[k];
-      }
-    }
+    for (int j = 0; j < G::F; ++j) b.v[j] = (float)B.v.v[j], c.v[j] = (float)C.v.v[j];
+    float* const dst = &lds.bc[lane / 8][0][0].v[0] + lane % 8 * G::F;
+    *reinterpret_cast<Fs<G::F>*>(dst) = b;
+    *reinterpret_cast<Fs<G::F>*>(dst + G::NP) = c;
   }
 };
 
@@ -294,141 +304,136 @@ enum Mode { kWhole, kMaps };
 
 // A workgroup carries a group of channels through a segment of time, a tile of four waves by eight steps at a time.  MAPS:
 // only the segment's map is wanted.
-template <typename T, int SL, Mode MODE>
+template <typename T, typename G, Mode MODE, bool GATED>
 __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArgs p) {
-  using W = Wave<SL>;
-  constexpr int E = W::E;
-  __shared__ WaveLds<SL> lds_all[kWaves];
-  __shared__ MapLds maps[2][kWaves][2];
+  constexpr int E = G::E, SL = G::SL, NS = G::NS;
+  __shared__ WaveLds<G> lds_all[kWaves];
+  __shared__ MapLds<G> maps[2][kWaves][2];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  WaveLds<SL>& lds = lds_all[wave];
+  WaveLds<G>& lds = lds_all[wave];
   const int seg = blockIdx.y;
-  const At at = place(p, slab_of(blockIdx.x, gridDim.x), W::CH);
-  const Slots<SL> mine(p, at, lane);
+  const At at = place(p, slab_of(blockIdx.x, gridDim.x), G::GROUP);
+  const Slots<G> mine(p, at, lane);
   const int64_t state_size = p.batch * p.D_ * p.N;
 
   // the layout that memory is read and written in
-  const int row = lane / 8, ec = lane % 8 * E, c = at.c0 + ec, n = min(max(p.D_ - c, 0), E);
-  float bias[E], skip[E], A[kSlots];
+  const int row = lane / 8, ec = lane % 8 * E, c = at.c0 + ec;
+  const int n = G::GROUP < 8 && ec >= G::GROUP ? 0 : min(max(p.D_ - c, 0), E);
+  float bias[E], skip[E], A[NS];
 #pragma unroll
   for (int j = 0; j < E; ++j) {
     bias[j] = j < n ? param<T>(p.bias, p.w32, c + j, 0.0f) : 0.0f;
     skip[j] = j < n ? param<T>(p.D, p.w32, c + j, 0.0f) : 0.0f;
   }
-#pragma unroll
-  for (int i = 0; i < kSlots; ++i) {
-    const int s = mine.n + i % kNs;
-    A[i] = i / kNs < mine.channels && s < p.N
-               ? kOpLog2e * param<T>(p.A, p.w32, (int64_t)(mine.c + i / kNs) * p.N + s, 0.0f) : 0.0f;
-  }
+  mine.template rates<T>(p, A);
 
   const int live = (at.len + kTileSteps - 1) / kTileSteps;  // tiles that the row reaches
   const int first = seg * p.seg_tiles, last = min(first + p.seg_tiles, p.tiles), live_last = min(last, live);
-  float carry[kSlots], decay[kSlots];
+  float carry[NS], decay[NS];
 #pragma unroll
-  for (int i = 0; i < kSlots; ++i) carry[i] = 0.0f, decay[i] = 1.0f;
+  for (int i = 0; i < NS; ++i) carry[i] = 0.0f, decay[i] = 1.0f;
   if (MODE == kWhole) {
     if (p.h0) mine.load(p, p.h0, at.b, carry);
     for (int s = 0; s < seg; ++s) {  // the segments before this one
-      float P[kSlots], Q[kSlots];
+      float P[NS], Q[NS];
       mine.load(p, p.seg + (int64_t)s * 2 * state_size, at.b, P);
       mine.load(p, p.seg + (int64_t)(s * 2 + 1) * state_size, at.b, Q);
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) carry[i] = fmaf(P[i], carry[i], Q[i]);
+      for (int i = 0; i < NS; ++i) carry[i] = fmaf(P[i], carry[i], Q[i]);
     }
   }
 
-  Rows<T, SL> nu, nd, nz;
-  Coefs<T, SL> nc;
-  const auto load = [&](int tile) __attribute__((always_inline)) {
-    const int t0 = tile * kTileSteps + wave * kRun, t = t0 + row;
-    nu.load(p.u, at, t, c, n);
-    nd.load(p.dt, at, t, c, n);
-    if (MODE == kWhole && p.z.p) nz.load(p.z, at, t, c, n);
-    nc.load(p, at, t0, lane);
+  int t = first * kTileSteps + wave * kRun + row;  // the lane's step
+  TileIn<T, G> next;
+  next.place(p, at, t, c, n, lane, kTileSteps);
+  const auto load = [&](int t) __attribute__((always_inline)) {
+    const bool on = t < at.len;
+    next.u.load(on), next.dt.load(on), next.B.load(on);
+    if (MODE == kWhole) {
+      if (GATED) next.z.load(on);
+      next.C.load(on);
+    }
   };
-  nz.v = {};
-  if (first < live_last) load(first);
-  for (int tile = first; tile < live_last; ++tile) {
-    const int t = tile * kTileSteps + wave * kRun + row;
+  T* out = static_cast<T*>(p.out) + (at.b * p.T_ + t) * p.D_ + c;
+  const int64_t out_step = (int64_t)kTileSteps * p.D_;
+  if (first < live_last) load(t);
+  for (int tile = first; tile < live_last; ++tile, t += kTileSteps, out += out_step) {
     // dt and dt u, B, C: into the wave's LDS
-    Vec<T, E> u = nu.v, z = nz.v;
-    {
-      float f[2 * E];
+    const Vec<T, E> u = next.u.v, z = next.z.v;
+    if (G::GROUP >= 8 || ec < G::GROUP) {
+      Fs<2 * E> f;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float raw = (float)nd.v.v[j] + bias[j], dt = t < at.len ? p.softplus ? softplus_of(raw) : raw : 0.0f;
-        f[2 * j] = dt, f[2 * j + 1] = dt * (float)u.v[j];
+        const float raw = (float)next.dt.v.v[j] + bias[j], dt = t < at.len ? p.softplus ? softplus(raw) : raw : 0.0f;
+        f.v[2 * j] = dt, f.v[2 * j + 1] = dt * (float)u.v[j];
       }
-      float* const dst = &lds.step[row][0].v[0] + 2 * ec;
-      __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E * 4 < 16 ? 8 : 16), f, sizeof(f));
-      nc.put(lds, lane);
+      *reinterpret_cast<Fs<2 * E>*>(&lds.step[row][ec]) = f;
     }
-    if (tile + 1 < live_last) load(tile + 1);
+    next.put_coefs(lds, lane);
+    if (tile + 1 < live_last) load(t + kTileSteps);
     wave_sync();
     // 1. decays and the run's map
-    float a[kRun][kSlots], Q[kSlots], sum[kCh] = {};
+    float a[kRun][NS], Q[NS], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) Q[i] = 0.0f;
+    for (int i = 0; i < NS; ++i) Q[i] = 0.0f;
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
-      const F4 s = lds.step[r][lane / SL], B = lds.bc[r][0][lane % SL];
+      const Fs<2> s = lds.step[r][lane / SL];
+      const Fs<NS> B = lds.bc[r][0][lane % SL];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        a[r][i] = __builtin_amdgcn_exp2f(s.v[i / kNs * 2] * A[i]);
-        Q[i] = fmaf(a[r][i], Q[i], s.v[i / kNs * 2 + 1] * B.v[i % kNs]);
+      for (int i = 0; i < NS; ++i) {
+        a[r][i] = __builtin_amdgcn_exp2f(s.v[0] * A[i]);
+        Q[i] = fmaf(a[r][i], Q[i], s.v[1] * B.v[i]);
       }
-      sum[0] += s.v[0], sum[1] += s.v[2];
+      sum += s.v[0];
     }
     // 2. the waves' maps
-    float P[kSlots], h[kSlots];
+    float P[NS], h[NS] = {};
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) P[i] = run_decay(sum[i / kNs] * A[i]);
-    MapLds(*const map)[2] = maps[tile & 1];
-    put_map(map[wave][0], lane, P);
-    put_map(map[wave][1], lane, Q);
+    for (int i = 0; i < NS; ++i) P[i] = run_decay(sum * A[i]);
+    MapLds<G>(*const map)[2] = maps[tile & 1];
+    map[wave][0].put(lane, P);
+    map[wave][1].put(lane, Q);
     if (MODE == kWhole && p.states && wave == 0) mine.store(p, p.states + tile * state_size, at.b, carry);
     lds_barrier();
+    // (selects, not branches: the maps are then read one after the other without a wait)
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (w == wave) {
+      float Pw[NS], Qw[NS];
+      map[w][0].get(lane, Pw);
+      map[w][1].get(lane, Qw);
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) h[i] = carry[i];
-      }
-      get_map(map[w][0], lane, P);
-      get_map(map[w][1], lane, Q);
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        carry[i] = fmaf(P[i], carry[i], Q[i]);
-        if (MODE == kMaps) decay[i] = fmaxf(decay[i] * P[i], 0x1p-126f);
+      for (int i = 0; i < NS; ++i) {
+        h[i] = w == wave ? carry[i] : h[i];
+        carry[i] = fmaf(Pw[i], carry[i], Qw[i]);
+        if (MODE == kMaps) decay[i] = fmaxf(decay[i] * Pw[i], 0x1p-126f);
       }
     }
     if (MODE == kMaps) continue;
     // 3. the steps from where they start
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
-      const F4 s = lds.step[r][lane / SL], B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
-      float y[kCh] = {};
+      const Fs<2> s = lds.step[r][lane / SL];
+      const Fs<NS> B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
+      float y = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        h[i] = fmaf(a[r][i], h[i], s.v[i / kNs * 2 + 1] * B.v[i % kNs]);
-        y[i / kNs] = fmaf(C.v[i % kNs], h[i], y[i / kNs]);
+      for (int i = 0; i < NS; ++i) {
+        h[i] = fmaf(a[r][i], h[i], s.v[1] * B.v[i]);
+        y = fmaf(C.v[i], h[i], y);
       }
-#pragma unroll
-      for (int i = 0; i < kCh; ++i) y[i] = states_sum<SL>(y[i]);
-      if (lane % SL == 0) *reinterpret_cast<F2*>(&lds.y[r][lane / SL * kCh]) = F2{{y[0], y[1]}};
+      lds.y[r][lane / SL] = states_sum<SL>(y);  // (the same from all lanes of a set, as below: a branch would part the steps)
     }
     wave_sync();
     if (t < p.T_ && n > 0) {
+      const Fs<E> sum = *reinterpret_cast<const Fs<E>*>(&lds.y[row][ec]);
       float y[E];
-      __builtin_memcpy(y, __builtin_assume_aligned(&lds.y[row][ec], E * 4 < 16 ? E * 4 : 16), sizeof(y));
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        y[j] = fmaf(skip[j], (float)u.v[j], y[j]);
-        if (p.z.p) y[j] *= silu((float)z.v[j]);
+        y[j] = fmaf(skip[j], (float)u.v[j], sum.v[j]);
+        if (GATED) y[j] *= silu((float)z.v[j]);
         if (t >= at.len) y[j] = 0.0f;
       }
-      store_some<T, E>(static_cast<T*>(p.out) + (at.b * p.T_ + t) * p.D_ + c, round_to<T, E>(y), n);
+      store_some<T, E>(out, round_to<T, E>(y), n);
     }
     wave_sync();
   }
@@ -439,10 +444,8 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     }
     return;
   }
-  for (int tile = max(first, live); tile < last; ++tile) {  // past the row
-    const int t = tile * kTileSteps + wave * kRun + row;
-    if (t < p.T_ && n > 0) store_some<T, E>(static_cast<T*>(p.out) + (at.b * p.T_ + t) * p.D_ + c, Vec<T, E>{}, n);
-  }
+  for (int tile = max(first, live_last); tile < last; ++tile, t += kTileSteps, out += out_step)  // past the row
+    if (t < p.T_) store_some<T, E>(out, Vec<T, E>{}, n);
   // (the last segment's carry is the row's: past the row nothing changes it)
   if (p.h_n && wave == 0 && seg == p.segs - 1) mine.store(p, p.h_n, at.b, carry);
 }
@@ -450,6 +453,7 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
 // ---- one token ----------------------------------------------------------------------------------
 
 // SL threads per channel with four states each, for ROWS rows one after the other with the channel's decays in registers.
+constexpr int kNs = 4;
 template <typename T, int SL, int ROWS>
 __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x, at = i / SL, rows = at / (uint32_t)p.D_;  // (less than 2^32 threads)
@@ -479,7 +483,7 @@ __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int64_t b = (int64_t)rows * ROWS + r;
-    const float v = (float)raw[r] + bias, dt = p.softplus ? softplus_of(v) : v, du = dt * (float)u[r];
+    const float v = (float)raw[r] + bias, dt = p.softplus ? softplus(v) : v, du = dt * (float)u[r];
     float y = 0.0f;
 #pragma unroll
     for (int j = 0; j < kNs; ++j) {
@@ -498,239 +502,262 @@ __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
 
 constexpr int kSide = 2;  // groups of channels of a workgroup, whose dB and dC it adds up
 
-template <int SL>
+template <typename G>
 struct BackLds {
-  WaveLds<SL> f;                    // (y: dy, then y; step: then s1, s2 of the pair's two channels)
-  float bc[kRun][2][Wave<SL>::NP];  // dB and dC of the wave's channels
+  WaveLds<G> f;               // (y: dy, then y; step: then s1, s2 of every channel)
+  alignas(16) float bc[kRun][2][G::NP];  // dB and dC of the wave's channels
+  // What a lane needs at both ends of a tile, of its E channels: registers that the steps in between take.
+  enum Kept { kU, kDt, kDy, kRawSlope, kGateSlope, kBias, kSkip, kSumSkip, kSumBias, kKept };
+  Fs<G::E> kept[kKept][64];
 };
 
 // The tiles of a segment from the last to the first.  MAPS: only the segment's map of E is wanted.
-template <typename T, int SL, Mode MODE>
-__global__ void __launch_bounds__(kSide* kWaves* kWave) selective_backward_kernel(SelArgs p) {
-  using W = Wave<SL>;
-  constexpr int E = W::E;
-  __shared__ BackLds<SL> lds_all[kSide][kWaves];
-  __shared__ MapLds maps[kSide][kWaves][3];
+template <typename T, typename G, Mode MODE, bool GATED>
+__global__ void __launch_bounds__(kSide* kWaves* kWave, kSide) selective_backward_kernel(SelArgs p) {
+  constexpr int E = G::E, SL = G::SL, NS = G::NS;
+  __shared__ BackLds<G> lds_all[kSide][kWaves];
+  __shared__ MapLds<G> maps[kSide][kWaves][3];
   const int lane = threadIdx.x % kWave, id = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wave = id % kWaves, side = id / kWaves;
-  BackLds<SL>& back = lds_all[side][wave];
-  WaveLds<SL>& lds = back.f;
+  BackLds<G>& back = lds_all[side][wave];
+  WaveLds<G>& lds = back.f;
   const int seg = blockIdx.y;
   const int64_t slab = slab_of(blockIdx.x, gridDim.x);
-  // A row's groups are taken in pairs (the last one may be alone); rows of one group each, in pairs of rows.
-  const bool pair_rows = p.groups == 1;
+  // A row's groups are taken kSide at a time; of rows of one group each, kSide rows.
+  const bool side_rows = p.groups == 1;
   const int per_row = (p.groups + kSide - 1) / kSide;
-  const int64_t b_of = pair_rows ? slab * kSide + side : slab / per_row;
-  const int group = pair_rows ? 0 : (int)(slab % per_row) * kSide + side;
+  const int64_t b_of = side_rows ? slab * kSide + side : slab / per_row;
+  const int group = side_rows ? 0 : (int)(slab % per_row) * kSide + side;
   const bool on = b_of < p.batch && group < p.groups;
-  const At at = place(p, on ? b_of * p.groups + group : p.units, W::CH);
-  const Slots<SL> mine(p, at, lane);
+  const int sides = side_rows ? 1 : p.groups - (group - side);  // that have a group, where they share a row
+  const At at = place(p, on ? b_of * p.groups + group : p.units, G::GROUP);
+  const Slots<G> mine(p, at, lane);
   const int64_t state_size = p.batch * p.D_ * p.N;
 
-  const int row = lane / 8, ec = lane % 8 * E, c = at.c0 + ec, n = min(max(p.D_ - c, 0), E);
-  float bias[E], skip[E], A[kSlots];
+  const int row = lane / 8, ec = lane % 8 * E, c = at.c0 + ec;
+  const int n = G::GROUP < 8 && ec >= G::GROUP ? 0 : min(max(p.D_ - c, 0), E);
+  using Kept = BackLds<G>;
+  const auto keep = [&](int k, const Fs<E>& v) __attribute__((always_inline)) { back.kept[k][lane] = v; };
+  const auto kept = [&](int k) __attribute__((always_inline)) { return back.kept[k][lane]; };
+  {
+    Fs<E> bias, skip;
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    bias[j] = j < n ? param<T>(p.bias, p.w32, c + j, 0.0f) : 0.0f;
-    skip[j] = j < n ? param<T>(p.D, p.w32, c + j, 0.0f) : 0.0f;
+    for (int j = 0; j < E; ++j) {
+      bias.v[j] = j < n ? param<T>(p.bias, p.w32, c + j, 0.0f) : 0.0f;
+      skip.v[j] = j < n ? param<T>(p.D, p.w32, c + j, 0.0f) : 0.0f;
+    }
+    keep(Kept::kBias, bias), keep(Kept::kSkip, skip), keep(Kept::kSumSkip, Fs<E>{}), keep(Kept::kSumBias, Fs<E>{});
+    wave_sync();
   }
-#pragma unroll
-  for (int i = 0; i < kSlots; ++i) {
-    const int s = mine.n + i % kNs;
-    A[i] = i / kNs < mine.channels && s < p.N
-               ? kOpLog2e * param<T>(p.A, p.w32, (int64_t)(mine.c + i / kNs) * p.N + s, 0.0f) : 0.0f;
-  }
+  float A[NS];
+  mine.template rates<T>(p, A);
 
   const auto length = [&](int64_t b) { return b >= p.batch ? 0 : p.lengths ? min(max(p.lengths[b], 0), p.T_) : p.T_; };
   const int row_len = length(b_of);  // (also of a wave without a group: it adds up its row's dB and dC)
-  const int most = pair_rows ? max(row_len, length(slab * kSide + 1 - side)) : row_len;  // the same in all waves
+  int most = row_len;  // the same in all waves
+  if (side_rows)
+    for (int i = 0; i < kSide; ++i) most = max(most, length(slab * kSide + i));
   const int live = (most + kTileSteps - 1) / kTileSteps;
   const int first = seg * p.seg_tiles, last = min(first + p.seg_tiles, p.tiles), live_last = min(last, live);
-  float carry[kSlots], decay[kSlots], dA[kSlots], d_skip[E], d_bias[E];
+  float carry[NS], decay[NS], dA[NS];
 #pragma unroll
-  for (int i = 0; i < kSlots; ++i) carry[i] = dA[i] = 0.0f, decay[i] = 1.0f;
-#pragma unroll
-  for (int j = 0; j < E; ++j) d_skip[j] = d_bias[j] = 0.0f;
+  for (int i = 0; i < NS; ++i) carry[i] = dA[i] = 0.0f, decay[i] = 1.0f;
   if (MODE == kWhole) {
     if (p.d_hn) mine.load(p, p.d_hn, at.b, carry);
     for (int s = p.segs - 1; s > seg; --s) {  // the segments after this one
-      float P[kSlots], Q[kSlots];
+      float P[NS], Q[NS];
       mine.load(p, p.seg + (int64_t)s * 2 * state_size, at.b, P);
       mine.load(p, p.seg + (int64_t)(s * 2 + 1) * state_size, at.b, Q);
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) carry[i] = fmaf(P[i], carry[i], Q[i]);
+      for (int i = 0; i < NS; ++i) carry[i] = fmaf(P[i], carry[i], Q[i]);
     }
   }
 
-  const Strided d_out = {p.d_out, (int64_t)p.T_ * p.D_, p.D_};
-  Rows<T, SL> nu, nd, nz, ng;
-  Coefs<T, SL> nc;
-  float nh[kSlots];
-  const auto load = [&](int tile) __attribute__((always_inline)) {
-    const int t0 = tile * kTileSteps + wave * kRun, t = t0 + row;
-    ng.load(d_out, at, t, c, n);
-    nd.load(p.dt, at, t, c, n);
-    if (MODE == kWhole) nu.load(p.u, at, t, c, n);
-    if (p.z.p) nz.load(p.z, at, t, c, n);
-    nc.load(p, at, t0, lane);
+  int t = (live_last - 1) * kTileSteps + wave * kRun + row;  // the lane's step
+  TileIn<T, G> next;
+  Rows<T, E> next_g;
+  next.place(p, at, t, c, n, lane, -kTileSteps);
+  next_g.place(Strided{p.d_out, (int64_t)p.T_ * p.D_, p.D_}, at.b, t, c, n, -kTileSteps);
+  const auto load = [&](int t) __attribute__((always_inline)) {
+    const bool on = t < at.len;
+    next_g.load(on), next.dt.load(on), next.C.load(on);
+    if (GATED) next.z.load(on);
+    if (MODE == kWhole) next.u.load(on), next.B.load(on);
+  };
+  // dB and dC of a tile that is done (its waves have met at a barrier since)
+  const int64_t bc_group = side_rows ? 0 : slab % per_row;
+  const int f = lane % 8 * G::F, f_states = G::NP < 8 && f >= G::NP ? 0 : min(max(p.N - f, 0), G::F);
+  const auto flush = [&](int t) __attribute__((always_inline)) {
+    if (t >= row_len) return;
+    float* const dst = p.part_bc + ((bc_group * p.batch + b_of) * p.T_ + t) * 2 * p.N + f;
+    const auto of = [&](int side, int k) __attribute__((always_inline)) {
+      return *reinterpret_cast<const Fs<G::F>*>(&lds_all[side][wave].bc[row][k][f < G::NP ? f : 0]);
+    };
+    const auto put = [&](int k, const Fs<G::F>& v) __attribute__((always_inline)) {
+      store_some<float, G::F>(dst + k * p.N, __builtin_bit_cast(FVec<G::F>, v), f_states);
+    };
+    if (side_rows) {
+      put(0, of(side, 0)), put(1, of(side, 1));
+    } else if (side < 2) {  // a row's sums: dB by the first side's waves, dC by the second one's
+      Fs<G::F> v = of(0, side);
+#pragma unroll
+      for (int i = 1; i < kSide; ++i) {
+        if (i >= sides) break;
+        const Fs<G::F> other = of(i, side);
+#pragma unroll
+        for (int j = 0; j < G::F; ++j) v.v[j] += other.v[j];
+      }
+      put(side, v);
+    }
+  };
+  if (first < live_last) load(t);
+  for (int tile = live_last - 1; tile >= first; --tile, t -= kTileSteps) {
+    float h[NS];
     if (MODE == kWhole) {
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) nh[i] = 0.0f;
-      if (tile * kTileSteps < at.len) mine.load(p, p.states + tile * state_size, at.b, nh);
+      for (int i = 0; i < NS; ++i) h[i] = 0.0f;
+      if (tile * kTileSteps < at.len) mine.load(p, p.states + tile * state_size, at.b, h);
     }
-  };
-  nz.v = {}, nu.v = {};
-  // dB and dC of a tile that is done (its waves have met at a barrier since)
-  const int64_t bc_group = pair_rows ? 0 : slab % per_row;
-  const auto flush = [&](int tile) __attribute__((always_inline)) {
-    const int t0 = tile * kTileSteps + wave * kRun;
-    for (int i = (pair_rows ? 0 : side * kWave) + lane; i < kRun * 2 * W::NP; i += (pair_rows ? 1 : kSide) * kWave) {
-      const int r = i / (2 * W::NP), k = i / W::NP % 2, s = i % W::NP, t = t0 + r;
-      if (t >= row_len || s >= p.N) continue;
-      float v = lds_all[pair_rows ? side : 0][wave].bc[r][k][s];
-      if (!pair_rows) v += lds_all[1][wave].bc[r][k][s];
-      p.part_bc[((bc_group * p.batch + b_of) * p.T_ + t) * 2 * p.N + k * p.N + s] = v;
-    }
-  };
-  if (first < live_last) load(live_last - 1);
-  for (int tile = live_last - 1; tile >= first; --tile) {
-    const int t = tile * kTileSteps + wave * kRun + row;
-    const Vec<T, E> u = nu.v, z = nz.v, g = ng.v, d = nd.v;
-    float dt[E], dy[E], start[kSlots];
     {
-      float f[2 * E];
+      const bool in = t < at.len;
+      const Fs<E> bias = kept(Kept::kBias);
+      Fs<E> u, dt, dy, d_raw, d_gate;  // (d_raw: the slope of dt; d_gate: the output's by z, but for the factor y)
+      Fs<2 * E> f;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float raw = (float)d.v[j] + bias[j];
-        dt[j] = t < at.len ? p.softplus ? softplus_of(raw) : raw : 0.0f;
-        f[2 * j] = dt[j], f[2 * j + 1] = dt[j] * (float)u.v[j];
-        dy[j] = (float)g.v[j];
-        if (p.z.p) dy[j] *= silu((float)z.v[j]);
+        u.v[j] = (float)next.u.v.v[j];
+        dt.v[j] = (float)next.dt.v.v[j] + bias.v[j], d_raw.v[j] = 1.0f;
+        if (p.softplus) softplus(dt.v[j], dt.v[j], d_raw.v[j]);
+        if (!in) dt.v[j] = 0.0f;
+        dy.v[j] = (float)next_g.v.v[j];
+        if (GATED) {
+          float value, slope;
+          silu((float)next.z.v.v[j], value, slope);
+          d_gate.v[j] = dy.v[j] * slope, dy.v[j] *= value;
+        }
+        f.v[2 * j] = dt.v[j], f.v[2 * j + 1] = dt.v[j] * u.v[j];
       }
-      float* const dst = &lds.step[row][0].v[0] + 2 * ec;
-      __builtin_memcpy(__builtin_assume_aligned(dst, 2 * E * 4 < 16 ? 8 : 16), f, sizeof(f));
-      __builtin_memcpy(__builtin_assume_aligned(&lds.y[row][ec], E * 4 < 16 ? E * 4 : 16), dy, sizeof(dy));
-      nc.put(lds, lane);
+      if (MODE == kWhole) {
+        keep(Kept::kU, u), keep(Kept::kDt, dt), keep(Kept::kDy, dy), keep(Kept::kRawSlope, d_raw);
+        if (GATED) keep(Kept::kGateSlope, d_gate);
+      }
+      if (G::GROUP >= 8 || ec < G::GROUP) {
+        *reinterpret_cast<Fs<2 * E>*>(&lds.step[row][ec]) = f;
+        *reinterpret_cast<Fs<E>*>(&lds.y[row][ec]) = dy;
+      }
     }
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) start[i] = nh[i];
-    if (tile > first) load(tile - 1);
+    next.put_coefs(lds, lane);
+    if (tile > first) load(t - kTileSteps);
     wave_sync();
     // 1. decays, the run's maps forward (h) and backward (E)
-    float a[kRun][kSlots], Qh[kSlots], Qe[kSlots], sum[kCh] = {};
+    float a[kRun][NS], Qh[NS], Qe[NS], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) Qh[i] = Qe[i] = 0.0f;
+    for (int i = 0; i < NS; ++i) Qh[i] = Qe[i] = 0.0f;
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
-      const F4 s = lds.step[r][lane / SL], B = lds.bc[r][0][lane % SL];
+      const Fs<2> s = lds.step[r][lane / SL];
+      const Fs<NS> B = lds.bc[r][0][lane % SL];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        a[r][i] = __builtin_amdgcn_exp2f(s.v[i / kNs * 2] * A[i]);
-        if (MODE == kWhole) Qh[i] = fmaf(a[r][i], Qh[i], s.v[i / kNs * 2 + 1] * B.v[i % kNs]);
+      for (int i = 0; i < NS; ++i) {
+        a[r][i] = __builtin_amdgcn_exp2f(s.v[0] * A[i]);
+        if (MODE == kWhole) Qh[i] = fmaf(a[r][i], Qh[i], s.v[1] * B.v[i]);
       }
-      sum[0] += s.v[0], sum[1] += s.v[2];
+      sum += s.v[0];
     }
 #pragma unroll
     for (int r = kRun - 1; r >= 0; --r) {
-      const F4 C = lds.bc[r][1][lane % SL];
-      const F2 q = *reinterpret_cast<const F2*>(&lds.y[r][lane / SL * kCh]);
+      const Fs<NS> C = lds.bc[r][1][lane % SL];
+      const float q = lds.y[r][lane / SL];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) Qe[i] = a[r][i] * fmaf(C.v[i % kNs], q.v[i / kNs], Qe[i]);
+      for (int i = 0; i < NS; ++i) Qe[i] = a[r][i] * fmaf(C.v[i], q, Qe[i]);
     }
     // 2. the waves' maps
-    float P[kSlots], h[kSlots], e[kSlots];
+    float P[NS], e[NS] = {};
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) P[i] = run_decay(sum[i / kNs] * A[i]);
-    MapLds(*const map)[3] = maps[side];
-    put_map(map[wave][0], lane, P);
-    put_map(map[wave][1], lane, Qe);
-    if (MODE == kWhole) put_map(map[wave][2], lane, Qh);
+    for (int i = 0; i < NS; ++i) P[i] = run_decay(sum * A[i]);
+    MapLds<G>(*const map)[3] = maps[side];
+    map[wave][0].put(lane, P);
+    map[wave][1].put(lane, Qe);
+    if (MODE == kWhole) map[wave][2].put(lane, Qh);
     lds_barrier();
-    if (MODE == kWhole && tile + 1 < live_last) flush(tile + 1);
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) h[i] = start[i];
+    if (MODE == kWhole && tile + 1 < live_last) flush(t + kTileSteps);
+    // (selects, not branches: the maps are then read one after the other without a wait)
 #pragma unroll
     for (int w = kWaves - 1; w >= 0; --w) {
-      if (w == wave) {
+      float Pw[NS], Qw[NS];
+      map[w][0].get(lane, Pw);
+      map[w][1].get(lane, Qw);
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) e[i] = carry[i];
-      }
-      get_map(map[w][0], lane, P);
-      get_map(map[w][1], lane, Qe);
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        carry[i] = fmaf(P[i], carry[i], Qe[i]);
-        if (MODE == kMaps) decay[i] = fmaxf(decay[i] * P[i], 0x1p-126f);
+      for (int i = 0; i < NS; ++i) {
+        e[i] = w == wave ? carry[i] : e[i];
+        carry[i] = fmaf(Pw[i], carry[i], Qw[i]);
+        if (MODE == kMaps) decay[i] = fmaxf(decay[i] * Pw[i], 0x1p-126f);
       }
     }
     if (MODE == kWhole) {
 #pragma unroll
       for (int w = 0; w + 1 < kWaves; ++w) {
-        if (w >= wave) break;
-        get_map(map[w][0], lane, P);
-        get_map(map[w][2], lane, Qh);
+        float Pw[NS], Qw[NS];
+        map[w][0].get(lane, Pw);
+        map[w][2].get(lane, Qw);
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) h[i] = fmaf(P[i], h[i], Qh[i]);
+        for (int i = 0; i < NS; ++i) h[i] = w < wave ? fmaf(Pw[i], h[i], Qw[i]) : h[i];
       }
     }
     lds_barrier();  // (the maps and the sums of the tile before have been read)
     if (MODE == kMaps) continue;
-    // 3. the states, step by step, each before its step; with a gate the outputs that it multiplies
-    float before[kRun][kSlots], out[kRun][kCh];
+    // 3. the states, each before its step
+    float before[kRun + 1][NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) before[0][i] = h[i];
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
-      const F4 s = lds.step[r][lane / SL], B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
-      out[r][0] = out[r][1] = 0.0f;
+      const Fs<2> s = lds.step[r][lane / SL];
+      const Fs<NS> B = lds.bc[r][0][lane % SL];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        before[r][i] = h[i];
-        h[i] = fmaf(a[r][i], h[i], s.v[i / kNs * 2 + 1] * B.v[i % kNs]);
-        out[r][i / kNs] = fmaf(C.v[i % kNs], h[i], out[r][i / kNs]);
-      }
+      for (int i = 0; i < NS; ++i)
+        before[r + 1][i] = fmaf(a[r][i], before[r][i], s.v[1] * B.v[i]);
     }
-    // 4. and backwards
+    wave_sync();  // (or what the steps read would be kept in registers for the way back)
+    // 4. and backwards through them
     const auto walk = [&](auto whole) __attribute__((always_inline)) {
       constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-    for (int r = kRun - 1; r >= 0; --r) {
-      const F4 s = lds.step[r][lane / SL], B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
-      const F2 q = *reinterpret_cast<const F2*>(&lds.y[r][lane / SL * kCh]);
-      const bool in = WHOLE || tile * kTileSteps + wave * kRun + r < at.len;
-      float s1[kCh] = {}, s2[kCh] = {}, dB[kNs] = {}, dC[kNs] = {};
+      for (int r = kRun - 1; r >= 0; --r) {
+        // (past the row E stays as it is, and a product of what is infinite there with a zero must not count)
+        if (!WHOLE && tile * kTileSteps + wave * kRun + r >= at.len) continue;
+        const Fs<2> s = lds.step[r][lane / SL];
+        const Fs<NS> B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
+        const float q = lds.y[r][lane / SL];
+        float s1 = 0.0f, s2 = 0.0f, y = 0.0f, dB[NS], dC[NS];
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        const int k = i / kNs, j = i % kNs;
-        const float G = fmaf(C.v[j], q.v[k], e[i]);
-        s1[k] = fmaf(G, B.v[j], s1[k]);
-        dB[j] = fmaf(G, s.v[2 * k + 1], dB[j]);
-        dC[j] = fmaf(q.v[k], r + 1 < kRun ? before[r + 1 < kRun ? r + 1 : r][i] : h[i], dC[j]);
-        e[i] = a[r][i] * G;
-        const float m = in ? e[i] * before[r][i] : 0.0f;  // (past the row it may be inf * 0)
-        s2[k] = fmaf(m, A[i], s2[k]);
-        dA[i] = fmaf(m, s.v[2 * k], dA[i]);
-      }
+        for (int j = 0; j < NS; ++j) {
+          const float g = fmaf(C.v[j], q, e[j]);
+          s1 = fmaf(g, B.v[j], s1);
+          dB[j] = g * s.v[1];
+          dC[j] = q * before[r + 1][j];
+          if (GATED) y = fmaf(C.v[j], before[r + 1][j], y);
+          e[j] = a[r][j] * g;
+          const float m = e[j] * before[r][j];
+          s2 = fmaf(m, A[j], s2);
+          dA[j] = fmaf(m, s.v[0], dA[j]);
+        }
+        lds.step[r][lane / SL] = Fs<2>{{states_sum<SL>(s1), states_sum<SL>(s2)}};
+        if (GATED) lds.y[r][lane / SL] = states_sum<SL>(y);
+        // dB to the low half of the wave, dC to the high one; with four states 0, 2 to the even rows of 16 lanes and 1, 3 to
+        // the odd ones, with two 0 and 1
+        float w[NS];
 #pragma unroll
-      for (int k = 0; k < kCh; ++k) {
-        s1[k] = states_sum<SL>(s1[k]);
-        s2[k] = states_sum<SL>(s2[k]);
-        if (p.z.p) out[r][k] = states_sum<SL>(out[r][k]);
+        for (int j = 0; j < NS; ++j) w[j] = pair_sum<true>(dB[j], dC[j]);
+        float* const dst = &back.bc[r][lane / 32][lane % SL * NS + (NS > 1 ? lane / 16 % 2 : 0)];
+        if constexpr (NS == 4) {
+          const float x0 = row_rest_sum<SL>(pair_sum<false>(w[0], w[1])), x2 = row_rest_sum<SL>(pair_sum<false>(w[2], w[3]));
+          dst[0] = x0, dst[2] = x2;
+        } else {
+          const float x0 = row_rest_sum<SL>(pair_sum<false>(w[0], w[NS - 1]));
+          dst[0] = x0;
+        }
       }
-      // dB to the low half, dC to the high one, states 0, 2 to the even rows of 16 lanes, 1, 3 to the odd ones
-      float w[kNs], x[2];
-#pragma unroll
-      for (int j = 0; j < kNs; ++j) w[j] = pair_sum<true>(dB[j], dC[j]);
-      x[0] = row_rest_sum<SL>(pair_sum<false>(w[0], w[1]));
-      x[1] = row_rest_sum<SL>(pair_sum<false>(w[2], w[3]));
-      if (lane % 16 < SL) {
-        float* const dst = &back.bc[r][lane / 32][lane % SL * kNs + lane / 16 % 2];
-        dst[0] = x[0], dst[2] = x[1];
-      }
-      if (lane % SL == 0) {
-        constexpr float kLn2 = 0.69314718f;
-        lds.step[r][lane / SL] = F4{{s1[0], s2[0] * kLn2, s1[1], s2[1] * kLn2}};
-        if (p.z.p) *reinterpret_cast<F2*>(&lds.y[r][lane / SL * kCh]) = F2{{out[r][0], out[r][1]}};
-      }
-    }
     };
     if (tile * kTileSteps + (wave + 1) * kRun <= at.len)
       walk(std::true_type());
@@ -738,28 +765,27 @@ __global__ void __launch_bounds__(kSide* kWaves* kWave) selective_backward_kerne
       walk(std::false_type());
     wave_sync();
     if (t < p.T_ && n > 0) {
-      float f[2 * E], y[E], du[E], dr[E], dz[E];
-      __builtin_memcpy(f, __builtin_assume_aligned(&lds.step[row][0].v[0] + 2 * ec, 2 * E * 4 < 16 ? 8 : 16), sizeof(f));
-      __builtin_memcpy(y, __builtin_assume_aligned(&lds.y[row][ec], E * 4 < 16 ? E * 4 : 16), sizeof(y));
       const bool in = t < at.len;
+      const Fs<2 * E> f = *reinterpret_cast<const Fs<2 * E>*>(&lds.step[row][ec]);
+      const Fs<E> y = *reinterpret_cast<const Fs<E>*>(&lds.y[row][ec]), skip = kept(Kept::kSkip);
+      const Fs<E> u = kept(Kept::kU), dt = kept(Kept::kDt), dy = kept(Kept::kDy), d_raw = kept(Kept::kRawSlope);
+      Fs<E> d_gate = {}, d_skip = kept(Kept::kSumSkip), d_bias = kept(Kept::kSumBias);
+      if (GATED) d_gate = kept(Kept::kGateSlope);
+      float du[E], dr[E], dz[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float uj = (float)u.v[j];
-        du[j] = in ? fmaf(dt[j], f[2 * j], dy[j] * skip[j]) : 0.0f;
-        dr[j] = fmaf(uj, f[2 * j], f[2 * j + 1]);
-        if (p.softplus) dr[j] *= sigmoid((float)d.v[j] + bias[j]);
-        if (!in) dr[j] = 0.0f;
-        if (in) d_skip[j] = fmaf(dy[j], uj, d_skip[j]);
-        d_bias[j] += dr[j];
-        if (p.z.p) {
-          const float zj = (float)z.v[j];
-          dz[j] = in ? (float)g.v[j] * fmaf(skip[j], uj, y[j]) * silu_slope(zj) : 0.0f;
-        }
+        constexpr float kLn2 = 0.69314718f;
+        du[j] = in ? fmaf(dt.v[j], f.v[2 * j], dy.v[j] * skip.v[j]) : 0.0f;
+        dr[j] = in ? fmaf(u.v[j], f.v[2 * j], f.v[2 * j + 1] * kLn2) * d_raw.v[j] : 0.0f;
+        dz[j] = in ? d_gate.v[j] * fmaf(skip.v[j], u.v[j], y.v[j]) : 0.0f;
+        if (in) d_skip.v[j] = fmaf(dy.v[j], u.v[j], d_skip.v[j]);
+        d_bias.v[j] += dr[j];
       }
+      keep(Kept::kSumSkip, d_skip), keep(Kept::kSumBias, d_bias);
       const int64_t o = (at.b * p.T_ + t) * p.D_ + c;
       store_some<T, E>(static_cast<T*>(p.d_u) + o, round_to<T, E>(du), n);
       store_some<T, E>(static_cast<T*>(p.d_dt) + o, round_to<T, E>(dr), n);
-      if (p.z.p) store_some<T, E>(static_cast<T*>(p.d_z) + o, round_to<T, E>(dz), n);
+      if (GATED) store_some<T, E>(static_cast<T*>(p.d_z) + o, round_to<T, E>(dz), n);
     }
     wave_sync();
   }
@@ -776,45 +802,37 @@ __global__ void __launch_bounds__(kSide* kWaves* kWave) selective_backward_kerne
     const int64_t o = (at.b * p.T_ + t) * p.D_ + c;
     store_some<T, E>(static_cast<T*>(p.d_u) + o, Vec<T, E>{}, n);
     store_some<T, E>(static_cast<T*>(p.d_dt) + o, Vec<T, E>{}, n);
-    if (p.z.p) store_some<T, E>(static_cast<T*>(p.d_z) + o, Vec<T, E>{}, n);
+    if (GATED) store_some<T, E>(static_cast<T*>(p.d_z) + o, Vec<T, E>{}, n);
   }
   if (p.d_h0 && wave == 0 && seg == 0) mine.store(p, p.d_h0, at.b, carry);
 
   // The waves' sums of dA, dD and dbias, added in their order.
   lds_barrier();
-  if (first < live_last) flush(first);
+  if (first < live_last) flush(first * kTileSteps + wave * kRun + row);
   lds_barrier();
   float* const part = p.part_w + ((int64_t)seg * p.batch + at.b) * p.D_ * (p.N + 2);
-  put_map(maps[side][wave][0], lane, dA);
-  // (lanes that share a channel: the eight rows)
-  float(*const edge)[2 * E] = reinterpret_cast<float(*)[2 * E]>(&back);  // [64]
-  wave_sync();
-#pragma unroll
-  for (int j = 0; j < E; ++j) edge[lane][j] = d_skip[j], edge[lane][E + j] = d_bias[j];
+  maps[side][wave][0].put(lane, dA);
   lds_barrier();
   if (wave == 0) {
-    float v[kSlots];
+    float v[NS];
     for (int w = 1; w < kWaves; ++w) {
-      get_map(maps[side][w][0], lane, v);
+      maps[side][w][0].get(lane, v);
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) dA[i] += v[i];
+      for (int i = 0; i < NS; ++i) dA[i] += v[i];
     }
     mine.store(p, part - at.b * p.D_ * p.N, at.b, dA);
   } else if (wave == 1 && lane < 16) {
-    // eight lanes with E channels each, for dD and for dbias
+    // eight lanes with E channels each, for dD and for dbias, over the lanes that share a channel: the eight rows
     const int k = lane / 8;
-    float v[E] = {};
+    Vec<float, E> v = {};
     for (int w = 0; w < kWaves; ++w) {
-      const float(*const other)[2 * E] = reinterpret_cast<const float(*)[2 * E]>(&lds_all[side][w]);
-      for (int r = 0; r < 8; ++r)
+      for (int r = 0; r < 8; ++r) {
+        const Fs<E> t = lds_all[side][w].kept[Kept::kSumSkip + k][r * 8 + lane % 8];
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] += other[r * 8 + lane % 8][k * E + j];
+        for (int j = 0; j < E; ++j) v.v[j] += t.v[j];
+      }
     }
-    Vec<float, E> out;
-#pragma unroll
-    for (int j = 0; j < E; ++j) out.v[j] = v[j];
-    const int cc = at.c0 + lane % 8 * E;
-    if (p.D_ > cc) store_some<float, E>(part + (int64_t)p.D_ * (p.N + k) + cc, out, p.D_ - cc);
+    store_some<float, E>(part + (int64_t)p.D_ * (p.N + k) + c, v, n);
   }
 }
 
@@ -836,10 +854,14 @@ __global__ void __launch_bounds__(256) selective_coefs_kernel(SelArgs p, T* d_B,
 
 // ---- host ---------------------------------------------------------------------------------------
 
-int state_lanes(int states) {
-  int sl = 1;
-  while (sl * kNs < states) sl *= 2;
-  return sl;
+// f(std::integral_constant of the lanes, and of the states per lane) that serve `states`.
+template <typename F>
+auto with_states(int states, F&& f) {
+  if (states <= 4) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
+  if (states <= 8) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
+  if (states <= 16) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
+  if (states <= 32) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 4>());
+  return f(std::integral_constant<int, 16>(), std::integral_constant<int, 4>());
 }
 
 struct SelLayout {
@@ -851,7 +873,9 @@ struct SelLayout {
 // Segments of the time axis so that the launch has about `want` workgroups.
 SelLayout sel_layout(int64_t batch, int64_t seq_len, int64_t channels, int states, bool backward) {
   SelLayout l;
-  const int per = 64 / state_lanes(states) * kCh;
+  const int per = with_states(states, [](auto sl, auto ns) {
+    return Geo<decltype(sl)::value, decltype(ns)::value>::GROUP;
+  });
   l.groups = (int)((channels + per - 1) / per);
   l.bc_groups = (l.groups + kSide - 1) / kSide;
   l.tiles = (int)((seq_len + kTileSteps - 1) / kTileSteps);
@@ -874,38 +898,29 @@ SelWorkspace sel_workspace(int64_t batch, int64_t seq_len, int64_t channels, int
   return s;
 }
 
-// f(std::integral_constant of the lanes).
-template <typename F>
-hipError_t with_lanes(int states, F&& f) {
-  switch (state_lanes(states)) {
-    case 1: return f(std::integral_constant<int, 1>());
-    case 2: return f(std::integral_constant<int, 2>());
-    case 4: return f(std::integral_constant<int, 4>());
-    case 8: return f(std::integral_constant<int, 8>());
-    case 16: return f(std::integral_constant<int, 16>());
-    default: return hipErrorInvalidValue;
-  }
-}
-
 template <typename T>
 hipError_t launch_sel_forward(const SelArgs& p, hipStream_t s) {
-  return with_lanes(p.N, [&](auto lanes) {
-    constexpr int SL = decltype(lanes)::value;
+  return with_states(p.N, [&](auto sl, auto ns) {
+    using G = Geo<decltype(sl)::value, decltype(ns)::value>;
     const dim3 block(kWaves * kWave);
     if (p.segs > 1) {
-      hipLaunchKernelGGL((selective_forward_kernel<T, SL, kMaps>), dim3((unsigned)p.units, p.segs - 1), block, 0, s, p);
+      hipLaunchKernelGGL((selective_forward_kernel<T, G, kMaps, false>), dim3((unsigned)p.units, p.segs - 1), block, 0, s, p);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((selective_forward_kernel<T, SL, kWhole>), dim3((unsigned)p.units, p.segs), block, 0, s, p);
+    const dim3 grid((unsigned)p.units, p.segs);
+    if (p.z.p)
+      hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, true>), grid, block, 0, s, p);
+    else
+      hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, false>), grid, block, 0, s, p);
     return hipGetLastError();
   });
 }
 
 template <typename T>
 hipError_t launch_sel_step(const SelArgs& p, hipStream_t s) {
-  return with_lanes(p.N, [&](auto lanes) {
-    constexpr int SL = decltype(lanes)::value;
+  const auto lanes = [&](auto sl) {
+    constexpr int SL = decltype(sl)::value;
     const auto run = [&](auto rows) {
       constexpr int ROWS = decltype(rows)::value;
       const dim3 grid((unsigned)(((p.batch + ROWS - 1) / ROWS * p.D_ * SL + 255) / 256));
@@ -913,7 +928,12 @@ hipError_t launch_sel_step(const SelArgs& p, hipStream_t s) {
       return hipGetLastError();
     };
     return p.batch * p.D_ * SL >= 4 * 256 * 1024 ? run(std::integral_constant<int, 4>()) : run(std::integral_constant<int, 1>());
-  });
+  };
+  if (p.N <= 4) return lanes(std::integral_constant<int, 1>());
+  if (p.N <= 8) return lanes(std::integral_constant<int, 2>());
+  if (p.N <= 16) return lanes(std::integral_constant<int, 4>());
+  if (p.N <= 32) return lanes(std::integral_constant<int, 8>());
+  return lanes(std::integral_constant<int, 16>());
 }
 
 template <typename T>
@@ -921,16 +941,20 @@ hipError_t launch_sel_backward(SelArgs p, void* d_A, void* d_B, void* d_C, void*
   hipError_t e = hipSuccess;
   if (p.batch > 0) {
     const int64_t slabs = p.groups == 1 ? (p.batch + kSide - 1) / kSide : p.batch * ((p.groups + kSide - 1) / kSide);
-    e = with_lanes(p.N, [&](auto lanes) {
-      constexpr int SL = decltype(lanes)::value;
-      const dim3 block(kSide * kWaves * kWave);
-      if (p.segs > 1) {
-        hipLaunchKernelGGL((selective_backward_kernel<T, SL, kMaps>), dim3((unsigned)slabs, p.segs), block, 0, s, p);
-        const hipError_t e2 = hipGetLastError();
-        if (e2 != hipSuccess) return e2;
-      }
-      hipLaunchKernelGGL((selective_backward_kernel<T, SL, kWhole>), dim3((unsigned)slabs, p.segs), block, 0, s, p);
-      return hipGetLastError();
+    e = with_states(p.N, [&](auto sl, auto ns) {
+      using G = Geo<decltype(sl)::value, decltype(ns)::value>;
+      const dim3 grid((unsigned)slabs, p.segs), block(kSide * kWaves * kWave);
+      const auto run = [&](auto gated) {
+        constexpr bool GATED = decltype(gated)::value;
+        if (p.segs > 1) {
+          hipLaunchKernelGGL((selective_backward_kernel<T, G, kMaps, GATED>), grid, block, 0, s, p);
+          const hipError_t e2 = hipGetLastError();
+          if (e2 != hipSuccess) return e2;
+        }
+        hipLaunchKernelGGL((selective_backward_kernel<T, G, kWhole, GATED>), grid, block, 0, s, p);
+        return hipGetLastError();
+      };
+      return p.z.p ? run(std::true_type()) : run(std::false_type());
     });
     const int64_t n = p.batch * p.T_ * 2 * p.N;
     if (e == hipSuccess && n > 0 && (d_B || d_C)) {
