@@ -870,7 +870,13 @@ struct SelLayout {
   int bc_groups;  // sums of dB and dC
 };
 
-// Segments of the time axis so that the launch has about `want` workgroups.
+// With few workgroups the time axis is split into segments, whose maps a launch of its own computes first (about half of
+// the work again).  Forward four workgroups fill a CU, backward one.  Measured, us of a call without and with about 1024
+// (backward 256) workgroups of 16 states bf16 with a gate:
+//   forward   64 workgroups (2 x 4096 x 512) 264 and 58, 80 (1 x 16384 x 1280) 1177 and 284, 128 (1 x 2048 x 2048)
+//             134 and 58, 256 (4 x 2048 x 1024) 153 and 99; 512 (4 x 2048 x 2048) 162, in two segments 174
+//   backward  32 (2 x 4096 x 512) 709 and 136, 40 (1 x 16384 x 1280) 2938 and 668, 128 (4 x 2048 x 1024) 353 and 242;
+//             256 (4 x 2048 x 2048) 397, in two segments 488
 SelLayout sel_layout(int64_t batch, int64_t seq_len, int64_t channels, int states, bool backward) {
   SelLayout l;
   const int per = with_states(states, [](auto sl, auto ns) {
@@ -879,9 +885,12 @@ SelLayout sel_layout(int64_t batch, int64_t seq_len, int64_t channels, int state
   l.groups = (int)((channels + per - 1) / per);
   l.bc_groups = (l.groups + kSide - 1) / kSide;
   l.tiles = (int)((seq_len + kTileSteps - 1) / kTileSteps);
-  l.seg_tiles = std::max(l.tiles, 1);
-  l.segs = 1;
-  (void)batch, (void)backward;
+  const int64_t units = batch * l.groups, slabs = l.groups == 1 ? (batch + kSide - 1) / kSide : batch * l.bc_groups;
+  const int64_t groups = std::max<int64_t>(1, backward ? slabs : units);  // of workgroups
+  // (no segment shorter than two tiles: a short one's start costs as much as its steps)
+  const int64_t most = backward ? 200 : 400, want = groups > most ? 1 : (backward ? 256 : 1024) / groups;
+  l.seg_tiles = (int)std::max<int64_t>(std::max(1, std::min(2, l.tiles)), (l.tiles + want - 1) / want);
+  l.segs = std::max(1, (l.tiles + l.seg_tiles - 1) / l.seg_tiles);
   return l;
 }
 
