@@ -9,9 +9,10 @@
 // and the new state's gradient is added to the inputs that it holds.  acc is computed again where the gradient needs
 // it (W products for two bytes less to write and to read).
 //
-// Everything is bound by the memory traffic: x in, y out (dy in and dx out).  A thread has 16 bytes of neighbouring
-// channels (backward 4 channels, whose sums take the registers) and walks along time with the last W - 1 inputs in
-// registers, so that an input is read once but for the W - 1 at the edges of its stretch.
+// Everything is bound by the memory traffic: x in, y out (dy in and dx out).  A thread has four neighbouring channels and
+// walks along time with the last W - 1 inputs in registers, so that an input is read once but for the W - 1 at the edges of
+// its stretch.  512 rows of 1000 steps x 256 channels fp16, W = 4: forward 103 us (5.1 TB/s), backward 184 (4.3); with rows
+// of 200 to 1000 steps 87 and 179.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -83,9 +84,26 @@ __device__ __forceinline__ Vec<T, VEC> load_input(const ConvArgs& p, int64_t b, 
   return v;
 }
 
+// kStep steps from step t on, of a row of len steps; src moves on.  (One check for all of them, and a pointer that moves:
+// every step's own take more instructions than the filter, backward 246 -> 229 us at the sizes above, ragged.)
+template <typename T, int VEC>
+__device__ __forceinline__ void load_steps(const T*& src, int64_t stride, int t, int len, Vec<T, VEC> (&v)[kStep]) {
+  if (t + kStep <= len) {
+#pragma unroll
+    for (int s = 0; s < kStep; ++s) v[s] = load_vec<T, VEC>(src + s * stride);
+  } else {
+#pragma unroll
+    for (int s = 0; s < kStep; ++s) {
+      v[s] = Vec<T, VEC>{};
+      if (t + s < len) v[s] = load_vec<T, VEC>(src + s * stride);
+    }
+  }
+  src += kStep * stride;
+}
+
 // ---- forward ------------------------------------------------------------------------------------
 
-template <typename T, int VEC, int W>
+template <typename T, int VEC, int W, bool SILU>
 __global__ void __launch_bounds__(256) conv_forward_kernel(ConvArgs p) {
   const uint32_t block = blockIdx.x;
   if (W > 1 && block >= p.blocks) {  // the new state: a piece per thread
@@ -104,38 +122,44 @@ __global__ void __launch_bounds__(256) conv_forward_kernel(ConvArgs p) {
   const int begin = (int)(unit % (uint32_t)p.stretches) * p.stretch, end = min(begin + p.stretch, p.T_);
   const int len = row_length(p, b);
   T* const y = static_cast<T*>(p.y) + (b * p.T_ + begin) * p.C + c;
-  if (begin >= len) {
-    for (int t = begin; t < end; ++t) store_vec(y + (int64_t)(t - begin) * p.C, Vec<T, VEC>{});
-    return;
-  }
+  const int live_end = max(begin, min(end, len));
+  for (int t = live_end; t < end; ++t) store_vec(y + (int64_t)(t - begin) * p.C, Vec<T, VEC>{});
+  if (live_end == begin) return;
   float w[W][VEC], bias[VEC], x[W - 1 + kStep][VEC];
   load_filters<T, VEC, W>(p, c, w);
   load_param<T, VEC>(p.bias, p.w32, c, 0.0f, bias);
-  Vec<T, VEC> next[kStep];
 #pragma unroll
   for (int k = 0; k < W - 1; ++k) to_float(load_input<T, VEC, W>(p, b, begin - (W - 1) + k, len, c), x[k]);
-#pragma unroll
-  for (int s = 0; s < kStep; ++s) next[s] = load_input<T, VEC, W>(p, b, begin + s, len, c);
-  for (int t = begin; t < end; t += kStep) {
-#pragma unroll
-    for (int s = 0; s < kStep; ++s) to_float(next[s], x[W - 1 + s]);
-    if (t + kStep < end) {
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) next[s] = load_input<T, VEC, W>(p, b, t + kStep + s, len, c);
-    }
+  Vec<T, VEC> next[kStep];
+  const T* src = static_cast<const T*>(p.x) + b * p.stride_b + (int64_t)begin * p.stride_t + c;
+  T* dst = y;
+  const auto load = [&](int t) __attribute__((always_inline)) { load_steps(src, p.stride_t, t, len, next); };
+  const auto steps = [&](auto inside, int t) __attribute__((always_inline)) {
+    constexpr bool INSIDE = decltype(inside)::value;  // none of the steps lies past live_end
 #pragma unroll
     for (int s = 0; s < kStep; ++s) {
-      if (t + s >= end) break;
+      if (!INSIDE && t + s >= live_end) continue;
       float out[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float acc = bias[j];
 #pragma unroll
         for (int k = 0; k < W; ++k) acc = fmaf(w[k][j], x[s + k][j], acc);
-        out[j] = t + s >= len ? 0.0f : p.silu ? silu(acc) : acc;
+        out[j] = SILU ? silu(acc) : acc;
       }
-      store_vec(y + (int64_t)(t + s - begin) * p.C, round_to<T, VEC>(out));
+      store_vec(dst + (int64_t)s * p.C, round_to<T, VEC>(out));
     }
+    dst += (int64_t)kStep * p.C;
+  };
+  load(begin);
+  for (int t = begin; t < live_end; t += kStep) {
+#pragma unroll
+    for (int s = 0; s < kStep; ++s) to_float(next[s], x[W - 1 + s]);
+    if (t + kStep < live_end) load(t + kStep);
+    if (t + kStep <= live_end)
+      steps(std::true_type(), t);
+    else
+      steps(std::false_type(), t);
 #pragma unroll
     for (int k = 0; k < W - 1; ++k)
 #pragma unroll
@@ -190,7 +214,7 @@ struct ConvGroup {
 
 // A workgroup has a slab of CT pieces of channels and, TG at a time, the stretches of all rows that its number gives
 // it; it keeps its sums of dw and db in registers until the end.
-template <typename T, int VEC, int W, int CT>
+template <typename T, int VEC, int W, int CT, bool SILU>
 __global__ void __launch_bounds__(256) conv_backward_kernel(ConvArgs p) {
   constexpr int TG = 256 / CT;
   const int slabs = (p.pieces + CT - 1) / CT, slab = blockIdx.x % slabs, group = blockIdx.x / slabs;
@@ -211,14 +235,18 @@ __global__ void __launch_bounds__(256) conv_backward_kernel(ConvArgs p) {
     const int64_t b = unit / p.stretches;
     const int begin = unit % p.stretches * p.stretch, end = min(begin + p.stretch, p.T_);
     const int len = row_length(p, b);
-    const T* const d_y = static_cast<const T*>(p.d_y) + b * p.T_ * p.C + c;
-    T* const d_x = p.d_x ? static_cast<T*>(p.d_x) + b * p.T_ * p.C + c : nullptr;
+    const int64_t at = (b * p.T_ + begin) * p.C + c;
+    const T *src = static_cast<const T*>(p.x) + b * p.stride_b + (int64_t)begin * p.stride_t + c,
+            *grad = static_cast<const T*>(p.d_y) + at;
+    T* d_x = p.d_x ? static_cast<T*>(p.d_x) + at - (int64_t)(W - 1) * p.C : nullptr;  // of position t - (W - 1)
     T* const d_state = W > 1 && p.d_state && begin == 0 ? static_cast<T*>(p.d_state) + b * (W - 1) * p.C + c : nullptr;
-    const auto load_grad = [&](int t) __attribute__((always_inline)) {
-      return t < len ? load_vec<T, VEC>(d_y + (int64_t)t * p.C) : Vec<T, VEC>{};
-    };
+    const int live_end = max(begin, min(end, len));
+    if (p.d_x)
+      for (int t = live_end; t < end; ++t)
+        store_vec(static_cast<T*>(p.d_x) + at + (int64_t)(t - begin) * p.C, Vec<T, VEC>{});
+    if (live_end == begin && !d_state) continue;
     // Position t of the walk: da_t, whose dx is complete for position t - (W - 1).  A stretch is walked W - 1 positions
-    // past its end; the first one gives the state's gradient too.
+    // past its (or the row's) end; the first one gives the state's gradient too.
     float x[W - 1 + kStep][VEC], da[W - 1 + kStep][VEC];
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
@@ -228,36 +256,26 @@ __global__ void __launch_bounds__(256) conv_backward_kernel(ConvArgs p) {
     }
     Vec<T, VEC> nx[kStep], ng[kStep];
     const auto load = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) {
-        nx[s] = load_input<T, VEC, W>(p, b, t + s, len, c);
-        ng[s] = load_grad(t + s);
-      }
+      load_steps(src, p.stride_t, t, len, nx);
+      load_steps(grad, (int64_t)p.C, t, len, ng);
     };
-    const int last = end + W - 1;
-    load(begin);
-    for (int t = begin; t < last; t += kStep) {
-#pragma unroll
+    const auto steps = [&](auto inside, int t) __attribute__((always_inline)) {
+      constexpr bool INSIDE = decltype(inside)::value;  // all of the steps lie in the row and in the stretch, and so do
+#pragma unroll                                          // the positions whose dx they complete
       for (int s = 0; s < kStep; ++s) {
-        to_float(nx[s], x[W - 1 + s]);
-        to_float(ng[s], da[W - 1 + s]);
-      }
-      if (t + kStep < last) load(t + kStep);
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) {
-        const bool live = t + s < len, own = t + s < end;
+        const bool live = INSIDE || t + s < len;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           float& g = da[W - 1 + s][j];
-          if (p.silu) {
+          if (SILU) {
             float acc = bias[j];
 #pragma unroll
             for (int k = 0; k < W; ++k) acc = fmaf(w[k][j], x[s + k][j], acc);
             g *= silu_slope(acc);
           }
-          g = live ? g : 0.0f;
+          if (!INSIDE) g = live ? g : 0.0f;
         }
-        if (live && own) {
+        if (INSIDE || (live && t + s < end)) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
             db[j] += da[W - 1 + s][j];
@@ -266,29 +284,40 @@ __global__ void __launch_bounds__(256) conv_backward_kernel(ConvArgs p) {
           }
         }
         const int q = t + s - (W - 1);
-        if (q >= end || (q < begin && !d_state)) continue;
+        if (!INSIDE && (q >= live_end || (q < begin && !d_state))) continue;
         float out[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          out[j] = 0.0f;
+          out[j] = w[0][j] * da[s + W - 1][j];
 #pragma unroll
-          for (int k = 0; k < W; ++k) out[j] = fmaf(w[k][j], da[s + W - 1 - k][j], out[j]);
+          for (int k = 1; k < W; ++k) out[j] = fmaf(w[k][j], da[s + W - 1 - k][j], out[j]);
         }
-        if (W > 1 && p.d_state_n && q >= len - (W - 1) && q < len) {
+        if (!INSIDE && W > 1 && p.d_state_n && q >= len - (W - 1)) {
           float extra[VEC];
           to_float(load_vec<T, VEC>(static_cast<const T*>(p.d_state_n) + (b * (W - 1) + q - len + W - 1) * p.C + c), extra);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) out[j] += extra[j];
         }
-        if (q >= len) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) out[j] = 0.0f;
-        }
-        if (q < 0)
+        if (W > 1 && !INSIDE && q < 0)
           store_vec(d_state + (int64_t)(q + W - 1) * p.C, round_to<T, VEC>(out));
         else if (d_x)
-          store_vec(d_x + (int64_t)q * p.C, round_to<T, VEC>(out));
+          store_vec(d_x + (int64_t)s * p.C, round_to<T, VEC>(out));
       }
+      if (d_x) d_x += (int64_t)kStep * p.C;
+    };
+    const int last = live_end + W - 1;
+    load(begin);
+    for (int t = begin; t < last; t += kStep) {
+#pragma unroll
+      for (int s = 0; s < kStep; ++s) {
+        to_float(nx[s], x[W - 1 + s]);
+        to_float(ng[s], da[W - 1 + s]);
+      }
+      if (t + kStep < last) load(t + kStep);
+      if (t - (W - 1) >= begin && t + kStep <= live_end)
+        steps(std::true_type(), t);
+      else
+        steps(std::false_type(), t);
 #pragma unroll
       for (int k = 0; k < W - 1; ++k)
 #pragma unroll
@@ -318,9 +347,9 @@ __global__ void __launch_bounds__(256) conv_backward_kernel(ConvArgs p) {
 
 // ---- host ---------------------------------------------------------------------------------------
 
-template <typename T>
-constexpr int kConvVec = 16 / (int)sizeof(T);
-constexpr int kConvBackVec = 4;
+// Channels of a thread: wider pieces (16 bytes) take the registers that hide the loads' latency (512 x 1000 x 256 fp16,
+// W = 4, ragged, forward 107 us with eight channels, 92 with four, 89 with two; backward 229, 221 and 217).
+constexpr int kConvVec = 4, kConvStepVec = 4;
 
 // f(std::integral_constant of the width).
 template <typename F>
@@ -338,7 +367,9 @@ hipError_t with_width(int width, F&& f) {
   }
 }
 
-// Steps of a thread's stretch: long ones read fewer inputs twice, short ones make more threads.
+// Steps of a thread's stretch: long ones read fewer inputs twice, short ones make more threads, among which rows of unequal
+// length are shared more evenly (at the sizes above, ragged, forward with 16, 32 and 64 steps 85, 101 and 107 us, all rows
+// full 103, 110 and 117).
 int stretch_for(int64_t batch, int64_t seq_len, int64_t pieces, int64_t threads, int most) {
   const int64_t want = batch * pieces * seq_len / std::max<int64_t>(threads, 1);  // steps per thread that fill the device
   const int64_t steps = std::min<int64_t>(std::max<int64_t>(want, kStep), most);
@@ -350,23 +381,26 @@ hipError_t launch_conv_forward(ConvArgs p, int width, hipStream_t s) {
   const auto run = [&](auto v) {
     constexpr int VEC = decltype(v)::value;
     p.pieces = (p.C + VEC - 1) / VEC;
-    p.stretch = stretch_for(p.batch, p.T_, p.pieces, 256 * 1024, 32);
+    p.stretch = stretch_for(p.batch, p.T_, p.pieces, 256 * 1024, 16);
     p.stretches = (p.T_ + p.stretch - 1) / p.stretch;
     p.blocks = (uint32_t)((p.batch * p.stretches * p.pieces + 255) / 256);
     const int64_t state_blocks = (p.batch * (width - 1) * p.pieces + 255) / 256;
     const dim3 grid((unsigned)(p.blocks + state_blocks));
     if (grid.x == 0) return hipSuccess;
     return with_width(width, [&](auto w) {
-      hipLaunchKernelGGL((conv_forward_kernel<T, VEC, decltype(w)::value>), grid, dim3(256), 0, s, p);
+      if (p.silu)
+        hipLaunchKernelGGL((conv_forward_kernel<T, VEC, decltype(w)::value, true>), grid, dim3(256), 0, s, p);
+      else
+        hipLaunchKernelGGL((conv_forward_kernel<T, VEC, decltype(w)::value, false>), grid, dim3(256), 0, s, p);
       return hipGetLastError();
     });
   };
-  return p.C >= kConvVec<T> ? run(std::integral_constant<int, kConvVec<T>>()) : run(std::integral_constant<int, 1>());
+  return p.C >= kConvVec ? run(std::integral_constant<int, kConvVec>()) : run(std::integral_constant<int, 1>());
 }
 
 template <typename T>
 hipError_t launch_conv_step(ConvArgs p, int width, hipStream_t s) {
-  constexpr int VEC = kConvVec<T>;
+  constexpr int VEC = kConvStepVec;
   p.pieces = (p.C + VEC - 1) / VEC;
   const dim3 grid((unsigned)((p.batch * p.pieces + 255) / 256));
   return with_width(width, [&](auto w) {
@@ -382,14 +416,15 @@ struct ConvLayout {
 };
 ConvLayout conv_layout(int64_t batch, int64_t seq_len, int64_t channels) {
   ConvLayout l;
-  l.vec = channels >= kConvBackVec ? kConvBackVec : 1;
+  l.vec = channels >= kConvVec ? kConvVec : 1;
   l.pieces = (int)((channels + l.vec - 1) / l.vec);
   l.ct = l.pieces > 16 ? 32 : l.pieces > 8 ? 16 : 8;
   l.slabs = (l.pieces + l.ct - 1) / l.ct;
   l.stretch = stretch_for(batch, seq_len, l.pieces, 256 * 1024, 64);
   l.stretches = (int)((seq_len + l.stretch - 1) / l.stretch);
   l.units = batch * l.stretches;
-  const int64_t tg = 256 / l.ct, most = std::max<int64_t>(1, 1024 / l.slabs);
+  // (with 1024 and 2048 workgroups the ragged rows above take 193 and 179 us)
+  const int64_t tg = 256 / l.ct, most = std::max<int64_t>(1, 2048 / l.slabs);
   l.groups = (int)std::max<int64_t>(1, std::min<int64_t>((l.units + tg - 1) / tg, most));
   return l;
 }
@@ -403,7 +438,11 @@ hipError_t launch_conv_backward(ConvArgs p, int width, hipStream_t s) {
   hipError_t e = with_width(width, [&](auto w) {
     constexpr int W = decltype(w)::value;
     const auto run = [&](auto v, auto ct) {
-      hipLaunchKernelGGL((conv_backward_kernel<T, decltype(v)::value, W, decltype(ct)::value>), grid, dim3(256), 0, s, p);
+      constexpr int VEC = decltype(v)::value, CT = decltype(ct)::value;
+      if (p.silu)
+        hipLaunchKernelGGL((conv_backward_kernel<T, VEC, W, CT, true>), grid, dim3(256), 0, s, p);
+      else
+        hipLaunchKernelGGL((conv_backward_kernel<T, VEC, W, CT, false>), grid, dim3(256), 0, s, p);
     };
     const auto vec = [&](auto v) {
       if (l.ct == 32)
@@ -413,8 +452,8 @@ hipError_t launch_conv_backward(ConvArgs p, int width, hipStream_t s) {
       else
         run(v, std::integral_constant<int, 8>());
     };
-    if (l.vec == kConvBackVec)
-      vec(std::integral_constant<int, kConvBackVec>());
+    if (l.vec == kConvVec)
+      vec(std::integral_constant<int, kConvVec>());
     else
       run(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
     return hipGetLastError();
