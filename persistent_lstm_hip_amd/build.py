@@ -90,7 +90,7 @@ def build(verbose: bool = False) -> str:
         run([host_compiler(), "-std=c++17", "-O2", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
              "-DTORCH_EXTENSION_NAME=plh_torch"] + [a for d in include for a in ("-isystem", d)] +
             ["-c", os.path.join(CSRC, "plh_torch.cpp"), "-o", obj])
-        return [host_compiler(), "-shared", obj, "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu",
+        return [host_compiler(), "-shared", obj, "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
                 "-ltorch", "-ltorch_python", "-L" + LIB_DIR, "-lpersistent_lstm_hip", "-Wl,-rpath,$ORIGIN"]
 
     with tempfile.TemporaryDirectory() as objects, ThreadPoolExecutor(4) as pool:

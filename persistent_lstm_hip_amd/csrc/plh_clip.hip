@@ -48,21 +48,27 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return v;
 }
 
-// f(element type, tensor, first element, elements) for every chunk of the workgroup's run.
-template <typename F>
+// f(element type, tensor, first element, elements) for every chunk of the workgroup's run, from the first to the last or
+// back.
+template <bool BACK, typename F>
 __device__ __forceinline__ void over_chunks(const ClipArgs& p, F&& f) {
   const int64_t per = (p.chunks + gridDim.x - 1) / gridDim.x, begin = blockIdx.x * per, end = min(begin + per, p.chunks);
   if (begin >= end) return;
-  int lo = 0, hi = p.count;  // the last tensor that starts at or before the first chunk
+  const int64_t start = BACK ? end - 1 : begin;
+  int lo = 0, hi = p.count;  // the last tensor that starts at or before the chunk to start with
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (p.first[mid] <= begin)
+    if (p.first[mid] <= start)
       lo = mid;
     else
       hi = mid;
   }
-  for (int64_t c = begin; c < end; ++c) {
-    while (lo + 1 < p.count && p.first[lo + 1] <= c) ++lo;
+  for (int64_t i = 0; i < end - begin; ++i) {
+    const int64_t c = BACK ? end - 1 - i : begin + i;
+    if (BACK)
+      while (p.first[lo] > c) --lo;
+    else
+      while (lo + 1 < p.count && p.first[lo + 1] <= c) ++lo;
     const int64_t at = (c - p.first[lo]) * kChunk;
     const int n = (int)min(p.n[lo] - at, (int64_t)kChunk);
     switch (p.dtype[lo]) {
@@ -76,7 +82,7 @@ __device__ __forceinline__ void over_chunks(const ClipArgs& p, F&& f) {
 __global__ void __launch_bounds__(256) clip_norm_kernel(ClipArgs p) {
   __shared__ double lds[256 / kWave];
   double sum[2] = {0.0, 0.0};
-  over_chunks(p, [&](auto zero, int k, int64_t at, int n) __attribute__((always_inline)) {
+  over_chunks<false>(p, [&](auto zero, int k, int64_t at, int n) __attribute__((always_inline)) {
     using T = decltype(zero);
     constexpr int VEC = 16 / (int)sizeof(T);
     const T* const src = static_cast<const T*>(p.in[k]) + at;
@@ -113,7 +119,7 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipArgs p) {
     const bool whole = ratio > 1.0 || p.max_norm == __builtin_huge_val();
     const float factor = whole ? 1.0f : (float)ratio;  // (NaN stays NaN)
     if (IN_PLACE && factor == 1.0f) return;
-    over_chunks(p, [&](auto zero, int k, int64_t at, int n) __attribute__((always_inline)) {
+    over_chunks<true>(p, [&](auto zero, int k, int64_t at, int n) __attribute__((always_inline)) {
       using T = decltype(zero);
       constexpr int VEC = 16 / (int)sizeof(T);
       const T* const src = static_cast<const T*>(p.in[k]) + at;

@@ -4,6 +4,7 @@
 // autograd node.  It is C++ because a call's host time bounds the small ones: through ctypes and a Python autograd
 // function a layer norm of one row took 11 us, and a training step of a small one, whose kernels run for 25 us, 125 us.
 // No kernel is in this file, and the library itself does not depend on torch.
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
@@ -81,8 +82,12 @@ MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::
 
 bool tracks(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// Without the way through the dispatcher (a call that returns 48 tensors EMPTY_BEFORE -> EMPTY_AFTER us).
 Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(device));
+  return at::detail::empty_cuda(shape, type, device, std::nullopt);
+}
+Tensor empty_strided(at::IntArrayRef shape, at::IntArrayRef strides, at::ScalarType type, at::Device device) {
+  return at::detail::empty_strided_cuda(shape, strides, type, device);
 }
 
 // t with its values in its storage (torch may hold a real tensor as the storage's negative, as the imaginary part of a
@@ -772,7 +777,7 @@ std::tuple<std::vector<Tensor>, Tensor> clip_grad_norm(const std::vector<Tensor>
       }
     } else {
       in[i] = whole ? values(g) : dense(g);
-      out[i] = at::empty_like(in[i]), result[i] = out[i];
+      out[i] = empty_strided(in[i].sizes(), in[i].strides(), in[i].scalar_type(), device), result[i] = out[i];
     }
     src[i] = ptr(in[i]), dst[i] = ptr(out[i]), numel[i] = g.numel(), dtypes[i] = dtype_code(g.scalar_type());
   }
