@@ -452,50 +452,43 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
 
 // ---- one token ----------------------------------------------------------------------------------
 
-// SL threads per channel with four states each, for ROWS rows one after the other with the channel's decays in registers.
-constexpr int kNs = 4;
-template <typename T, int SL, int ROWS>
+// SL threads per channel with four states each.  Bound by the traffic of the states: 512 x 1024 x 16 bf16 16.8 us, 4.2
+// TB/s (a copy of the states 10.1).  (Two, four and eight rows per thread, which read A once for all of them: 18.5, 18.9 and
+// 31 us.)
+constexpr int kStepStates = 4;
+template <typename T, int SL, bool GATED>
 __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x, at = i / SL, rows = at / (uint32_t)p.D_;  // (less than 2^32 threads)
-  const int d = (int)(at % (uint32_t)p.D_), n0 = (int)(i % SL) * kNs, n = p.N - n0;
-  if ((int64_t)rows * ROWS >= p.batch) return;  // (whole groups of SL lanes)
-  float A[kNs];
+  constexpr int NS = kStepStates;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, at = i / SL;  // (less than 2^32 threads)
+  const int64_t b = at / (uint32_t)p.D_;
+  if (b >= p.batch) return;  // (whole groups of SL lanes)
+  const int d = (int)(at % (uint32_t)p.D_), n0 = (int)(i % SL) * NS, n = min(max(p.N - n0, 0), NS);
+  const int64_t state = (int64_t)at * p.N + n0;
+  Vec<float, NS> h = load_some<float, NS>(p.h0 + state, n), A;
+  const Vec<T, NS> B = load_some<T, NS>(static_cast<const T*>(p.B.p) + b * p.B.b + n0, n);
+  const Vec<T, NS> C = load_some<T, NS>(static_cast<const T*>(p.C.p) + b * p.C.b + n0, n);
+  const float u = (float)static_cast<const T*>(p.u.p)[b * p.u.b + d];
+  const float raw = (float)static_cast<const T*>(p.dt.p)[b * p.dt.b + d] + param<T>(p.bias, p.w32, d, 0.0f);
+  const float z = GATED ? (float)static_cast<const T*>(p.z.p)[b * p.z.b + d] : 0.0f;
+  const float skip = param<T>(p.D, p.w32, d, 0.0f);
+  if (p.w32) {
+    A = load_some<float, NS>(static_cast<const float*>(p.A) + (int64_t)d * p.N + n0, n);
+  } else {
+    const Vec<T, NS> v = load_some<T, NS>(static_cast<const T*>(p.A) + (int64_t)d * p.N + n0, n);
 #pragma unroll
-  for (int j = 0; j < kNs; ++j) A[j] = j < n ? kOpLog2e * param<T>(p.A, p.w32, (int64_t)d * p.N + n0 + j, 0.0f) : 0.0f;
-  const float bias = param<T>(p.bias, p.w32, d, 0.0f), skip = param<T>(p.D, p.w32, d, 0.0f);
-  Vec<float, kNs> h[ROWS];
-  Vec<T, kNs> B[ROWS], C[ROWS];
-  T u[ROWS], raw[ROWS], z[ROWS];
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int64_t b = (int64_t)rows * ROWS + r;
-    h[r] = {}, B[r] = {}, C[r] = {};
-    u[r] = raw[r] = z[r] = (T)0.0f;
-    if (b >= p.batch) continue;
-    u[r] = static_cast<const T*>(p.u.p)[b * p.u.b + d];
-    raw[r] = static_cast<const T*>(p.dt.p)[b * p.dt.b + d];
-    if (p.z.p) z[r] = static_cast<const T*>(p.z.p)[b * p.z.b + d];
-    if (n <= 0) continue;
-    h[r] = load_some<float, kNs>(p.h0 + (b * p.D_ + d) * p.N + n0, n);
-    B[r] = load_some<T, kNs>(static_cast<const T*>(p.B.p) + b * p.B.b + n0, n);
-    C[r] = load_some<T, kNs>(static_cast<const T*>(p.C.p) + b * p.C.b + n0, n);
+    for (int j = 0; j < NS; ++j) A.v[j] = (float)v.v[j];
   }
+  const float dt = p.softplus ? softplus(raw) : raw, du = dt * u;
+  float y = 0.0f;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int64_t b = (int64_t)rows * ROWS + r;
-    const float v = (float)raw[r] + bias, dt = p.softplus ? softplus(v) : v, du = dt * (float)u[r];
-    float y = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kNs; ++j) {
-      h[r].v[j] = fmaf(__builtin_amdgcn_exp2f(dt * A[j]), h[r].v[j], du * (float)B[r].v[j]);
-      if (j < n) y = fmaf((float)C[r].v[j], h[r].v[j], y);
-    }
-    y = fmaf(skip, (float)u[r], states_sum<SL>(y));
-    if (p.z.p) y *= silu((float)z[r]);
-    if (b >= p.batch) continue;
-    if (n > 0) store_some<float, kNs>(p.h_n + (b * p.D_ + d) * p.N + n0, h[r], n);
-    if (i % SL == 0) static_cast<T*>(p.out)[b * p.D_ + d] = round_to<T>(y);
+  for (int j = 0; j < NS; ++j) {
+    h.v[j] = fmaf(__builtin_amdgcn_exp2f(dt * (kOpLog2e * A.v[j])), h.v[j], du * (float)B.v[j]);
+    if (j < n) y = fmaf((float)C.v[j], h.v[j], y);
   }
+  y = fmaf(skip, u, states_sum<SL>(y));
+  if (GATED) y *= silu(z);
+  store_some<float, NS>(p.h_n + state, h, n);
+  if (i % SL == 0) static_cast<T*>(p.out)[at] = round_to<T>(y);
 }
 
 // ---- backward -----------------------------------------------------------------------------------
@@ -928,21 +921,20 @@ hipError_t launch_sel_forward(const SelArgs& p, hipStream_t s) {
 
 template <typename T>
 hipError_t launch_sel_step(const SelArgs& p, hipStream_t s) {
-  const auto lanes = [&](auto sl) {
-    constexpr int SL = decltype(sl)::value;
-    const auto run = [&](auto rows) {
-      constexpr int ROWS = decltype(rows)::value;
-      const dim3 grid((unsigned)(((p.batch + ROWS - 1) / ROWS * p.D_ * SL + 255) / 256));
-      hipLaunchKernelGGL((selective_step_kernel<T, SL, ROWS>), grid, dim3(256), 0, s, p);
-      return hipGetLastError();
-    };
-    return p.batch * p.D_ * SL >= 4 * 256 * 1024 ? run(std::integral_constant<int, 4>()) : run(std::integral_constant<int, 1>());
+  const auto run = [&](auto lanes) {
+    constexpr int SL = decltype(lanes)::value;
+    const dim3 grid((unsigned)((p.batch * p.D_ * SL + 255) / 256));
+    if (p.z.p)
+      hipLaunchKernelGGL((selective_step_kernel<T, SL, true>), grid, dim3(256), 0, s, p);
+    else
+      hipLaunchKernelGGL((selective_step_kernel<T, SL, false>), grid, dim3(256), 0, s, p);
+    return hipGetLastError();
   };
-  if (p.N <= 4) return lanes(std::integral_constant<int, 1>());
-  if (p.N <= 8) return lanes(std::integral_constant<int, 2>());
-  if (p.N <= 16) return lanes(std::integral_constant<int, 4>());
-  if (p.N <= 32) return lanes(std::integral_constant<int, 8>());
-  return lanes(std::integral_constant<int, 16>());
+  if (p.N <= 4) return run(std::integral_constant<int, 1>());
+  if (p.N <= 8) return run(std::integral_constant<int, 2>());
+  if (p.N <= 16) return run(std::integral_constant<int, 4>());
+  if (p.N <= 32) return run(std::integral_constant<int, 8>());
+  return run(std::integral_constant<int, 16>());
 }
 
 template <typename T>
