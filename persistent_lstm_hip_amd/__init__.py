@@ -1,4 +1,4 @@
-"""MI355X-native stacked LSTM + Linear inference forward, and the operators of a residual block around a
+"""MI355X-native stacked LSTM + Linear inference forward, and the operators of residual blocks around a
 recurrence that is parallel over time (gfx950 HIP kernels behind a C ABI).
 
 The LSTM's public surface mirrors mantuoluozk/persistent_lstm_hip's `persistent_lstm_hip` package
@@ -25,6 +25,7 @@ from .ops import (
     selective_scan,
     selective_scan_step,
 )
+from .selective import SelectiveScanBlock, SelectiveScanRegressor
 
 __all__ = [
     "PersistentLSTM",
@@ -39,6 +40,8 @@ __all__ = [
     "load_extension",
     "GatedScanBlock",
     "GatedScanRegressor",
+    "SelectiveScanBlock",
+    "SelectiveScanRegressor",
     "gated_scan",
     "gated_scan_step",
     "layer_norm",

@@ -76,13 +76,16 @@ class GatedScanRegressor(nn.Module):
     def __init__(self, input_dim: int, hidden_dim: int, output_dim: int, n_layers: int, dropout: float = 0.2):
         super().__init__()
         self.stem = nn.Linear(input_dim, hidden_dim)
-        self.blocks = nn.ModuleList(GatedScanBlock(hidden_dim, dropout) for _ in range(n_layers))
+        self.blocks = nn.ModuleList(self._block(hidden_dim, dropout) for _ in range(n_layers))
         self.norm_weight = nn.Parameter(torch.ones(hidden_dim))
         self.norm_bias = nn.Parameter(torch.zeros(hidden_dim))
         self.linear = nn.Linear(hidden_dim, output_dim)
         self.seed = int(torch.initial_seed())
         self._passes = 0  # training passes so far: every layer of every pass has a mask of its own
         self._numbers = {}  # of the last passes, by what they drew from torch's generator
+
+    def _block(self, dim: int, dropout: float) -> nn.Module:
+        return GatedScanBlock(dim, dropout)
 
     def _pass_number(self, device: torch.device) -> Union[int, torch.Tensor]:
         drawn = _draw(device)

@@ -1,17 +1,20 @@
-"""Trains a GatedScanRegressor on synthetic series, then serves it step by step.
+"""Trains a GatedScanRegressor or a SelectiveScanRegressor on synthetic series, then serves it step by step.
 
-    python -m persistent_lstm_hip_amd.gated_demo [--hidden 128 --layers 4 --batch 128 --seq-len 1000 --steps 100]
+    python -m persistent_lstm_hip_amd.gated_demo [--block gated|selective --hidden 128 --layers 4 --batch 128
+                                                  --seq-len 1000 --steps 100 --clip 1.0]
 """
 from __future__ import annotations
 
 import argparse
 import time
-from typing import List
+from typing import List, Optional
 
 import torch
 import torch.nn.functional as F
 
 from .gated import GatedScanRegressor
+from .ops import clip_grad_norm
+from .selective import SelectiveScanRegressor
 
 
 def _series(batch: int, steps: int, ahead: int, device, gen: torch.Generator):
@@ -25,8 +28,8 @@ def _series(batch: int, steps: int, ahead: int, device, gen: torch.Generator):
 
 
 def train(model: GatedScanRegressor, *, batch: int, seq_len: int, steps: int, lr: float = 2e-3, seed: int = 1,
-          report=None) -> List[float]:
-    """`steps` optimizer steps on synthetic series; the losses."""
+          report=None, clip: Optional[float] = None) -> List[float]:
+    """`steps` optimizer steps on synthetic series, with the gradients' global norm held at `clip`; the losses."""
     gen = torch.Generator(device="cuda").manual_seed(seed)
     opt = torch.optim.AdamW(model.parameters(), lr=lr)
     dtype, losses = model.linear.weight.dtype, []
@@ -36,6 +39,8 @@ def train(model: GatedScanRegressor, *, batch: int, seq_len: int, steps: int, lr
         loss = F.mse_loss(model(x.to(dtype)).float(), want)
         opt.zero_grad(set_to_none=True)
         loss.backward()
+        if clip is not None:
+            clip_grad_norm([p.grad for p in model.parameters()], clip, inplace=True)
         opt.step()
         losses.append(loss.detach())
         if report and (i + 1) % report == 0:
@@ -44,7 +49,9 @@ def train(model: GatedScanRegressor, *, batch: int, seq_len: int, steps: int, lr
 
 
 def main() -> None:
-    ap = argparse.ArgumentParser(description="Train a gated-scan forecaster on synthetic series and serve it.")
+    ap = argparse.ArgumentParser(description="Train a forecaster on synthetic series and serve it.")
+    ap.add_argument("--block", choices=("gated", "selective"), default="gated")
+    ap.add_argument("--clip", type=float, default=None, help="hold the gradients' global norm at this")
     ap.add_argument("--hidden", type=int, default=128)
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--batch", type=int, default=128)
@@ -52,9 +59,10 @@ def main() -> None:
     ap.add_argument("--steps", type=int, default=100)
     a = ap.parse_args()
     torch.manual_seed(42)
-    model = GatedScanRegressor(1, a.hidden, 24, a.layers, dropout=0.05).to("cuda")
+    kind = SelectiveScanRegressor if a.block == "selective" else GatedScanRegressor
+    model = kind(1, a.hidden, 24, a.layers, dropout=0.05).to("cuda")
     t0 = time.perf_counter()
-    losses = train(model, batch=a.batch, seq_len=a.seq_len, steps=a.steps, report=max(1, a.steps // 5))
+    losses = train(model, batch=a.batch, seq_len=a.seq_len, steps=a.steps, report=max(1, a.steps // 5), clip=a.clip)
     print(f"{a.steps} steps of {a.batch} x {a.seq_len}: {1e3 * (time.perf_counter() - t0) / a.steps:.2f} ms each, "
           f"loss {losses[0]:.4f} -> {losses[-1]:.4f}")
     model.eval()
