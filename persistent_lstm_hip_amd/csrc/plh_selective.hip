@@ -79,6 +79,11 @@ struct Geo {
   // channels and F neighbouring states each.
   static constexpr int E = GROUP >= 8 ? GROUP / 8 : 1, F = NP >= 8 ? NP / 8 : 1;
   static_assert(kRun == 8, "eight steps by eight lanes");
+  // Groups of a workgroup of the backward pass, whose dB and dC it adds up.  One leaves three workgroups per CU, with rows of
+  // their own pace, two save half of the partial sums' traffic, which grows with the states: 16 states 8 x 2048 x 2048 bf16
+  // 772 and 758 us with the sums' kernel, 128 x 1000 x 256 fp16 ragged 479 and 581; 32 states 4 x 2048 x 1024 bf16 467 and
+  // 415, 64 states 998 and 954.
+  static constexpr int SIDE = SL == 4 ? 1 : 2;
 };
 
 // Orders the LDS accesses of a wave's lanes among each other (they run in order; this is for the compiler).
@@ -493,7 +498,6 @@ __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
 
 // ---- backward -----------------------------------------------------------------------------------
 
-constexpr int kSide = 2;  // groups of channels of a workgroup, whose dB and dC it adds up
 
 template <typename G>
 struct BackLds {
@@ -506,23 +510,23 @@ struct BackLds {
 
 // The tiles of a segment from the last to the first.  MAPS: only the segment's map of E is wanted.
 template <typename T, typename G, Mode MODE, bool GATED>
-__global__ void __launch_bounds__(kSide* kWaves* kWave, kSide) selective_backward_kernel(SelArgs p) {
-  constexpr int E = G::E, SL = G::SL, NS = G::NS;
-  __shared__ BackLds<G> lds_all[kSide][kWaves];
-  __shared__ MapLds<G> maps[kSide][kWaves][3];
+__global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) selective_backward_kernel(SelArgs p) {
+  constexpr int SIDE = G::SIDE, E = G::E, SL = G::SL, NS = G::NS;
+  __shared__ BackLds<G> lds_all[SIDE][kWaves];
+  __shared__ MapLds<G> maps[SIDE][kWaves][3];
   const int lane = threadIdx.x % kWave, id = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wave = id % kWaves, side = id / kWaves;
   BackLds<G>& back = lds_all[side][wave];
   WaveLds<G>& lds = back.f;
   const int seg = blockIdx.y;
   const int64_t slab = slab_of(blockIdx.x, gridDim.x);
-  // A row's groups are taken kSide at a time; of rows of one group each, kSide rows.
-  const bool side_rows = p.groups == 1;
-  const int per_row = (p.groups + kSide - 1) / kSide;
-  const int64_t b_of = side_rows ? slab * kSide + side : slab / per_row;
-  const int group = side_rows ? 0 : (int)(slab % per_row) * kSide + side;
+  // A row's groups are taken SIDE at a time; of rows of one group each, SIDE rows.
+  const bool side_rows = p.groups == 1, alone = SIDE == 1 || side_rows;  // alone: no other group's dB and dC to add
+  const int per_row = (p.groups + SIDE - 1) / SIDE;
+  const int64_t b_of = side_rows ? slab * SIDE + side : slab / per_row;
+  const int group = side_rows ? 0 : (int)(slab % per_row) * SIDE + side;
   const bool on = b_of < p.batch && group < p.groups;
-  const int sides = side_rows ? 1 : p.groups - (group - side);  // that have a group, where they share a row
+  const int sides = alone ? 1 : p.groups - (group - side);  // that have a group, where they share a row
   const At at = place(p, on ? b_of * p.groups + group : p.units, G::GROUP);
   const Slots<G> mine(p, at, lane);
   const int64_t state_size = p.batch * p.D_ * p.N;
@@ -549,7 +553,7 @@ __global__ void __launch_bounds__(kSide* kWaves* kWave, kSide) selective_backwar
   const int row_len = length(b_of);  // (also of a wave without a group: it adds up its row's dB and dC)
   int most = row_len;  // the same in all waves
   if (side_rows)
-    for (int i = 0; i < kSide; ++i) most = max(most, length(slab * kSide + i));
+    for (int i = 0; i < SIDE; ++i) most = max(most, length(slab * SIDE + i));
   const int live = (most + kTileSteps - 1) / kTileSteps;
   const int first = seg * p.seg_tiles, last = min(first + p.seg_tiles, p.tiles), live_last = min(last, live);
   float carry[NS], decay[NS], dA[NS];
@@ -589,12 +593,12 @@ __global__ void __launch_bounds__(kSide* kWaves* kWave, kSide) selective_backwar
     const auto put = [&](int k, const Fs<G::F>& v) __attribute__((always_inline)) {
       store_some<float, G::F>(dst + k * p.N, __builtin_bit_cast(FVec<G::F>, v), f_states);
     };
-    if (side_rows) {
+    if (alone) {
       put(0, of(side, 0)), put(1, of(side, 1));
     } else if (side < 2) {  // a row's sums: dB by the first side's waves, dC by the second one's
       Fs<G::F> v = of(0, side);
 #pragma unroll
-      for (int i = 1; i < kSide; ++i) {
+      for (int i = 1; i < SIDE; ++i) {
         if (i >= sides) break;
         const Fs<G::F> other = of(i, side);
 #pragma unroll
@@ -864,24 +868,26 @@ struct SelLayout {
 };
 
 // With few workgroups the time axis is split into segments, whose maps a launch of its own computes first (about half of
-// the work again).  Forward four workgroups fill a CU, backward one.  Measured, us of a call without and with about 1024
-// (backward 256) workgroups of 16 states bf16 with a gate:
+// the work again).  Workgroups that fill the device, at as many registers as they take: 1024 forward, 768 backward (256 with
+// two groups each).  Measured, us of a call without and with about that many, 16 states bf16 with a gate:
 //   forward   64 workgroups (2 x 4096 x 512) 264 and 58, 80 (1 x 16384 x 1280) 1177 and 284, 128 (1 x 2048 x 2048)
 //             134 and 58, 256 (4 x 2048 x 1024) 153 and 99; 512 (4 x 2048 x 2048) 162, in two segments 174
-//   backward  32 (2 x 4096 x 512) 709 and 136, 40 (1 x 16384 x 1280) 2938 and 668, 128 (4 x 2048 x 1024) 353 and 242;
-//             256 (4 x 2048 x 2048) 397, in two segments 488
+//   backward  64 594 and 122, 80 2483 and 616, 128 316 and 132, 256 312 and 209; 512 427, in two segments 487
 SelLayout sel_layout(int64_t batch, int64_t seq_len, int64_t channels, int states, bool backward) {
   SelLayout l;
-  const int per = with_states(states, [](auto sl, auto ns) {
-    return Geo<decltype(sl)::value, decltype(ns)::value>::GROUP;
+  int per = 0, side = 0;
+  with_states(states, [&](auto sl, auto ns) {
+    using G = Geo<decltype(sl)::value, decltype(ns)::value>;
+    per = G::GROUP, side = G::SIDE;
   });
   l.groups = (int)((channels + per - 1) / per);
-  l.bc_groups = (l.groups + kSide - 1) / kSide;
+  l.bc_groups = (l.groups + side - 1) / side;
   l.tiles = (int)((seq_len + kTileSteps - 1) / kTileSteps);
-  const int64_t units = batch * l.groups, slabs = l.groups == 1 ? (batch + kSide - 1) / kSide : batch * l.bc_groups;
+  const int64_t units = batch * l.groups, slabs = l.groups == 1 ? (batch + side - 1) / side : batch * l.bc_groups;
   const int64_t groups = std::max<int64_t>(1, backward ? slabs : units);  // of workgroups
+  const int64_t fill = backward ? side == 1 ? 768 : 256 : 1024, most = backward ? fill / 2 : 400;
+  const int64_t want = groups > most ? 1 : fill / groups;
   // (no segment shorter than two tiles: a short one's start costs as much as its steps)
-  const int64_t most = backward ? 200 : 400, want = groups > most ? 1 : (backward ? 256 : 1024) / groups;
   l.seg_tiles = (int)std::max<int64_t>(std::max(1, std::min(2, l.tiles)), (l.tiles + want - 1) / want);
   l.segs = std::max(1, (l.tiles + l.seg_tiles - 1) / l.seg_tiles);
   return l;
@@ -941,10 +947,10 @@ template <typename T>
 hipError_t launch_sel_backward(SelArgs p, void* d_A, void* d_B, void* d_C, void* d_D, void* d_bias, hipStream_t s) {
   hipError_t e = hipSuccess;
   if (p.batch > 0) {
-    const int64_t slabs = p.groups == 1 ? (p.batch + kSide - 1) / kSide : p.batch * ((p.groups + kSide - 1) / kSide);
     e = with_states(p.N, [&](auto sl, auto ns) {
       using G = Geo<decltype(sl)::value, decltype(ns)::value>;
-      const dim3 grid((unsigned)slabs, p.segs), block(kSide * kWaves * kWave);
+      const int64_t slabs = p.groups == 1 ? (p.batch + G::SIDE - 1) / G::SIDE : p.batch * p.bc_groups;
+      const dim3 grid((unsigned)slabs, p.segs), block(G::SIDE * kWaves * kWave);
       const auto run = [&](auto gated) {
         constexpr bool GATED = decltype(gated)::value;
         if (p.segs > 1) {
