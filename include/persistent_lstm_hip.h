@@ -316,7 +316,7 @@ int plh_dropout_add(int dtype, const void* x, const void* residual, void* out, i
  *   state_n       [batch][width - 1][channels]: the last width - 1 inputs of every row (of its state, where it is shorter);
  *                 not the memory of state
  * The step takes one input per row and a state; its state_n may be state (in place).
- * Limits: channels <= 2^24, batch * channels <= 2^28, batch * channels * seq_len <= 2^35.
+ * Limits: channels <= 2^22, seq_len <= 2^30, batch * channels <= 2^28, batch * channels * seq_len <= 2^35.
  */
 int plh_causal_conv_forward(int dtype, int wdtype, const void* x, int64_t stride_b, int64_t stride_t, int64_t batch,
                             int64_t seq_len, int64_t channels, int width, const void* weight, const void* bias,
@@ -351,8 +351,8 @@ int plh_causal_conv_backward(int dtype, int wdtype, const void* x, int64_t strid
  *   states_out     device fp32 [plh_selective_scan_states(seq_len)][batch][channels][states] or NULL: what the backward
  *                  pass needs
  * The step is seq_len = 1 without lengths, from h to h_n, which may be the same memory.
- * Limits: 1 <= states <= 64, channels <= 2^24, seq_len <= 2^30, batch * ceil(channels / 8) <= 2^23,
- * batch * seq_len * states <= 2^30.
+ * Limits: 1 <= states <= 64, channels <= 2^20, seq_len <= 2^30, batch * ceil(channels / 8) <= 2^21,
+ * batch * seq_len * states <= 2^30; of the step batch <= 2^30, batch * channels * states <= 2^32.
  */
 typedef struct plh_selective_scan_args {
   int dtype, wdtype;

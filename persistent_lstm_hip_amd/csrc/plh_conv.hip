@@ -475,7 +475,7 @@ int check_conv(const char* what, int dtype, int wdtype, const void* x, int64_t s
   if (wdtype != dtype && wdtype != PLH_F32) return op_error(PLH_ERR_INVALID, what, "wdtype must be dtype or PLH_F32");
   if (batch < 0 || seq_len < 0) return op_error(PLH_ERR_INVALID, what, "batch and seq_len must be non-negative");
   if (width < 1 || width > kMaxWidth) return op_error(PLH_ERR_UNSUPPORTED, what, "width must lie in [1, 8]");
-  if (channels < 1 || channels > (1 << 24)) return op_error(PLH_ERR_UNSUPPORTED, what, "channels must lie in [1, 2^24]");
+  if (channels < 1 || channels > (1 << 22)) return op_error(PLH_ERR_UNSUPPORTED, what, "channels must lie in [1, 2^22]");
   if (seq_len > (1 << 30)) return op_error(PLH_ERR_UNSUPPORTED, what, "seq_len must not exceed 2^30");
   if (batch > (1 << 28) || batch * channels > (1 << 28) ||
       (seq_len > 0 && batch * channels > (int64_t(1) << 35) / seq_len))
@@ -503,7 +503,7 @@ ConvArgs conv_args(int wdtype, const void* x, int64_t stride_b, int64_t stride_t
 extern "C" {
 
 int64_t plh_causal_conv_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int width) {
-  if (batch < 0 || seq_len < 0 || seq_len > (1 << 30) || channels < 1 || channels > (1 << 24) || width < 1 ||
+  if (batch < 0 || seq_len < 0 || seq_len > (1 << 30) || channels < 1 || channels > (1 << 22) || width < 1 ||
       width > plh::kMaxWidth)
     return -1;
   return plh::conv_layout(batch, seq_len, channels).groups * channels * (width + 1) * (int64_t)sizeof(float);

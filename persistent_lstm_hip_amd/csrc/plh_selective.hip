@@ -150,6 +150,10 @@ __device__ __forceinline__ void softplus(float v, float& value, float& slope) {
   slope = v < 0.0f ? e * r : r;
 }
 
+// A decay's rate, times log2 e.  Minus infinity becomes the largest finite one: a step of size zero, as past a row's end,
+// leaves the state as it is, and 0 * inf would not.
+__device__ __forceinline__ float rate(float A) { return __builtin_elementwise_maximum(A * kOpLog2e, -3e38f); }
+
 // The decay of a run of steps.  Every step's own is positive; their product may underflow (or, of a growing state,
 // overflow), and 0 * inf would be NaN where the steps one after the other are not.
 __device__ __forceinline__ float run_decay(float log2_decay) {
@@ -259,7 +263,7 @@ struct Slots {
   __device__ __forceinline__ void rates(const SelArgs& p, float (&v)[G::NS]) const {
 #pragma unroll
     for (int j = 0; j < G::NS; ++j)
-      v[j] = j < states ? kOpLog2e * param<T>(p.A, p.w32, (int64_t)c * p.N + n + j, 0.0f) : 0.0f;
+      v[j] = j < states ? rate(param<T>(p.A, p.w32, (int64_t)c * p.N + n + j, 0.0f)) : 0.0f;
   }
 };
 
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
   float y = 0.0f;
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    h.v[j] = fmaf(__builtin_amdgcn_exp2f(dt * (kOpLog2e * A.v[j])), h.v[j], du * (float)B.v[j]);
+    h.v[j] = fmaf(__builtin_amdgcn_exp2f(dt * rate(A.v[j])), h.v[j], du * (float)B.v[j]);
     if (j < n) y = fmaf((float)C.v[j], h.v[j], y);
   }
   y = fmaf(skip, u, states_sum<SL>(y));
@@ -979,7 +983,7 @@ hipError_t launch_sel_backward(SelArgs p, void* d_A, void* d_B, void* d_C, void*
   return e;
 }
 
-int check_selective(const char* what, const plh_selective_scan_args* a) noexcept {
+int check_selective(const char* what, const plh_selective_scan_args* a, bool step) noexcept {
   if (!a) return op_error(PLH_ERR_INVALID, what, "args is required");
   if (a->dtype != PLH_F16 && a->dtype != PLH_BF16 && a->dtype != PLH_F32)
     return op_error(PLH_ERR_INVALID, what, "dtype must be PLH_F16, PLH_BF16 or PLH_F32");
@@ -987,12 +991,15 @@ int check_selective(const char* what, const plh_selective_scan_args* a) noexcept
     return op_error(PLH_ERR_INVALID, what, "wdtype must be dtype or PLH_F32");
   if (a->batch < 0 || a->seq_len < 0) return op_error(PLH_ERR_INVALID, what, "batch and seq_len must be non-negative");
   if (a->states < 1 || a->states > kMaxStates) return op_error(PLH_ERR_UNSUPPORTED, what, "states must lie in [1, 64]");
-  if (a->channels < 1 || a->channels > (1 << 24))
-    return op_error(PLH_ERR_UNSUPPORTED, what, "channels must lie in [1, 2^24]");
+  if (a->channels < 1 || a->channels > (1 << 20))
+    return op_error(PLH_ERR_UNSUPPORTED, what, "channels must lie in [1, 2^20]");
   if (a->seq_len > (1 << 30)) return op_error(PLH_ERR_UNSUPPORTED, what, "seq_len must not exceed 2^30");
-  if (a->batch > (1 << 23) || a->batch * ((a->channels + 7) / 8) > (1 << 23))
-    return op_error(PLH_ERR_UNSUPPORTED, what, "batch * ceil(channels / 8) must not exceed 2^23");
-  if (a->batch * a->seq_len * a->states > (1 << 30))
+  // (what a grid of workgroups holds)
+  if (step && (a->batch > (1 << 30) || a->batch * a->channels * a->states > (int64_t(1) << 32)))
+    return op_error(PLH_ERR_UNSUPPORTED, what, "batch * channels * states must not exceed 2^32");
+  if (!step && (a->batch > (1 << 21) || a->batch * ((a->channels + 7) / 8) > (1 << 21)))
+    return op_error(PLH_ERR_UNSUPPORTED, what, "batch * ceil(channels / 8) must not exceed 2^21");
+  if (!step && a->batch * a->seq_len * a->states > (1 << 30))
     return op_error(PLH_ERR_UNSUPPORTED, what, "batch * seq_len * states must not exceed 2^30");
   if (!a->A) return op_error(PLH_ERR_INVALID, what, "A is required");
   if (a->batch > 0 && a->seq_len > 0 && (!a->u || !a->dt || !a->B || !a->C))
@@ -1025,7 +1032,7 @@ int64_t plh_selective_scan_states(int64_t seq_len) {
 }
 
 int64_t plh_selective_scan_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int states, int backward) {
-  if (batch < 0 || seq_len < 0 || seq_len > (1 << 30) || channels < 1 || channels > (1 << 24) || states < 1 ||
+  if (batch < 0 || seq_len < 0 || seq_len > (1 << 30) || channels < 1 || channels > (1 << 20) || states < 1 ||
       states > plh::kMaxStates)
     return -1;
   return plh::sel_workspace(batch, seq_len, channels, states, backward != 0).bytes;
@@ -1034,7 +1041,7 @@ int64_t plh_selective_scan_workspace_bytes(int64_t batch, int64_t seq_len, int64
 int plh_selective_scan_forward(const plh_selective_scan_args* a, const float* h0, void* out, float* h_n, float* states,
                                void* workspace, int64_t workspace_bytes, void* stream) {
   const char* const what = "selective_scan_forward";
-  const int rc = plh::check_selective(what, a);
+  const int rc = plh::check_selective(what, a, false);
   if (rc != PLH_OK) return rc;
   if (a->batch == 0) return PLH_OK;
   if (a->seq_len > 0 && !out) return plh::op_error(PLH_ERR_INVALID, what, "out is required");
@@ -1051,7 +1058,7 @@ int plh_selective_scan_forward(const plh_selective_scan_args* a, const float* h0
 
 int plh_selective_scan_step(const plh_selective_scan_args* a, const float* h, void* out, float* h_n, void* stream) {
   const char* const what = "selective_scan_step";
-  const int rc = plh::check_selective(what, a);
+  const int rc = plh::check_selective(what, a, true);
   if (rc != PLH_OK) return rc;
   if (a->seq_len != 1) return plh::op_error(PLH_ERR_INVALID, what, "seq_len must be 1");
   if (a->lengths) return plh::op_error(PLH_ERR_INVALID, what, "a step has no lengths");
@@ -1068,7 +1075,7 @@ int plh_selective_scan_backward(const plh_selective_scan_args* a, const float* s
                                 const float* d_hn, const plh_selective_scan_grads* g, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
   const char* const what = "selective_scan_backward";
-  const int rc = plh::check_selective(what, a);
+  const int rc = plh::check_selective(what, a, false);
   if (rc != PLH_OK) return rc;
   if (!g) return plh::op_error(PLH_ERR_INVALID, what, "grads is required");
   if (a->batch > 0 && a->seq_len > 0 && (!states || !d_out || !g->d_u || !g->d_dt || (a->z && !g->d_z)))

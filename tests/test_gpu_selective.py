@@ -206,6 +206,27 @@ def test_a_closed_gate_and_step(gpu, low):
         assert torch.equal(h_n, h4)
 
 
+def test_a_state_that_decays_at_once(gpu):
+    """A rate of minus infinity: a state of the last input alone, kept past a row's end; no NaN, gradients included."""
+    _say("selective scan rate")
+    d = _inputs(2, 40, 9, 16, F32)
+    d["A"][4, 3] = float("-inf")
+    dev = {name: t.cuda().requires_grad_(True) for name, t in d.items()}
+    out, h_n = _call(dev, lengths=[40, 13])
+    grads = torch.autograd.grad((out, h_n), [dev[n] for n in LEAVES], (torch.ones_like(out), torch.ones_like(h_n)))
+    assert all(bool(torch.isfinite(t).all()) for t in (out, h_n, *grads))
+    e = {**d, "A": d["A"].clamp(min=-1e6)}  # (decays within one step of any size that occurs here)
+    want = plain.scan(*(e[n] for n in LEAVES), lengths=[40, 13])
+    assert_within(out, *want["out"], F32, "out")
+    assert_within(h_n, *want["h_n"], F32, "h_n")
+    one = {n: t.detach()[:, 0] if n in ("u", "dt", "B", "C", "z") else t.detach() for n, t in dev.items()}
+    out, h = P.selective_scan_step(one["u"], one["dt"], one["A"], one["B"], one["C"], one["h0"], one["D"], one["z"],
+                                   dt_bias=one["dt_bias"])
+    first = {n: t.detach()[:, :1] if n in ("u", "dt", "B", "C", "z") else t.detach() for n, t in dev.items()}
+    want = _call(first)
+    assert (out - want[0][:, 0]).abs().max() < 1e-4 and (h - want[1]).abs().max() < 1e-4
+
+
 def test_strides_and_alignments(gpu):
     """Parts of one projection's output, a time-major one, an odd offset, an expanded row, a channel-strided tensor."""
     _say("selective scan strides")

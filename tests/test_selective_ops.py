@@ -149,7 +149,7 @@ def test_conv_refusals(lib):
     assert fwd(wdtype=1) == PLH_ERR_INVALID and b"wdtype" in lib.plh_last_error()
     assert fwd(B=-1) == PLH_ERR_INVALID and fwd(T=-1) == PLH_ERR_INVALID
     assert fwd(W=0) == PLH_ERR_UNSUPPORTED and fwd(W=9) == PLH_ERR_UNSUPPORTED and b"width" in lib.plh_last_error()
-    assert fwd(C=0) == PLH_ERR_UNSUPPORTED and fwd(C=(1 << 24) + 1) == PLH_ERR_UNSUPPORTED
+    assert fwd(C=0) == PLH_ERR_UNSUPPORTED and fwd(C=(1 << 22) + 1) == PLH_ERR_UNSUPPORTED
     assert fwd(T=(1 << 30) + 1) == PLH_ERR_UNSUPPORTED
     assert fwd(B=1 << 26) == PLH_ERR_UNSUPPORTED and b"batch" in lib.plh_last_error()
     assert fwd(T=1 << 30, B=8) == PLH_ERR_UNSUPPORTED
@@ -210,8 +210,9 @@ def test_scan_refusals(lib):
         assert call(wdtype=1) == PLH_ERR_INVALID and b"wdtype" in lib.plh_last_error()
         assert call(batch=-1) == PLH_ERR_INVALID
         assert call(states=0) == PLH_ERR_UNSUPPORTED if call is not back else True
-        assert call(channels=0) == PLH_ERR_UNSUPPORTED and call(channels=(1 << 24) + 1) == PLH_ERR_UNSUPPORTED
-        assert call(batch=1 << 23, channels=9) == PLH_ERR_UNSUPPORTED and b"2^23" in lib.plh_last_error()
+        assert call(channels=0) == PLH_ERR_UNSUPPORTED and call(channels=(1 << 20) + 1) == PLH_ERR_UNSUPPORTED
+        if call is not step:
+            assert call(batch=1 << 21, channels=9) == PLH_ERR_UNSUPPORTED and b"2^21" in lib.plh_last_error()
         for name in ("u", "dt", "B", "C", "A"):
             assert call(**{name: None}) == PLH_ERR_INVALID, name
         for name in ("u", "dt", "z", "B", "C"):
@@ -221,6 +222,7 @@ def test_scan_refusals(lib):
     assert fwd(seq_len=(1 << 30) + 1) == PLH_ERR_UNSUPPORTED and fwd(seq_len=1 << 30) == PLH_ERR_UNSUPPORTED
     assert fwd(out=None) == PLH_ERR_INVALID and fwd(batch=0) == PLH_OK
     assert lib.plh_selective_scan_forward(None, None, ANY, None, None, None, 0, None) == PLH_ERR_INVALID
+    assert step(batch=1 << 24, channels=1 << 10) == PLH_ERR_UNSUPPORTED and b"2^32" in lib.plh_last_error()
     assert step(seq_len=2) == PLH_ERR_INVALID and step(lengths=256) == PLH_ERR_INVALID
     assert step(h=None) == PLH_ERR_INVALID and step(out=None) == PLH_ERR_INVALID and step(h_n=None) == PLH_ERR_INVALID
     assert back(states=None) == PLH_ERR_INVALID and back(d_out=None) == PLH_ERR_INVALID
