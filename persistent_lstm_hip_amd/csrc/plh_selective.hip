@@ -307,12 +307,38 @@ struct TileIn {
   }
 };
 
-// ---- forward ------------------------------------------------------------------------------------
-
 enum Mode { kWhole, kMaps };
 
+// The map of a segment from its waves' maps, from the first to the last, or back.
+template <typename G, bool BACK>
+__device__ __forceinline__ void store_segment(const SelArgs& p, const Slots<G>& mine, const At& at, int seg, int lane,
+                                              int wave, MapLds<G>* maps, const float (&decay)[G::NS],
+                                              const float (&sum)[G::NS]) {
+  maps[wave * 2].put(lane, decay);
+  maps[wave * 2 + 1].put(lane, sum);
+  lds_barrier();
+  if (wave != 0) return;
+  float P[G::NS], Q[G::NS];
+#pragma unroll
+  for (int i = 0; i < G::NS; ++i) P[i] = 1.0f, Q[i] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    const int w = BACK ? kWaves - 1 - k : k;
+    float Pw[G::NS], Qw[G::NS];
+    maps[w * 2].get(lane, Pw);
+    maps[w * 2 + 1].get(lane, Qw);
+#pragma unroll
+    for (int i = 0; i < G::NS; ++i) Q[i] = fmaf(Pw[i], Q[i], Qw[i]), P[i] = fmaxf(P[i] * Pw[i], 0x1p-126f);
+  }
+  float* const dst = p.seg + (int64_t)seg * 2 * p.batch * p.D_ * p.N;
+  mine.store(p, dst, at.b, P);
+  mine.store(p, dst + p.batch * p.D_ * p.N, at.b, Q);
+}
+
+// ---- forward ------------------------------------------------------------------------------------
+
 // A workgroup carries a group of channels through a segment of time, a tile of four waves by eight steps at a time.  MAPS:
-// only the segment's map is wanted.
+// only the segment's map is wanted; every wave then runs a quarter of the segment by itself, and their maps meet at the end.
 template <typename T, typename G, Mode MODE, bool GATED>
 __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArgs p) {
   constexpr int E = G::E, SL = G::SL, NS = G::NS;
@@ -352,9 +378,12 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     }
   }
 
-  int t = first * kTileSteps + wave * kRun + row;  // the lane's step
+  constexpr int kNext = MODE == kMaps ? kRun : kTileSteps;  // steps between a wave's runs
+  const int start = MODE == kMaps ? (first * kWaves + wave * (last - first)) * kRun : first * kTileSteps + wave * kRun;
+  const int runs = MODE == kMaps ? min(max((at.len - start + kRun - 1) / kRun, 0), last - first) : live_last - first;
+  int t = start + row;  // the lane's step
   TileIn<T, G> next;
-  next.place(p, at, t, c, n, lane, kTileSteps);
+  next.place(p, at, t, c, n, lane, kNext);
   const auto load = [&](int t) __attribute__((always_inline)) {
     const bool on = t < at.len;
     next.u.load(on), next.dt.load(on), next.B.load(on);
@@ -365,8 +394,9 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
   };
   T* out = static_cast<T*>(p.out) + (at.b * p.T_ + t) * p.D_ + c;
   const int64_t out_step = (int64_t)kTileSteps * p.D_;
-  if (first < live_last) load(t);
-  for (int tile = first; tile < live_last; ++tile, t += kTileSteps, out += out_step) {
+  if (runs > 0) load(t);
+  for (int run = 0; run < runs; ++run, t += kNext, out += out_step) {
+    const int tile = first + run;
     // dt and dt u, B, C: into the wave's LDS
     const Vec<T, E> u = next.u.v, z = next.z.v;
     if (G::GROUP >= 8 || ec < G::GROUP) {
@@ -379,12 +409,12 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
       *reinterpret_cast<Fs<2 * E>*>(&lds.step[row][ec]) = f;
     }
     next.put_coefs(lds, lane);
-    if (tile + 1 < live_last) load(t + kTileSteps);
+    if (run + 1 < runs) load(t + kNext);
     wave_sync();
     // 1. decays and the run's map
     float a[kRun][NS], Q[NS], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) Q[i] = 0.0f;
+    for (int i = 0; i < NS; ++i) Q[i] = MODE == kMaps ? carry[i] : 0.0f;
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
       const Fs<2> s = lds.step[r][lane / SL];
@@ -400,10 +430,16 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     float P[NS], h[NS] = {};
 #pragma unroll
     for (int i = 0; i < NS; ++i) P[i] = run_decay(sum * A[i]);
+    if (MODE == kMaps) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) carry[i] = Q[i], decay[i] = fmaxf(decay[i] * P[i], 0x1p-126f);
+      wave_sync();
+      continue;
+    }
     MapLds<G>(*const map)[2] = maps[tile & 1];
     map[wave][0].put(lane, P);
     map[wave][1].put(lane, Q);
-    if (MODE == kWhole && p.states && wave == 0) mine.store(p, p.states + tile * state_size, at.b, carry);
+    if (p.states && wave == 0) mine.store(p, p.states + tile * state_size, at.b, carry);
     lds_barrier();
     // (selects, not branches: the maps are then read one after the other without a wait)
 #pragma unroll
@@ -415,10 +451,8 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
       for (int i = 0; i < NS; ++i) {
         h[i] = w == wave ? carry[i] : h[i];
         carry[i] = fmaf(Pw[i], carry[i], Qw[i]);
-        if (MODE == kMaps) decay[i] = fmaxf(decay[i] * Pw[i], 0x1p-126f);
       }
     }
-    if (MODE == kMaps) continue;
     // 3. the steps from where they start
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
@@ -447,10 +481,7 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     wave_sync();
   }
   if (MODE == kMaps) {
-    if (wave == 0) {
-      mine.store(p, p.seg + (int64_t)seg * 2 * state_size, at.b, decay);
-      mine.store(p, p.seg + (int64_t)(seg * 2 + 1) * state_size, at.b, carry);
-    }
+    store_segment<G, false>(p, mine, at, seg, lane, wave, maps[0][0], decay, carry);
     return;
   }
   for (int tile = max(first, live_last); tile < last; ++tile, t += kTileSteps, out += out_step)  // past the row
@@ -512,7 +543,7 @@ struct BackLds {
   Fs<G::E> kept[kKept][64];
 };
 
-// The tiles of a segment from the last to the first.  MAPS: only the segment's map of E is wanted.
+// The tiles of a segment from the last to the first.  MAPS: only the segment's map of E is wanted, as above.
 template <typename T, typename G, Mode MODE, bool GATED>
 __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) selective_backward_kernel(SelArgs p) {
   constexpr int SIDE = G::SIDE, E = G::E, SL = G::SL, NS = G::NS;
@@ -574,11 +605,14 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
     }
   }
 
-  int t = (live_last - 1) * kTileSteps + wave * kRun + row;  // the lane's step
+  constexpr int kNext = MODE == kMaps ? kRun : kTileSteps;  // steps between a wave's runs
+  const int start = MODE == kMaps ? (first * kWaves + wave * (last - first)) * kRun : first * kTileSteps + wave * kRun;
+  const int runs = MODE == kMaps ? min(max((at.len - start + kRun - 1) / kRun, 0), last - first) : live_last - first;
+  int t = start + (runs - 1) * kNext + row;  // the lane's step
   TileIn<T, G> next;
   Rows<T, E> next_g;
-  next.place(p, at, t, c, n, lane, -kTileSteps);
-  next_g.place(Strided{p.d_out, (int64_t)p.T_ * p.D_, p.D_}, at.b, t, c, n, -kTileSteps);
+  next.place(p, at, t, c, n, lane, -kNext);
+  next_g.place(Strided{p.d_out, (int64_t)p.T_ * p.D_, p.D_}, at.b, t, c, n, -kNext);
   const auto load = [&](int t) __attribute__((always_inline)) {
     const bool on = t < at.len;
     next_g.load(on), next.dt.load(on), next.C.load(on);
@@ -611,8 +645,9 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
       put(side, v);
     }
   };
-  if (first < live_last) load(t);
-  for (int tile = live_last - 1; tile >= first; --tile, t -= kTileSteps) {
+  if (runs > 0) load(t);
+  for (int run = runs - 1; run >= 0; --run, t -= kNext) {
+    const int tile = first + run;
     float h[NS];
     if (MODE == kWhole) {
 #pragma unroll
@@ -648,12 +683,12 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
       }
     }
     next.put_coefs(lds, lane);
-    if (tile > first) load(t - kTileSteps);
+    if (run > 0) load(t - kNext);
     wave_sync();
     // 1. decays, the run's maps forward (h) and backward (E)
     float a[kRun][NS], Qh[NS], Qe[NS], sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) Qh[i] = Qe[i] = 0.0f;
+    for (int i = 0; i < NS; ++i) Qh[i] = 0.0f, Qe[i] = MODE == kMaps ? carry[i] : 0.0f;
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
       const Fs<2> s = lds.step[r][lane / SL];
@@ -676,12 +711,18 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
     float P[NS], e[NS] = {};
 #pragma unroll
     for (int i = 0; i < NS; ++i) P[i] = run_decay(sum * A[i]);
+    if (MODE == kMaps) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) carry[i] = Qe[i], decay[i] = fmaxf(decay[i] * P[i], 0x1p-126f);
+      wave_sync();
+      continue;
+    }
     MapLds<G>(*const map)[3] = maps[side];
     map[wave][0].put(lane, P);
     map[wave][1].put(lane, Qe);
-    if (MODE == kWhole) map[wave][2].put(lane, Qh);
+    map[wave][2].put(lane, Qh);
     lds_barrier();
-    if (MODE == kWhole && tile + 1 < live_last) flush(t + kTileSteps);
+    if (run + 1 < runs) flush(t + kTileSteps);
     // (selects, not branches: the maps are then read one after the other without a wait)
 #pragma unroll
     for (int w = kWaves - 1; w >= 0; --w) {
@@ -692,21 +733,17 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
       for (int i = 0; i < NS; ++i) {
         e[i] = w == wave ? carry[i] : e[i];
         carry[i] = fmaf(Pw[i], carry[i], Qw[i]);
-        if (MODE == kMaps) decay[i] = fmaxf(decay[i] * Pw[i], 0x1p-126f);
       }
     }
-    if (MODE == kWhole) {
 #pragma unroll
-      for (int w = 0; w + 1 < kWaves; ++w) {
-        float Pw[NS], Qw[NS];
-        map[w][0].get(lane, Pw);
-        map[w][2].get(lane, Qw);
+    for (int w = 0; w + 1 < kWaves; ++w) {
+      float Pw[NS], Qw[NS];
+      map[w][0].get(lane, Pw);
+      map[w][2].get(lane, Qw);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) h[i] = w < wave ? fmaf(Pw[i], h[i], Qw[i]) : h[i];
-      }
+      for (int i = 0; i < NS; ++i) h[i] = w < wave ? fmaf(Pw[i], h[i], Qw[i]) : h[i];
     }
     lds_barrier();  // (the maps and the sums of the tile before have been read)
-    if (MODE == kMaps) continue;
     // 3. the states, each before its step
     float before[kRun + 1][NS];
 #pragma unroll
@@ -791,10 +828,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
     wave_sync();
   }
   if (MODE == kMaps) {
-    if (wave == 0) {
-      mine.store(p, p.seg + (int64_t)seg * 2 * state_size, at.b, decay);
-      mine.store(p, p.seg + (int64_t)(seg * 2 + 1) * state_size, at.b, carry);
-    }
+    store_segment<G, true>(p, mine, at, seg, lane, wave, maps[side][0], decay, carry);
     return;
   }
   for (int tile = max(first, live_last); tile < last; ++tile) {  // past the row
