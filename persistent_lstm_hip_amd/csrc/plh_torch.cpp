@@ -784,7 +784,7 @@ std::tuple<std::vector<Tensor>, Tensor> clip_grad_norm(const std::vector<Tensor>
   std::sort(ranges.begin(), ranges.end());
   for (size_t i = 1; i < ranges.size(); ++i)
     TORCH_CHECK_VALUE(ranges[i].first >= ranges[i - 1].second,
-                      "two gradients share memory (or are the same): they cannot be updated in place");
+                      "two gradients share memory (or are the same, or lie in each other's gaps): they cannot be updated in place");
   Tensor norm = empty({}, at::kFloat, device);
   const Tensor ws = empty({plh_clip_grad_norm_workspace_bytes((int64_t)count, numel.data())}, at::kByte, device);
   check(plh_clip_grad_norm((int64_t)count, dtypes.data(), src.data(), dst.data(), numel.data(), max_norm,

@@ -168,6 +168,15 @@ def test_refusals(gpu):
         P.clip_grad_norm([torch.ones(3, device="cuda", requires_grad=True)], 1.0, inplace=True)
 
 
+def test_inference_mode(gpu):
+    _say("clip inference")
+    with torch.inference_mode():
+        t = torch.full((5,), 2.0, device="cuda")
+        out, norm = P.clip_grad_norm([t], 1.0)
+        P.clip_grad_norm([t], 1.0, inplace=True)
+    assert torch.equal(out[0], t) and abs(norm.item() - math.sqrt(20.0)) < 1e-5
+
+
 def test_more_than_32_bits_of_elements(gpu):
     _say("clip large")
     n = (1 << 31) + 12345

@@ -352,6 +352,42 @@ def test_another_stream(gpu):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_two_calls_at_once(gpu):
+    """Calls that overlap on two streams, each with segments and so with a workspace."""
+    _say("selective scan two streams")
+    cases = []
+    for seed in (1, 2):
+        d = {n: t.cuda().requires_grad_(True) for n, t in _inputs(1, 1500, 20, 16, F32, seed=seed).items()}
+        g = torch.randn(1, 1500, 20, device="cuda")
+
+        def run(d=d, g=g):
+            out, h = _call(d)
+            return (out.detach(), h.detach(), *torch.autograd.grad(out, [d[n] for n in LEAVES], g))
+
+        cases.append((run, run(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for run, _, s in cases:
+            with torch.cuda.stream(s):
+                got.append(run())
+        torch.cuda.synchronize()
+        for (_, want, _), have in zip(cases, got):
+            assert all(torch.equal(a, b) for a, b in zip(have, want))
+
+
+def test_inference_mode(gpu):
+    _say("selective scan inference")
+    d = {n: t.cuda() for n, t in _inputs(2, 20, 24, 16, F16).items()}
+    want = _call(d)
+    with torch.inference_mode():
+        got = _call(d)
+        h = d["h0"].clone()
+        P.selective_scan_step(d["u"][:, 0], d["dt"][:, 0], d["A"], d["B"][:, 0], d["C"][:, 0], h, d["D"], d["z"][:, 0],
+                              dt_bias=d["dt_bias"], inplace=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and not torch.equal(h, d["h0"])
+
+
 def test_a_captured_training_step_replays(gpu):
     """Two graphs and eager work between their replays; every replay gives the eager result of its inputs."""
     _say("selective scan graph")
