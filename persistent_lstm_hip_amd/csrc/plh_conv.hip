@@ -460,7 +460,8 @@ hipError_t launch_conv_backward(ConvArgs p, int width, hipStream_t s) {
   });
   if (e == hipSuccess && p.part) {
     ColumnSums sums = {};
-    sums.part = p.part, sums.rows = p.batch > 0 && p.T_ > 0 ? l.groups : 0, sums.cols = (int64_t)p.C * (width + 1), sums.out32 = p.w32;
+    sums.part = p.part, sums.rows = p.batch > 0 && p.T_ > 0 ? l.groups : 0;
+    sums.cols = (int64_t)p.C * (width + 1), sums.out32 = p.w32;
     sums.out[0] = p.d_weight, sums.begin[1] = (int64_t)p.C * width, sums.out[1] = p.d_bias;
     sums.begin[2] = sums.begin[3] = sums.cols;
     e = launch_column_sums<T>(sums, s);

@@ -81,10 +81,10 @@ struct Geo {
   // channels and F neighbouring states each.
   static constexpr int E = GROUP >= 8 ? GROUP / 8 : 1, F = NP >= 8 ? NP / 8 : 1;
   static_assert(kRun == 8, "eight steps by eight lanes");
-  // Groups of a workgroup of the backward pass, whose dB and dC it adds up.  One leaves three workgroups per CU, with rows of
-  // their own pace, two save half of the partial sums' traffic, which grows with the states: 16 states 8 x 2048 x 2048 bf16
-  // 772 and 758 us with the sums' kernel, 128 x 1000 x 256 fp16 ragged 479 and 581; 32 states 4 x 2048 x 1024 bf16 467 and
-  // 415, 64 states 998 and 954.
+  // Groups of a workgroup of the backward pass, whose dB and dC it adds up.  One leaves three workgroups per CU, with rows
+  // of their own pace, two save half of the partial sums' traffic, which grows with the states.  One and two, us: 16 states
+  // 8 x 2048 x 2048 bf16 772 and 758 with the sums' kernel, 128 x 1000 x 256 fp16 ragged 479 and 581; 32 states
+  // 4 x 2048 x 1024 bf16 467 and 415, 64 states 998 and 954.
   static constexpr int SIDE = SL == 4 ? 1 : 2;
 };
 
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
         h[i] = fmaf(a[r][i], h[i], s.v[1] * B.v[i]);
         y = fmaf(C.v[i], h[i], y);
       }
-      lds.y[r][lane / SL] = states_sum<SL>(y);  // (the same from all lanes of a set, as below: a branch would part the steps)
+      lds.y[r][lane / SL] = states_sum<SL>(y);  // (the same from all SL lanes, as below: a branch would part the steps)
     }
     wave_sync();
     if (t < p.T_ && n > 0) {
@@ -535,10 +535,9 @@ __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
 
 // ---- backward -----------------------------------------------------------------------------------
 
-
 template <typename G>
 struct BackLds {
-  WaveLds<G> f;               // (y: dy, then y; step: then s1, s2 of every channel)
+  WaveLds<G> f;                          // (y: dy, then y; step: then s1, s2 of every channel)
   alignas(16) float bc[kRun][2][G::NP];  // dB and dC of the wave's channels
   // What a lane needs at both ends of a tile, of its E channels: registers that the steps in between take.
   enum Kept { kU, kDt, kDy, kRawSlope, kGateSlope, kBias, kSkip, kSumSkip, kSumBias, kKept };
@@ -877,7 +876,8 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
   }
 }
 
-// dB and dC: the workgroups' sums, in their order.
+// dB and dC: the workgroups' sums, in their order (of four neighbouring ones per thread: 57.5 us against 61.5 at
+// 8 x 2048 x 2048 x 16 states, 27.3 against 26.8 at 128 x 1000 x 256 ragged: left as it is).
 template <typename T>
 __global__ void __launch_bounds__(256) selective_coefs_kernel(SelArgs p, T* d_B, T* d_C) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = p.batch * p.T_;
@@ -956,7 +956,8 @@ hipError_t launch_sel_forward(const SelArgs& p, hipStream_t s) {
     using G = Geo<decltype(sl)::value, decltype(ns)::value>;
     const dim3 block(kWaves * kWave);
     if (p.segs > 1) {
-      hipLaunchKernelGGL((selective_forward_kernel<T, G, kMaps, false>), dim3((unsigned)p.units, p.segs - 1), block, 0, s, p);
+      const dim3 all_but_last((unsigned)p.units, p.segs - 1);
+      hipLaunchKernelGGL((selective_forward_kernel<T, G, kMaps, false>), all_but_last, block, 0, s, p);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
@@ -1009,7 +1010,8 @@ hipError_t launch_sel_backward(SelArgs p, void* d_A, void* d_B, void* d_C, void*
     });
     const int64_t n = p.batch * p.T_ * 2 * p.N;
     if (e == hipSuccess && n > 0 && (d_B || d_C)) {
-      hipLaunchKernelGGL(selective_coefs_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, (T*)d_B, (T*)d_C);
+      const dim3 grid((unsigned)((n + 255) / 256));
+      hipLaunchKernelGGL(selective_coefs_kernel<T>, grid, dim3(256), 0, s, p, (T*)d_B, (T*)d_C);
       e = hipGetLastError();
     }
   }

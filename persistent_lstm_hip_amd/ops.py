@@ -209,7 +209,8 @@ def clip_grad_norm(grads: Iterable[Optional[torch.Tensor]], max_norm: float, *,
         clip_grad_norm([p.grad for p in model.parameters()], 1.0, inplace=True)
 
     serves a training step.  The tensors are on one device, of any shapes, strides and mixed types; those that are
-    overwritten must lie in ranges of memory that do not overlap.  Squares are summed in 64 bits.  max_norm may be infinite: nothing is scaled.  A norm of infinity scales by zero and one of NaN by NaN, as
+    overwritten must lie in ranges of memory that do not overlap.  Squares are summed in 64 bits.  max_norm may be infinite:
+    nothing is scaled.  A norm of infinity scales by zero and one of NaN by NaN, as
     torch.nn.utils.clip_grad_norm_ does.  Not differentiable.
     """
     if isinstance(grads, torch.Tensor):

@@ -114,7 +114,8 @@ def test_infinite_and_nan_norms(gpu):
         _, norm = P.clip_grad_norm(mine, 1.0, inplace=True)
         assert torch.equal(torch.nan_to_num(norm, nan=-1.0), torch.nan_to_num(theirs, nan=-1.0))
         for a, p in zip(mine, params):
-            assert torch.equal(torch.isnan(a), torch.isnan(p.grad)) and torch.equal(torch.nan_to_num(a), torch.nan_to_num(p.grad))
+            assert torch.equal(torch.isnan(a), torch.isnan(p.grad))
+            assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(p.grad))
         same, _ = P.clip_grad_norm([t], float("inf"), inplace=True)  # no limit: nothing is touched
         assert torch.equal(torch.isnan(same[0]), torch.isnan(t))
 

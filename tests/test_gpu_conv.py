@@ -64,8 +64,8 @@ def _lengths(B, T):
 
 # (B, T, C): one of everything; no steps, no rows; fewer channels than a vector; odd; vectors' edges; long rows and a
 # stretch's edges; more channels than a slab
-SHAPES = [(1, 1, 1), (2, 0, 5), (0, 4, 3), (3, 2, 3), (4, 5, 7), (2, 33, 8), (3, 64, 9), (2, 65, 60), (5, 130, 129), (1, 700, 24),
-          (40, 3, 333), (1, 3000, 2)]
+SHAPES = [(1, 1, 1), (2, 0, 5), (0, 4, 3), (3, 2, 3), (4, 5, 7), (2, 33, 8), (3, 64, 9), (2, 65, 60), (5, 130, 129),
+          (1, 700, 24), (40, 3, 333), (1, 3000, 2)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -165,7 +165,8 @@ def test_strides(gpu):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("W", [1, 2, 3, 4, 5, 6, 7, 8])
 def test_step(gpu, W, dtype):
-    for B, C, wdtype, silu in ((1, 1, F32, True), (3, 7, dtype, False), (65, 129, F32, True), (2, 64, dtype, True), (0, 3, F32, True)):
+    for B, C, wdtype, silu in ((1, 1, F32, True), (3, 7, dtype, False), (65, 129, F32, True),
+                               (2, 64, dtype, True), (0, 3, F32, True)):
         _say(f"conv step {B} {C} {W} {dtype}")
         x, w, b, st = _inputs(B, 1, C, W, dtype, wdtype)
         want = plain.conv(x, w, b, st, None, silu)
