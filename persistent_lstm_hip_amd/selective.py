@@ -26,7 +26,8 @@ State = Tuple[torch.Tensor, torch.Tensor]  # the convolution's last inputs, the 
 
 class SelectiveScanBlock(nn.Module):
     """One residual block of width dim, expand * dim channels wide inside.  Its state is a pair: the convolution's
-    [batch, width - 1, channels] of the activations' type, the scan's [batch, channels, states] float32."""
+    [batch, width - 1, channels], the scan's [batch, channels, states] float32.  The convolution's is of the activations'
+    type, under autocast the lower one; forward takes one of any type, step one of the activations' type or float32."""
 
     def __init__(self, dim: int, dropout: float = 0.0, *, states: int = 16, width: int = 4, expand: int = 2):
         super().__init__()
@@ -59,6 +60,8 @@ class SelectiveScanBlock(nn.Module):
         GatedScanBlock."""
         before, h0 = state if state is not None else (None, None)
         u, z = self._inner(x)
+        if before is not None:
+            before = before.to(u.dtype)
         u, before = causal_conv(u, self.conv_weight, self.conv_bias, before, lengths=lengths)
         h, h_n = selective_scan(u, *self._coefs(u), z, h0, dt_bias=self.dt_bias.float(), lengths=lengths)
         p = self.dropout if self.training else 0.0
@@ -69,7 +72,11 @@ class SelectiveScanBlock(nn.Module):
     def step(self, x: torch.Tensor, state: State) -> torch.Tensor:
         """One token x [batch, dim] -> y; both parts of the state are updated in place.  For inference."""
         u, z = self._inner(x)
-        u, _ = causal_conv_step(u, state[0], self.conv_weight, self.conv_bias, inplace=True)
+        if state[0].dtype == torch.float32 and u.dtype != torch.float32:  # under autocast: it holds 16-bit inputs exactly
+            u, last = causal_conv_step(u, state[0].to(u.dtype), self.conv_weight, self.conv_bias)
+            state[0].copy_(last)
+        else:
+            u, _ = causal_conv_step(u, state[0], self.conv_weight, self.conv_bias, inplace=True)
         dt, A, B, C, D = self._coefs(u)
         h, _ = selective_scan_step(u, dt, A, B, C, state[1], D, z, dt_bias=self.dt_bias.float(), inplace=True)
         return x + self.out(h)
