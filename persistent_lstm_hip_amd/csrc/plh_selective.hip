@@ -498,6 +498,8 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
 // TB/s (a copy of the states 10.1).  (Two, four and eight rows per thread, which read A once for all of them: 18.5, 18.9 and
 // 31 us.)
 constexpr int kStepStates = 4;
+int step_lanes(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
+
 template <typename T, int SL, bool GATED>
 __global__ void __launch_bounds__(256) selective_step_kernel(SelArgs p) {
   constexpr int NS = kStepStates;
@@ -981,11 +983,13 @@ hipError_t launch_sel_step(const SelArgs& p, hipStream_t s) {
       hipLaunchKernelGGL((selective_step_kernel<T, SL, false>), grid, dim3(256), 0, s, p);
     return hipGetLastError();
   };
-  if (p.N <= 4) return run(std::integral_constant<int, 1>());
-  if (p.N <= 8) return run(std::integral_constant<int, 2>());
-  if (p.N <= 16) return run(std::integral_constant<int, 4>());
-  if (p.N <= 32) return run(std::integral_constant<int, 8>());
-  return run(std::integral_constant<int, 16>());
+  switch (step_lanes(p.N)) {
+    case 1: return run(std::integral_constant<int, 1>());
+    case 2: return run(std::integral_constant<int, 2>());
+    case 4: return run(std::integral_constant<int, 4>());
+    case 8: return run(std::integral_constant<int, 8>());
+    default: return run(std::integral_constant<int, 16>());
+  }
 }
 
 template <typename T>
@@ -1036,9 +1040,10 @@ int check_selective(const char* what, const plh_selective_scan_args* a, bool ste
   if (a->channels < 1 || a->channels > (1 << 20))
     return op_error(PLH_ERR_UNSUPPORTED, what, "channels must lie in [1, 2^20]");
   if (a->seq_len > (1 << 30)) return op_error(PLH_ERR_UNSUPPORTED, what, "seq_len must not exceed 2^30");
+  // (a launch has fewer than 2^32 threads, in whole workgroups of 256)
+  if (step && (a->batch > (int64_t(1) << 32) || a->batch * a->channels * step_lanes(a->states) > (int64_t(1) << 32) - 256))
+    return op_error(PLH_ERR_UNSUPPORTED, what, "batch * channels * lanes per channel must not exceed 2^32 - 256");
   // (what a grid of workgroups holds)
-  if (step && (a->batch > (1 << 30) || a->batch * a->channels * a->states > (int64_t(1) << 32)))
-    return op_error(PLH_ERR_UNSUPPORTED, what, "batch * channels * states must not exceed 2^32");
   if (!step && (a->batch > (1 << 21) || a->batch * ((a->channels + 7) / 8) > (1 << 21)))
     return op_error(PLH_ERR_UNSUPPORTED, what, "batch * ceil(channels / 8) must not exceed 2^21");
   if (!step && a->batch * a->seq_len * a->states > (1 << 30))
