@@ -1043,9 +1043,13 @@ int check_selective(const char* what, const plh_selective_scan_args* a, bool ste
   // (a launch has fewer than 2^32 threads, in whole workgroups of 256)
   if (step && (a->batch > (int64_t(1) << 32) || a->batch * a->channels * step_lanes(a->states) > (int64_t(1) << 32) - 256))
     return op_error(PLH_ERR_UNSUPPORTED, what, "batch * channels * lanes per channel must not exceed 2^32 - 256");
-  // (what a grid of workgroups holds)
-  if (!step && (a->batch > (1 << 21) || a->batch * ((a->channels + 7) / 8) > (1 << 21)))
-    return op_error(PLH_ERR_UNSUPPORTED, what, "batch * ceil(channels / 8) must not exceed 2^21");
+  // (Both directions' launches stay below 2^32 threads: a workgroup of 256 has 16 channels with up to 16 states, then 8, then
+  // 4; one of 512, the backward pass's with more than 16 states, twice as many.  What remains beside the second limit, 2^21
+  // rows and more of up to eight channels, has 2^30.)
+  const int64_t eights = a->batch > (1 << 23) ? int64_t(1) << 23 : a->batch * ((a->channels + 7) / 8);
+  if (!step && eights > (a->batch < (1 << 21) ? (1 << 23) - 1 : 1 << 21))
+    return op_error(PLH_ERR_UNSUPPORTED, what,
+                    "batch * ceil(channels / 8) must be below 2^23, and from 2^21 rows on not exceed 2^21");
   if (!step && a->batch * a->seq_len * a->states > (1 << 30))
     return op_error(PLH_ERR_UNSUPPORTED, what, "batch * seq_len * states must not exceed 2^30");
   if (!a->A) return op_error(PLH_ERR_INVALID, what, "A is required");

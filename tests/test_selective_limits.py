@@ -6,7 +6,13 @@ import ctypes
 
 import pytest
 
-from persistent_lstm_hip_amd.extension import PLH_ERR_INVALID, PLH_ERR_UNSUPPORTED, SelectiveScanArgs, require_extension
+from persistent_lstm_hip_amd.extension import (
+    PLH_ERR_INVALID,
+    PLH_ERR_UNSUPPORTED,
+    SelectiveScanArgs,
+    SelectiveScanGrads,
+    require_extension,
+)
 
 ANY = ctypes.c_void_p(256)  # never dereferenced
 
@@ -36,3 +42,31 @@ def test_a_step_has_fewer_threads_than_a_launch_holds(lib, states, lanes):
         assert rc == PLH_ERR_INVALID and b"out" in msg, (batch, channels)
     for batch, channels in ((most + 1, 1), ((1 << 32) // lanes, 1), ((1 << 12) // lanes + 1, 1 << 20), (1 << 62, 1 << 20)):
         assert step(batch, channels)[0] == PLH_ERR_UNSUPPORTED, (batch, channels)
+
+
+@pytest.mark.parametrize("states", [1, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("backward", [False, True])
+def test_rows_and_channels_that_a_launch_holds(lib, states, backward):
+    def call(batch, channels):
+        a = _args(batch, 2, channels, states)
+        if backward:  # (without the forward pass's states)
+            rc = lib.plh_selective_scan_backward(a, None, ANY, None, ctypes.byref(SelectiveScanGrads()), ANY, 1 << 62, None)
+        else:
+            rc = lib.plh_selective_scan_forward(a, None, None, None, None, None, 0, None)
+        return rc, lib.plh_last_error()
+
+    for batch, channels in ((16385, 1024), (65535, 1024), ((1 << 21) - 1, 24), (7, 1 << 20), (63, 1 << 20), (1 << 21, 8),
+                            ((1 << 21) - 1, 9)):
+        rc, msg = call(batch, channels)
+        if batch * 2 * states > 1 << 30:
+            continue
+        # the workgroups of either direction, each with its threads
+        per, side = (16, 1) if states <= 16 else (8, 2) if states <= 32 else (4, 2)
+        groups = (channels + per - 1) // per
+        assert batch * groups * 256 < 1 << 32
+        assert ((batch + side - 1) // side if groups == 1 else batch * ((groups + side - 1) // side)) * side * 256 < 1 << 32
+        assert rc == PLH_ERR_INVALID and (b"required" in msg), (batch, channels, msg)
+    for batch, channels in ((65536, 1024), (1 << 21, 9), ((1 << 21) + 1, 1), (64, 1 << 20), ((1 << 21) - 1, 33), (1 << 40, 1),
+                            (1 << 62, 1 << 20)):
+        rc, msg = call(batch, channels)
+        assert rc == PLH_ERR_UNSUPPORTED and b"2^2" in msg, (batch, channels, msg)
