@@ -162,7 +162,9 @@ __device__ __forceinline__ float run_decay(float log2_decay) {
   return __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(log2_decay, -126.0f, 127.0f));
 }
 
-// Sum over the SL lanes that share a pair of channels, to all of them.
+__device__ __forceinline__ bool any_lane(bool v) { return __builtin_amdgcn_ballot_w64(v) != 0; }
+
+// Sum over the SL lanes that share a channel, to all of them.
 template <int CTRL>
 __device__ __forceinline__ float add_dpp(float v) {
   const int u = __builtin_bit_cast(int, v);
@@ -240,8 +242,10 @@ struct MapLds {
   }
 };
 
-// A thread's states, in [B][D][N] at row b; zero outside.
-template <typename G>
+// A thread's states, in [B][D][N] at row b; zero outside.  PADDED: there are fewer states than NP.  Those that are missing have
+// B = C = 0 and the smallest rate, which leaves their h and E zero as long as u, dt and dy are finite; an infinity times zero
+// would be a NaN in the sums over a channel's states.
+template <typename G, bool PADDED>
 struct Slots {
   int c, n;    // channel and first state
   int states;  // of the NS that there are
@@ -260,12 +264,18 @@ struct Slots {
     for (int j = 0; j < G::NS; ++j) t.v[j] = v[j];
     store_some<float, G::NS>(base + (b * p.D_ + c) * p.N + n, t, states);
   }
-  // The decays' rates, times log2 e.
+  // v of state i, zero where that is missing.
+  __device__ __forceinline__ float of(int i, float v) const { return PADDED && i >= states ? 0.0f : v; }
+  __device__ __forceinline__ void clear_missing(float (&v)[G::NS]) const {
+#pragma unroll
+    for (int i = 0; i < G::NS; ++i) v[i] = of(i, v[i]);
+  }
+  // The decays' rates, times log2 e.  (Of missing states one that is not zero: an infinite step's decay is then zero, not NaN.)
   template <typename T>
   __device__ __forceinline__ void rates(const SelArgs& p, float (&v)[G::NS]) const {
 #pragma unroll
     for (int j = 0; j < G::NS; ++j)
-      v[j] = j < states ? rate(param<T>(p.A, p.w32, (int64_t)c * p.N + n + j, 0.0f)) : 0.0f;
+      v[j] = j < states ? rate(param<T>(p.A, p.w32, (int64_t)c * p.N + n + j, 0.0f)) : -0x1p-126f;
   }
 };
 
@@ -312,8 +322,8 @@ struct TileIn {
 enum Mode { kWhole, kMaps };
 
 // The map of a segment from its waves' maps, from the first to the last, or back.
-template <typename G, bool BACK>
-__device__ __forceinline__ void store_segment(const SelArgs& p, const Slots<G>& mine, const At& at, int seg, int lane,
+template <typename G, bool BACK, typename S>
+__device__ __forceinline__ void store_segment(const SelArgs& p, const S& mine, const At& at, int seg, int lane,
                                               int wave, MapLds<G>* maps, const float (&decay)[G::NS],
                                               const float (&sum)[G::NS]) {
   maps[wave * 2].put(lane, decay);
@@ -341,7 +351,7 @@ __device__ __forceinline__ void store_segment(const SelArgs& p, const Slots<G>& 
 
 // A workgroup carries a group of channels through a segment of time, a tile of four waves by eight steps at a time.  MAPS:
 // only the segment's map is wanted; every wave then runs a quarter of the segment by itself, and their maps meet at the end.
-template <typename T, typename G, Mode MODE, bool GATED>
+template <typename T, typename G, Mode MODE, bool GATED, bool PADDED>
 __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArgs p) {
   constexpr int E = G::E, SL = G::SL, NS = G::NS;
   __shared__ WaveLds<G> lds_all[kWaves];
@@ -350,7 +360,7 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
   WaveLds<G>& lds = lds_all[wave];
   const int seg = blockIdx.y;
   const At at = place(p, slab_of(blockIdx.x, gridDim.x), G::GROUP);
-  const Slots<G> mine(p, at, lane);
+  const Slots<G, PADDED> mine(p, at, lane);
   const int64_t state_size = p.batch * p.D_ * p.N;
 
   // the layout that memory is read and written in
@@ -401,12 +411,14 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     const int tile = first + run;
     // dt and dt u, B, C: into the wave's LDS
     const Vec<T, E> u = next.u.v, z = next.z.v;
+    bool odd = false;
     if (G::GROUP >= 8 || ec < G::GROUP) {
       Fs<2 * E> f;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float raw = (float)next.dt.v.v[j] + bias[j], dt = t < at.len ? p.softplus ? softplus(raw) : raw : 0.0f;
         f.v[2 * j] = dt, f.v[2 * j + 1] = dt * (float)u.v[j];
+        odd = odd || !__builtin_isfinite(f.v[2 * j + 1]);
       }
       *reinterpret_cast<Fs<2 * E>*>(&lds.step[row][ec]) = f;
     }
@@ -456,18 +468,28 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
       }
     }
     // 3. the steps from where they start
+    mine.clear_missing(h), mine.clear_missing(carry);
+    const auto steps = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < kRun; ++r) {
-      const Fs<2> s = lds.step[r][lane / SL];
-      const Fs<NS> B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
-      float y = 0.0f;
+      for (int r = 0; r < kRun; ++r) {
+        const Fs<2> s = lds.step[r][lane / SL];
+        const Fs<NS> B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
+        float y = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        h[i] = fmaf(a[r][i], h[i], s.v[1] * B.v[i]);
-        y = fmaf(C.v[i], h[i], y);
+        for (int i = 0; i < NS; ++i) {
+          h[i] = fmaf(a[r][i], h[i], s.v[1] * B.v[i]);
+          if (decltype(careful)::value) h[i] = mine.of(i, h[i]);
+          y = fmaf(C.v[i], h[i], y);
+        }
+        lds.y[r][lane / SL] = states_sum<SL>(y);  // (the same from all SL lanes, as below: a branch would part the steps)
       }
-      lds.y[r][lane / SL] = states_sum<SL>(y);  // (the same from all SL lanes, as below: a branch would part the steps)
-    }
+    };
+    // (Missing states are cleared at every step only by a wave that has something infinite.  16 x 1024 x 1024 channels x 10 states
+    // bf16: 114 us, where every wave did it 130, without any of it 112; the backward pass, which always does, 340 and 327.)
+    if (PADDED && any_lane(odd))
+      steps(std::bool_constant<PADDED>());
+    else
+      steps(std::false_type());
     wave_sync();
     if (t < p.T_ && n > 0) {
       const Fs<E> sum = *reinterpret_cast<const Fs<E>*>(&lds.y[row][ec]);
@@ -547,7 +569,7 @@ struct BackLds {
 };
 
 // The tiles of a segment from the last to the first.  MAPS: only the segment's map of E is wanted, as above.
-template <typename T, typename G, Mode MODE, bool GATED>
+template <typename T, typename G, Mode MODE, bool GATED, bool PADDED>
 __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) selective_backward_kernel(SelArgs p) {
   constexpr int SIDE = G::SIDE, E = G::E, SL = G::SL, NS = G::NS;
   __shared__ BackLds<G> lds_all[SIDE][kWaves];
@@ -566,8 +588,17 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
   const bool on = b_of < p.batch && group < p.groups;
   const int sides = alone ? 1 : p.groups - (group - side);  // that have a group, where they share a row
   const At at = place(p, on ? b_of * p.groups + group : p.units, G::GROUP);
-  const Slots<G> mine(p, at, lane);
+  const Slots<G, PADDED> mine(p, at, lane);
   const int64_t state_size = p.batch * p.D_ * p.N;
+
+  // B and C of the lane's states, step r's at r * kCoefs.  Those of missing channels are zeros, as their u and dy are: an
+  // infinite coefficient would make them NaN, and with them dB and dC, the sums over the channels.
+  constexpr int kCoefs = 2 * SL;
+  __shared__ Fs<NS> none[MODE == kWhole ? kRun * kCoefs : 1];
+  if (MODE == kWhole)
+    for (int i = threadIdx.x; i < kRun * kCoefs; i += SIDE * kWaves * kWave) none[i] = Fs<NS>{};
+  const Fs<NS>* const B_at = MODE == kMaps || mine.c < p.D_ ? &lds.bc[0][0][lane % SL] : &none[lane % SL];
+  const Fs<NS>* const C_at = B_at + SL;
 
   const int row = lane / 8, ec = lane % 8 * E, c = at.c0 + ec;
   const int n = G::GROUP < 8 && ec >= G::GROUP ? 0 : min(max(p.D_ - c, 0), E);
@@ -582,7 +613,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
       skip.v[j] = j < n ? param<T>(p.D, p.w32, c + j, 0.0f) : 0.0f;
     }
     keep(Kept::kBias, bias), keep(Kept::kSkip, skip), keep(Kept::kSumSkip, Fs<E>{}), keep(Kept::kSumBias, Fs<E>{});
-    wave_sync();
+    lds_barrier();
   }
   float A[NS];
   mine.template rates<T>(p, A);
@@ -695,7 +726,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
       const Fs<2> s = lds.step[r][lane / SL];
-      const Fs<NS> B = lds.bc[r][0][lane % SL];
+      const Fs<NS> B = B_at[r * kCoefs];
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         a[r][i] = __builtin_amdgcn_exp2f(s.v[0] * A[i]);
@@ -705,7 +736,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
     }
 #pragma unroll
     for (int r = kRun - 1; r >= 0; --r) {
-      const Fs<NS> C = lds.bc[r][1][lane % SL];
+      const Fs<NS> C = C_at[r * kCoefs];
       const float q = lds.y[r][lane / SL];
 #pragma unroll
       for (int i = 0; i < NS; ++i) Qe[i] = a[r][i] * fmaf(C.v[i], q, Qe[i]);
@@ -747,6 +778,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
       for (int i = 0; i < NS; ++i) h[i] = w < wave ? fmaf(Pw[i], h[i], Qw[i]) : h[i];
     }
     lds_barrier();  // (the maps and the sums of the tile before have been read)
+    mine.clear_missing(h), mine.clear_missing(e), mine.clear_missing(carry);
     // 3. the states, each before its step
     float before[kRun + 1][NS];
 #pragma unroll
@@ -754,10 +786,10 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
 #pragma unroll
     for (int r = 0; r < kRun; ++r) {
       const Fs<2> s = lds.step[r][lane / SL];
-      const Fs<NS> B = lds.bc[r][0][lane % SL];
+      const Fs<NS> B = B_at[r * kCoefs];
 #pragma unroll
       for (int i = 0; i < NS; ++i)
-        before[r + 1][i] = fmaf(a[r][i], before[r][i], s.v[1] * B.v[i]);
+        before[r + 1][i] = mine.of(i, fmaf(a[r][i], before[r][i], s.v[1] * B.v[i]));
     }
     wave_sync();  // (or what the steps read would be kept in registers for the way back)
     // 4. and backwards through them
@@ -768,12 +800,12 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
         // (past the row E stays as it is, and a product of what is infinite there with a zero must not count)
         if (!WHOLE && tile * kTileSteps + wave * kRun + r >= at.len) continue;
         const Fs<2> s = lds.step[r][lane / SL];
-        const Fs<NS> B = lds.bc[r][0][lane % SL], C = lds.bc[r][1][lane % SL];
+        const Fs<NS> B = B_at[r * kCoefs], C = C_at[r * kCoefs];
         const float q = lds.y[r][lane / SL];
         float s1 = 0.0f, s2 = 0.0f, y = 0.0f, dB[NS], dC[NS];
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-          const float g = fmaf(C.v[j], q, e[j]);
+          const float g = mine.of(j, fmaf(C.v[j], q, e[j]));
           s1 = fmaf(g, B.v[j], s1);
           dB[j] = g * s.v[1];
           dC[j] = q * before[r + 1][j];
@@ -959,16 +991,20 @@ hipError_t launch_sel_forward(const SelArgs& p, hipStream_t s) {
     const dim3 block(kWaves * kWave);
     if (p.segs > 1) {
       const dim3 all_but_last((unsigned)p.units, p.segs - 1);
-      hipLaunchKernelGGL((selective_forward_kernel<T, G, kMaps, false>), all_but_last, block, 0, s, p);
+      hipLaunchKernelGGL((selective_forward_kernel<T, G, kMaps, false, false>), all_but_last, block, 0, s, p);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
-    const dim3 grid((unsigned)p.units, p.segs);
-    if (p.z.p)
-      hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, true>), grid, block, 0, s, p);
-    else
-      hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, false>), grid, block, 0, s, p);
-    return hipGetLastError();
+    const auto run = [&](auto gated, auto padded) {
+      const dim3 grid((unsigned)p.units, p.segs);
+      hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, decltype(gated)::value, decltype(padded)::value>), grid,
+                         block, 0, s, p);
+      return hipGetLastError();
+    };
+    const auto of_states = [&](auto gated) {
+      return p.N < G::NP ? run(gated, std::true_type()) : run(gated, std::false_type());
+    };
+    return p.z.p ? of_states(std::true_type()) : of_states(std::false_type());
   });
 }
 
@@ -1003,11 +1039,14 @@ hipError_t launch_sel_backward(SelArgs p, void* d_A, void* d_B, void* d_C, void*
       const auto run = [&](auto gated) {
         constexpr bool GATED = decltype(gated)::value;
         if (p.segs > 1) {
-          hipLaunchKernelGGL((selective_backward_kernel<T, G, kMaps, GATED>), grid, block, 0, s, p);
+          hipLaunchKernelGGL((selective_backward_kernel<T, G, kMaps, GATED, false>), grid, block, 0, s, p);
           const hipError_t e2 = hipGetLastError();
           if (e2 != hipSuccess) return e2;
         }
-        hipLaunchKernelGGL((selective_backward_kernel<T, G, kWhole, GATED>), grid, block, 0, s, p);
+        if (p.N < G::NP)
+          hipLaunchKernelGGL((selective_backward_kernel<T, G, kWhole, GATED, true>), grid, block, 0, s, p);
+        else
+          hipLaunchKernelGGL((selective_backward_kernel<T, G, kWhole, GATED, false>), grid, block, 0, s, p);
         return hipGetLastError();
       };
       return p.z.p ? run(std::true_type()) : run(std::false_type());

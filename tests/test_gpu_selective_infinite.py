@@ -43,13 +43,14 @@ def _compare(got, want, bound, what):
 @pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 7, 8, 10, 15, 16, 17, 31, 32, 33, 63, 64])
 @pytest.mark.parametrize("gate", [True, False])
 def test_infinite_values(gpu, N, gate):
-    """One in u, in dt and in the output's gradient in turn; one tile and several, the first and a later wave's steps."""
+    """One in u, in dt, in the output's gradient and, for all channels, in B and C in turn; one tile and several, the first
+    and a later wave's steps, channels that fill no group."""
     for T, at in ((7, 2), (70, 0), (70, 20), (70, 37)):
-        for name in ("u", "dt", "d_out"):
+        for name in ("u", "dt", "d_out", "B", "C"):
             _say(f"selective infinite N={N} gate={gate} T={T} {name}[{at}]")
-            d = _inputs(2, T, 12, N, gate)
-            d_out = 0.1 + torch.rand(2, T, 12, generator=torch.Generator().manual_seed(5))
-            (d_out if name == "d_out" else d[name])[0, at, 5] = INF
+            d = _inputs(2, T, 11, N, gate)
+            d_out = 0.1 + torch.rand(2, T, 11, generator=torch.Generator().manual_seed(5))
+            (d_out if name == "d_out" else d[name])[0, at, 0 if name in "BC" else 5] = INF
             want = plain.scan(*(d[n] for n in LEAVES), d_out=d_out)
             dev = {n: None if t is None else t.cuda().requires_grad_(True) for n, t in d.items()}
             out, h_n = P.selective_scan(*(dev[n] for n in LEAVES[:-1]), dt_bias=dev["dt_bias"])
