@@ -156,10 +156,30 @@ __device__ __forceinline__ void softplus(float v, float& value, float& slope) {
 // leaves the state as it is, and 0 * inf would not.
 __device__ __forceinline__ float rate(float A) { return __builtin_elementwise_maximum(A * kOpLog2e, -3e38f); }
 
-// The decay of a run of steps.  Every step's own is positive; their product may underflow (or, of a growing state,
-// overflow), and 0 * inf would be NaN where the steps one after the other are not.
+// The map of a run of steps, h -> P h + Q, with P = 2^log2_decay.  Every step's own decay is positive, but their product may be
+// too small for fp32 (or, where step sizes are negative and the state grows, too large), and 0 * inf would be NaN where the steps
+// one after the other are not.  So P is held at 2^-126 at least, which leaves next to nothing of a state.  Where it may grow
+// again, which it cannot with softplus, P is held as its square root (GROWS), which is in range down to P = 2^-252 and up to
+// 2^254: what lies beyond leaves no normal number of a normal one.  (8 x 2048 x 2048 channels x 16 states bf16 forward 236 us,
+// backward 667, with the root 240 and 673.)
+__device__ __forceinline__ float bounded_exp2(float v) {
+  return __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(v, -126.0f, 127.0f));
+}
+template <bool GROWS>
 __device__ __forceinline__ float run_decay(float log2_decay) {
-  return __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(log2_decay, -126.0f, 127.0f));
+  return bounded_exp2(GROWS ? 0.5f * log2_decay : log2_decay);
+}
+template <bool GROWS>
+__device__ __forceinline__ float apply_map(float P, float Q, float h) {
+  return GROWS ? fmaf(P * h, P, Q) : fmaf(P, h, Q);
+}
+
+// Waits for what v was loaded from.  (The compiler would wait in the loop that uses v next, every time, and so for that loop's
+// own loads too: 8 x 2048 x 2048 channels x 16 states bf16 forward 246 us, with the wait in front of it 235.)
+template <int N>
+__device__ __forceinline__ void arrived(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
 }
 
 __device__ __forceinline__ bool any_lane(bool v) { return __builtin_amdgcn_ballot_w64(v) != 0; }
@@ -321,18 +341,24 @@ struct TileIn {
 
 enum Mode { kWhole, kMaps };
 
-// The map of a segment from its waves' maps, from the first to the last, or back.
+// What a call's states are: as many as lanes hold and decaying (with softplus), fewer, or of any number and growing.
+enum Kind { kFull, kPadded, kGrowing };
+
+// The map of a segment from its waves' maps, from the first to the last, or back: the root of its decay, and its sum.  (Decays
+// meet as their logarithms: a product of what is too small with what is too large would be neither.)
 template <typename G, bool BACK, typename S>
 __device__ __forceinline__ void store_segment(const SelArgs& p, const S& mine, const At& at, int seg, int lane,
-                                              int wave, MapLds<G>* maps, const float (&decay)[G::NS],
+                                              int wave, MapLds<G>* maps, const float (&A)[G::NS], double time,
                                               const float (&sum)[G::NS]) {
-  maps[wave * 2].put(lane, decay);
+  float P[G::NS], Q[G::NS];
+#pragma unroll
+  for (int i = 0; i < G::NS; ++i) P[i] = (float)(time * A[i]);
+  maps[wave * 2].put(lane, P);
   maps[wave * 2 + 1].put(lane, sum);
   lds_barrier();
   if (wave != 0) return;
-  float P[G::NS], Q[G::NS];
 #pragma unroll
-  for (int i = 0; i < G::NS; ++i) P[i] = 1.0f, Q[i] = 0.0f;
+  for (int i = 0; i < G::NS; ++i) P[i] = Q[i] = 0.0f;
 #pragma unroll
   for (int k = 0; k < kWaves; ++k) {
     const int w = BACK ? kWaves - 1 - k : k;
@@ -340,8 +366,10 @@ __device__ __forceinline__ void store_segment(const SelArgs& p, const S& mine, c
     maps[w * 2].get(lane, Pw);
     maps[w * 2 + 1].get(lane, Qw);
 #pragma unroll
-    for (int i = 0; i < G::NS; ++i) Q[i] = fmaf(Pw[i], Q[i], Qw[i]), P[i] = fmaxf(P[i] * Pw[i], 0x1p-126f);
+    for (int i = 0; i < G::NS; ++i) Q[i] = apply_map<true>(run_decay<true>(Pw[i]), Qw[i], Q[i]), P[i] += Pw[i];
   }
+#pragma unroll
+  for (int i = 0; i < G::NS; ++i) P[i] = run_decay<true>(P[i]);
   float* const dst = p.seg + (int64_t)seg * 2 * p.batch * p.D_ * p.N;
   mine.store(p, dst, at.b, P);
   mine.store(p, dst + p.batch * p.D_ * p.N, at.b, Q);
@@ -351,7 +379,7 @@ __device__ __forceinline__ void store_segment(const SelArgs& p, const S& mine, c
 
 // A workgroup carries a group of channels through a segment of time, a tile of four waves by eight steps at a time.  MAPS:
 // only the segment's map is wanted; every wave then runs a quarter of the segment by itself, and their maps meet at the end.
-template <typename T, typename G, Mode MODE, bool GATED, bool PADDED>
+template <typename T, typename G, Mode MODE, bool GATED, Kind KIND>
 __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArgs p) {
   constexpr int E = G::E, SL = G::SL, NS = G::NS;
   __shared__ WaveLds<G> lds_all[kWaves];
@@ -360,7 +388,7 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
   WaveLds<G>& lds = lds_all[wave];
   const int seg = blockIdx.y;
   const At at = place(p, slab_of(blockIdx.x, gridDim.x), G::GROUP);
-  const Slots<G, PADDED> mine(p, at, lane);
+  const Slots<G, KIND != kFull> mine(p, at, lane);
   const int64_t state_size = p.batch * p.D_ * p.N;
 
   // the layout that memory is read and written in
@@ -376,9 +404,10 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
 
   const int live = (at.len + kTileSteps - 1) / kTileSteps;  // tiles that the row reaches
   const int first = seg * p.seg_tiles, last = min(first + p.seg_tiles, p.tiles), live_last = min(last, live);
-  float carry[NS], decay[NS];
+  double time = 0.0;  // of the wave's steps (kMaps)
+  float carry[NS];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) carry[i] = 0.0f, decay[i] = 1.0f;
+  for (int i = 0; i < NS; ++i) carry[i] = 0.0f;
   if (MODE == kWhole) {
     if (p.h0) mine.load(p, p.h0, at.b, carry);
     for (int s = 0; s < seg; ++s) {  // the segments before this one
@@ -386,8 +415,9 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
       mine.load(p, p.seg + (int64_t)s * 2 * state_size, at.b, P);
       mine.load(p, p.seg + (int64_t)(s * 2 + 1) * state_size, at.b, Q);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) carry[i] = fmaf(P[i], carry[i], Q[i]);
+      for (int i = 0; i < NS; ++i) carry[i] = apply_map<true>(P[i], Q[i], carry[i]);
     }
+    arrived(carry);
   }
 
   constexpr int kNext = MODE == kMaps ? kRun : kTileSteps;  // steps between a wave's runs
@@ -443,10 +473,11 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     // 2. the waves' maps
     float P[NS], h[NS] = {};
 #pragma unroll
-    for (int i = 0; i < NS; ++i) P[i] = run_decay(sum * A[i]);
+    for (int i = 0; i < NS; ++i) P[i] = run_decay<KIND == kGrowing>(sum * A[i]);
     if (MODE == kMaps) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) carry[i] = Q[i], decay[i] = fmaxf(decay[i] * P[i], 0x1p-126f);
+      for (int i = 0; i < NS; ++i) carry[i] = Q[i];
+      time += sum;
       wave_sync();
       continue;
     }
@@ -464,7 +495,7 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         h[i] = w == wave ? carry[i] : h[i];
-        carry[i] = fmaf(Pw[i], carry[i], Qw[i]);
+        carry[i] = apply_map<KIND == kGrowing>(Pw[i], Qw[i], carry[i]);
       }
     }
     // 3. the steps from where they start
@@ -486,8 +517,8 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     };
     // (Missing states are cleared at every step only by a wave that has something infinite.  16 x 1024 x 1024 channels x 10 states
     // bf16: 114 us, where every wave did it 130, without any of it 112; the backward pass, which always does, 340 and 327.)
-    if (PADDED && any_lane(odd))
-      steps(std::bool_constant<PADDED>());
+    if (KIND != kFull && any_lane(odd))
+      steps(std::bool_constant<KIND != kFull>());
     else
       steps(std::false_type());
     wave_sync();
@@ -505,7 +536,7 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
     wave_sync();
   }
   if (MODE == kMaps) {
-    store_segment<G, false>(p, mine, at, seg, lane, wave, maps[0][0], decay, carry);
+    store_segment<G, false>(p, mine, at, seg, lane, wave, maps[0][0], A, time, carry);
     return;
   }
   for (int tile = max(first, live_last); tile < last; ++tile, t += kTileSteps, out += out_step)  // past the row
@@ -569,7 +600,7 @@ struct BackLds {
 };
 
 // The tiles of a segment from the last to the first.  MAPS: only the segment's map of E is wanted, as above.
-template <typename T, typename G, Mode MODE, bool GATED, bool PADDED>
+template <typename T, typename G, Mode MODE, bool GATED, Kind KIND>
 __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) selective_backward_kernel(SelArgs p) {
   constexpr int SIDE = G::SIDE, E = G::E, SL = G::SL, NS = G::NS;
   __shared__ BackLds<G> lds_all[SIDE][kWaves];
@@ -588,7 +619,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
   const bool on = b_of < p.batch && group < p.groups;
   const int sides = alone ? 1 : p.groups - (group - side);  // that have a group, where they share a row
   const At at = place(p, on ? b_of * p.groups + group : p.units, G::GROUP);
-  const Slots<G, PADDED> mine(p, at, lane);
+  const Slots<G, KIND != kFull> mine(p, at, lane);
   const int64_t state_size = p.batch * p.D_ * p.N;
 
   // B and C of the lane's states, step r's at r * kCoefs.  Those of missing channels are zeros, as their u and dy are: an
@@ -625,9 +656,10 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
     for (int i = 0; i < SIDE; ++i) most = max(most, length(slab * SIDE + i));
   const int live = (most + kTileSteps - 1) / kTileSteps;
   const int first = seg * p.seg_tiles, last = min(first + p.seg_tiles, p.tiles), live_last = min(last, live);
-  float carry[NS], decay[NS], dA[NS];
+  double time = 0.0;
+  float carry[NS], dA[NS];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) carry[i] = dA[i] = 0.0f, decay[i] = 1.0f;
+  for (int i = 0; i < NS; ++i) carry[i] = dA[i] = 0.0f;
   if (MODE == kWhole) {
     if (p.d_hn) mine.load(p, p.d_hn, at.b, carry);
     for (int s = p.segs - 1; s > seg; --s) {  // the segments after this one
@@ -635,8 +667,9 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
       mine.load(p, p.seg + (int64_t)s * 2 * state_size, at.b, P);
       mine.load(p, p.seg + (int64_t)(s * 2 + 1) * state_size, at.b, Q);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) carry[i] = fmaf(P[i], carry[i], Q[i]);
+      for (int i = 0; i < NS; ++i) carry[i] = apply_map<true>(P[i], Q[i], carry[i]);
     }
+    arrived(carry);
   }
 
   constexpr int kNext = MODE == kMaps ? kRun : kTileSteps;  // steps between a wave's runs
@@ -744,10 +777,11 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
     // 2. the waves' maps
     float P[NS], e[NS] = {};
 #pragma unroll
-    for (int i = 0; i < NS; ++i) P[i] = run_decay(sum * A[i]);
+    for (int i = 0; i < NS; ++i) P[i] = run_decay<KIND == kGrowing>(sum * A[i]);
     if (MODE == kMaps) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) carry[i] = Qe[i], decay[i] = fmaxf(decay[i] * P[i], 0x1p-126f);
+      for (int i = 0; i < NS; ++i) carry[i] = Qe[i];
+      time += sum;
       wave_sync();
       continue;
     }
@@ -766,7 +800,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         e[i] = w == wave ? carry[i] : e[i];
-        carry[i] = fmaf(Pw[i], carry[i], Qw[i]);
+        carry[i] = apply_map<KIND == kGrowing>(Pw[i], Qw[i], carry[i]);
       }
     }
 #pragma unroll
@@ -775,7 +809,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
       map[w][0].get(lane, Pw);
       map[w][2].get(lane, Qw);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) h[i] = w < wave ? fmaf(Pw[i], h[i], Qw[i]) : h[i];
+      for (int i = 0; i < NS; ++i) h[i] = w < wave ? apply_map<KIND == kGrowing>(Pw[i], Qw[i], h[i]) : h[i];
     }
     lds_barrier();  // (the maps and the sums of the tile before have been read)
     mine.clear_missing(h), mine.clear_missing(e), mine.clear_missing(carry);
@@ -867,7 +901,7 @@ __global__ void __launch_bounds__(G::SIDE* kWaves* kWave, G::SIDE == 1 ? 3 : 2) 
     wave_sync();
   }
   if (MODE == kMaps) {
-    store_segment<G, true>(p, mine, at, seg, lane, wave, maps[side][0], decay, carry);
+    store_segment<G, true>(p, mine, at, seg, lane, wave, maps[side][0], A, time, carry);
     return;
   }
   for (int tile = max(first, live_last); tile < last; ++tile) {  // past the row
@@ -984,6 +1018,13 @@ SelWorkspace sel_workspace(int64_t batch, int64_t seq_len, int64_t channels, int
   return s;
 }
 
+// f(std::integral_constant of the kind of states), of which lanes hold `padded`.
+template <typename F>
+hipError_t with_kind(const SelArgs& p, int padded, F&& f) {
+  if (!p.softplus) return f(std::integral_constant<Kind, kGrowing>());
+  return p.N < padded ? f(std::integral_constant<Kind, kPadded>()) : f(std::integral_constant<Kind, kFull>());
+}
+
 template <typename T>
 hipError_t launch_sel_forward(const SelArgs& p, hipStream_t s) {
   return with_states(p.N, [&](auto sl, auto ns) {
@@ -991,20 +1032,19 @@ hipError_t launch_sel_forward(const SelArgs& p, hipStream_t s) {
     const dim3 block(kWaves * kWave);
     if (p.segs > 1) {
       const dim3 all_but_last((unsigned)p.units, p.segs - 1);
-      hipLaunchKernelGGL((selective_forward_kernel<T, G, kMaps, false, false>), all_but_last, block, 0, s, p);
+      hipLaunchKernelGGL((selective_forward_kernel<T, G, kMaps, false, kFull>), all_but_last, block, 0, s, p);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
-    const auto run = [&](auto gated, auto padded) {
+    return with_kind(p, G::NP, [&](auto kind) {
+      constexpr Kind KIND = decltype(kind)::value;
       const dim3 grid((unsigned)p.units, p.segs);
-      hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, decltype(gated)::value, decltype(padded)::value>), grid,
-                         block, 0, s, p);
+      if (p.z.p)
+        hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, true, KIND>), grid, block, 0, s, p);
+      else
+        hipLaunchKernelGGL((selective_forward_kernel<T, G, kWhole, false, KIND>), grid, block, 0, s, p);
       return hipGetLastError();
-    };
-    const auto of_states = [&](auto gated) {
-      return p.N < G::NP ? run(gated, std::true_type()) : run(gated, std::false_type());
-    };
-    return p.z.p ? of_states(std::true_type()) : of_states(std::false_type());
+    });
   });
 }
 
@@ -1039,15 +1079,14 @@ hipError_t launch_sel_backward(SelArgs p, void* d_A, void* d_B, void* d_C, void*
       const auto run = [&](auto gated) {
         constexpr bool GATED = decltype(gated)::value;
         if (p.segs > 1) {
-          hipLaunchKernelGGL((selective_backward_kernel<T, G, kMaps, GATED, false>), grid, block, 0, s, p);
+          hipLaunchKernelGGL((selective_backward_kernel<T, G, kMaps, GATED, kFull>), grid, block, 0, s, p);
           const hipError_t e2 = hipGetLastError();
           if (e2 != hipSuccess) return e2;
         }
-        if (p.N < G::NP)
-          hipLaunchKernelGGL((selective_backward_kernel<T, G, kWhole, GATED, true>), grid, block, 0, s, p);
-        else
-          hipLaunchKernelGGL((selective_backward_kernel<T, G, kWhole, GATED, false>), grid, block, 0, s, p);
-        return hipGetLastError();
+        return with_kind(p, G::NP, [&](auto kind) {
+          hipLaunchKernelGGL((selective_backward_kernel<T, G, kWhole, GATED, decltype(kind)::value>), grid, block, 0, s, p);
+          return hipGetLastError();
+        });
       };
       return p.z.p ? run(std::true_type()) : run(std::false_type());
     });

@@ -171,10 +171,10 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         h_t = exp(s_t A[d, n]) h_{t-1} + s_t u_t B_t[n]        y_t = sum_n C_t[n] h_t + D[d] u_t
 
     and out_t = y_t silu(z_t), or y_t without z [batch, time, channels].  A [channels, states] with 1 to 64 states, not
-    positive (it is a decay); D and dt_bias [channels], either may be missing; these three have u's type or float32 (all
-    the same), the others u's type.  Returns (out of u's shape and type, h_n [batch, channels, states] float32).  h0: the
-    state before the first step (default: zeros).  lengths: as for gated_scan; a row's h_n is the state after its last
-    step, its outputs are zero from there on.
+    positive: it is a decay (with softplus=False a step size may lie below zero, and the state grows).  D and dt_bias
+    [channels], either may be missing; these three have u's type or float32 (all the same), the others u's type.  Returns
+    (out of u's shape and type, h_n [batch, channels, states] float32).  h0: the state before the first step (default:
+    zeros).  lengths: as for gated_scan; a row's h_n is the state after its last step, its outputs are zero from there on.
 
     u, dt, z, B and C may have any batch and time strides (parts of projections' outputs).  Differentiable in all of
     them, A, D, dt_bias and h0, from both results.
