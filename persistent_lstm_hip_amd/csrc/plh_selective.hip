@@ -24,9 +24,11 @@
 //   3. the eight steps from there, with the outputs
 // so that an exponential is taken once although four times as many waves run as there are channels for.  (Two channels
 // by four states per thread read B and C half as often, and add up dB and dC in half the operations, but take twice the
-// registers: 8 x 2048 x 2048 channels x 16 states bf16 forward 256 -> 320 us, backward 886 -> 1770, with spills.)
-// At these sizes the forward kernel now takes 250 us, VALU busy 74% of the time, the backward one 605, 72%, and its sums
-// 62: 12 instructions per state and step forward, of which the formulas' own are 7, and 30 backward, of which they are 17.
+// registers: 8 x 2048 x 2048 channels x 16 states bf16 forward 256 -> 320 us, backward 886 -> 1770, with spills; measured
+// before the backward pass kept part of its values in LDS.)
+// At these sizes the forward kernel now takes 250 us, VALU busy 74% of the time, the backward one 605, 74%, and its sums 62.
+// Per state and step it issues 12 instructions forward, of which 5 are the formulas' and 2 those of them that two passes do (the
+// input's product and the recurrence); 30 backward, of which 13 and 4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -82,9 +84,9 @@ struct Geo {
   static constexpr int E = GROUP >= 8 ? GROUP / 8 : 1, F = NP >= 8 ? NP / 8 : 1;
   static_assert(kRun == 8, "eight steps by eight lanes");
   // Groups of a workgroup of the backward pass, whose dB and dC it adds up.  One leaves three workgroups per CU, with rows
-  // of their own pace, two save half of the partial sums' traffic, which grows with the states.  One and two, us: 16 states
-  // 8 x 2048 x 2048 bf16 772 and 758 with the sums' kernel, 128 x 1000 x 256 fp16 ragged 479 and 581; 32 states
-  // 4 x 2048 x 1024 bf16 467 and 415, 64 states 998 and 954.
+  // of their own pace, two save half of the partial sums' traffic, which grows with the states.  One and two, us of a
+  // training call less those of a forward one: 16 states 8 x 2048 x 2048 bf16 650 and 742, 128 x 1000 x 256 fp16 ragged 431
+  // and 580; 32 states 4 x 2048 x 1024 bf16 455 and 404, 64 states 1073 and 960.
   static constexpr int SIDE = SL == 4 ? 1 : 2;
 };
 
