@@ -49,6 +49,11 @@ class SelectiveScanBlock(nn.Module):
     def _inner(self, x: torch.Tensor):
         return self.inner(layer_norm(x, self.norm_weight, self.norm_bias)).chunk(2, -1)
 
+    def _filter(self, u: torch.Tensor):
+        """The convolution's weight and bias for u, in 32 bits where u is of another 16-bit type (under autocast)."""
+        w, b = self.conv_weight, self.conv_bias
+        return (w, b) if w.dtype in (u.dtype, torch.float32) else (w.float(), b.float())
+
     def _coefs(self, u: torch.Tensor):
         """What the scan of u takes beside it: dt, A, B, C, D."""
         dt, B, C = self.coefs(u).split([self.rank, self.states, self.states], -1)
@@ -62,7 +67,7 @@ class SelectiveScanBlock(nn.Module):
         u, z = self._inner(x)
         if before is not None:
             before = before.to(u.dtype)
-        u, before = causal_conv(u, self.conv_weight, self.conv_bias, before, lengths=lengths)
+        u, before = causal_conv(u, *self._filter(u), before, lengths=lengths)
         h, h_n = selective_scan(u, *self._coefs(u), z, h0, dt_bias=self.dt_bias.float(), lengths=lengths)
         p = self.dropout if self.training else 0.0
         if offset is None:
@@ -73,17 +78,20 @@ class SelectiveScanBlock(nn.Module):
         """One token x [batch, dim] -> y; both parts of the state are updated in place.  For inference."""
         u, z = self._inner(x)
         if state[0].dtype == torch.float32 and u.dtype != torch.float32:  # under autocast: it holds 16-bit inputs exactly
-            u, last = causal_conv_step(u, state[0].to(u.dtype), self.conv_weight, self.conv_bias)
+            u, last = causal_conv_step(u, state[0].to(u.dtype), *self._filter(u))
             state[0].copy_(last)
         else:
-            u, _ = causal_conv_step(u, state[0], self.conv_weight, self.conv_bias, inplace=True)
+            u, _ = causal_conv_step(u, state[0], *self._filter(u), inplace=True)
         dt, A, B, C, D = self._coefs(u)
         h, _ = selective_scan_step(u, dt, A, B, C, state[1], D, z, dt_bias=self.dt_bias.float(), inplace=True)
         return x + self.out(h)
 
     def initial_state(self, batch: int) -> State:
         w = self.conv_weight
-        return (torch.zeros(batch, w.size(1) - 1, w.size(0), dtype=self.inner.weight.dtype, device=w.device),
+        kind = self.inner.weight.dtype
+        if kind != torch.float32 and torch.is_autocast_enabled(w.device.type):  # (float32 holds either 16-bit type)
+            kind = torch.get_autocast_dtype(w.device.type)
+        return (torch.zeros(batch, w.size(1) - 1, w.size(0), dtype=kind, device=w.device),
                 torch.zeros(batch, w.size(0), self.states, dtype=torch.float32, device=w.device))
 
 

@@ -127,3 +127,25 @@ def test_gradients_through_a_given_state(gpu):
     for a, b in zip(got, want):
         assert a.dtype == torch.float32
         _close(a, b, torch.float16)
+
+
+@pytest.mark.parametrize("dtype,other", [(torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)])
+def test_a_model_of_the_other_16_bit_type(gpu, dtype, other):
+    _say(f"selective autocast {dtype} in {other}")
+    torch.manual_seed(8)
+    block = SelectiveScanBlock(32).cuda().eval()
+    x = torch.randn(2, 12, 32, device="cuda")
+    with torch.no_grad():
+        whole, _ = block(x)
+        block, x = block.to(dtype), x.to(dtype)
+        with torch.autocast("cuda", dtype=other):
+            state = block.initial_state(2)
+            assert state[0].dtype == other
+            y, handed = block(x[:, :8])
+            ys = [y]
+            for t in range(8, 12):
+                ys.append(block.step(x[:, t], handed).unsqueeze(1).to(dtype))
+            _close(torch.cat(ys, 1), whole, torch.bfloat16)
+            for t in range(12):
+                out = block.step(x[:, t], state)
+            _close(out, whole[:, -1], torch.bfloat16)
