@@ -352,8 +352,8 @@ int plh_causal_conv_backward(int dtype, int wdtype, const void* x, int64_t strid
  *                  pass needs
  * The step is seq_len = 1 without lengths, from h to h_n, which may be the same memory.
  * Limits: 1 <= states <= 64, channels <= 2^20, seq_len <= 2^30, batch * ceil(channels / 8) < 2^23 and, from 2^21 rows on,
- * <= 2^21, batch * seq_len * states <= 2^30; of the step batch * channels * lanes <= 2^32 - 256 with ceil(states / 4) lanes, rounded up
- * to a power of two.
+ * <= 2^21, batch * seq_len * states <= 2^30; of the step batch * channels * lanes <= 2^32 - 256 with ceil(states / 4)
+ * lanes, rounded up to a power of two.
  */
 typedef struct plh_selective_scan_args {
   int dtype, wdtype;

@@ -6,8 +6,8 @@
 // launch are one list of chunks, of which every workgroup has an equal run, so that many small tensors cost one launch
 // and no more than a chunk each.  Squares are summed in 64 bits: nothing between the smallest and the largest fp32 value
 // overflows or vanishes, and the conversion hides under the loads.  The workgroups' sums are added in a fixed order by
-// every workgroup of the second pass, which saves a launch in between (and a wait for one workgroup).  59 tensors of 0.51 G bf16
-// elements, us: to new tensors 573, in place 598, in place with the norm within the limit, where nothing is written, 184
+// every workgroup of the second pass, which saves a launch in between (and a wait for one workgroup).  59 tensors of 0.51 G
+// bf16 elements, us: to new tensors 573, in place 598, in place with the norm within the limit, where nothing is written, 184
 // (5.6 TB/s); 48 tensors of 0.47 M fp32 elements in place 20.
 #include <hip/hip_runtime.h>
 

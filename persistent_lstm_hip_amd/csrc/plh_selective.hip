@@ -27,8 +27,8 @@
 // registers: 8 x 2048 x 2048 channels x 16 states bf16 forward 256 -> 320 us, backward 886 -> 1770, with spills; measured
 // before the backward pass kept part of its values in LDS.)
 // At these sizes the forward kernel now takes 250 us, VALU busy 74% of the time, the backward one 605, 74%, and its sums 62.
-// Per state and step it issues 12 instructions forward, of which 5 are the formulas' and 2 those of them that two passes do (the
-// input's product and the recurrence); 30 backward, of which 13 and 4.
+// Per state and step it issues 12 instructions forward, of which 5 are the formulas' and 2 those of them that two passes do
+// (the input's product and the recurrence); 30 backward, of which 13 and 4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -158,9 +158,9 @@ __device__ __forceinline__ void softplus(float v, float& value, float& slope) {
 // leaves the state as it is, and 0 * inf would not.
 __device__ __forceinline__ float rate(float A) { return __builtin_elementwise_maximum(A * kOpLog2e, -3e38f); }
 
-// The map of a run of steps, h -> P h + Q, with P = 2^log2_decay.  Every step's own decay is positive, but their product may be
-// too small for fp32 (or, where step sizes are negative and the state grows, too large), and 0 * inf would be NaN where the steps
-// one after the other are not.  So P is held at 2^-126 at least, which leaves next to nothing of a state.  Where it may grow
+// The map of a run of steps, h -> P h + Q, with P = 2^log2_decay.  Every step's own decay is positive, but their product may
+// be too small for fp32 (or, where step sizes are negative and the state grows, too large), and 0 * inf would be NaN where the
+// steps one after the other are not.  So P is held at 2^-126 at least, which leaves next to nothing of a state.  Where it may grow
 // again, which it cannot with softplus, P is held as its square root (GROWS), which is in range down to P = 2^-252 and up to
 // 2^254: what lies beyond leaves no normal number of a normal one.  (8 x 2048 x 2048 channels x 16 states bf16 forward 236 us,
 // backward 667, with the root 240 and 673.)
@@ -517,8 +517,8 @@ __global__ void __launch_bounds__(kWaves* kWave) selective_forward_kernel(SelArg
         lds.y[r][lane / SL] = states_sum<SL>(y);  // (the same from all SL lanes, as below: a branch would part the steps)
       }
     };
-    // (Missing states are cleared at every step only by a wave that has something infinite.  16 x 1024 x 1024 channels x 10 states
-    // bf16: 114 us, where every wave did it 130, without any of it 112; the backward pass, which always does, 340 and 327.)
+    // (Missing states are cleared at every step only by a wave that has something infinite.  16 x 1024 x 1024 channels x 10
+    // states bf16: 114 us, where every wave did it 130, without any of it 112; the backward pass, which always does, 340 and 327.)
     if (KIND != kFull && any_lane(odd))
       steps(std::bool_constant<KIND != kFull>());
     else

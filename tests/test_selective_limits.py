@@ -30,7 +30,8 @@ def _args(batch, seq_len, channels, states):
 
 
 # lanes per channel, four states each
-@pytest.mark.parametrize("states,lanes", [(1, 1), (4, 1), (5, 2), (8, 2), (9, 4), (16, 4), (17, 8), (32, 8), (33, 16), (64, 16)])
+@pytest.mark.parametrize("states,lanes", [(1, 1), (4, 1), (5, 2), (8, 2), (9, 4), (16, 4), (17, 8), (32, 8), (33, 16),
+                                          (64, 16)])
 def test_a_step_has_fewer_threads_than_a_launch_holds(lib, states, lanes):
     def step(batch, channels):
         rc = lib.plh_selective_scan_step(_args(batch, 1, channels, states), ANY, None, ANY, None)
